@@ -59,6 +59,7 @@ extern "C" {
 #define IFR_PLAN_SPLIT_MERGE 0   /* split-KV partials + log-sum-exp merge   */
 #define IFR_PLAN_TOKEN_DIRECT 1  /* one item per token, finalised as acc/l */
 #define IFR_PLAN_TOKEN_MERGE 2   /* one item per token, one-segment merge  */
+#define IFR_PLAN_WINDOW 3        /* a plan of ifr_plan_window              */
 
 /* ---- status, version ---------------------------------------------------- */
 int32_t ifr_abi_version(void);
@@ -390,6 +391,88 @@ int32_t ifr_bq_attention_block_quant(const void* image_dev, const int64_t* info,
  * (0 when amax is 0).  The FWHT variant (apply_fwht=True) is not provided. */
 int32_t ifr_bq_block_quant(const void* src, void* x_i8, float* x_sa, int64_t cols,
                            int64_t block, int64_t seq_len, uint64_t stream);
+
+/* ---- attention with a window and sinks, and the 8-bit block-scaled cache -----
+ * No counterpart in the reference.  These operators use the softmax as defined,
+ * not the reference's biased exp, and their results do not depend on a worker
+ * capacity.  With the queries' positions p:
+ *   visible(p) = { j <= p : window == 0, or j > p - window, or j < sinks }
+ *   s_j = scale * q . k_j       o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)
+ * over j in visible(p), m = max_j s_j; sums and products in f32, the weights of
+ * a sum over v in bf16 (decode: two bf16 parts), o rounded once to bf16.  What
+ * a position holds that a query does not see does not enter its result, be it
+ * infinite or NaN.
+ *
+ * head_dim 128, 256 or 512; 1 to 16 q heads a kv head; pages of 32 rows or more.
+ * q and output [seq_len][num_q][head_dim] bf16, 16-byte aligned; caches
+ * [row][kv_stride] as elsewhere.
+ *
+ * ifr_plan_window (host only; no HIP call) plans a step once for all layers of
+ * the same heads.  The run table is that of a full-attention plan: page j of a
+ * run holds the positions from j * page_len.  Of it only pages with a visible
+ * position are read, so with a window the entries of the pages in between may
+ * be anything (-1, or pages that another run has taken over since).
+ * block_len: 0 for a bf16 cache; else the rows of a scale block of an 8-bit
+ * cache, a power of two in [16, page_len], every page starting at a block.
+ * image: ifr_plan_window_bytes of host memory, of which info[4] bytes are used;
+ * info[IFR_WINDOW_INFO_LEN]: as for ifr_plan_attention, but info[2] =
+ * IFR_PLAN_WINDOW, info[3] partial columns, info[14] prompt blocks, info[15]
+ * write blocks, info[16] sinks, info[17..19] num_q, num_kv, head_dim, info[20]
+ * block_len, info[21] workspace bytes of the attention; the rest is internal.
+ * The image also serves ifr_rope_cache_write and ifr_rms_norm_rope_cache_write
+ * (page_mask -1), and no other entry point above. */
+#define IFR_WINDOW_INFO_LEN 32
+int64_t ifr_plan_window_bytes(int64_t num_runs, int64_t num_rows, int64_t seq_len,
+                              int64_t block_len);
+int32_t ifr_plan_window(void* image, int64_t image_bytes, const int32_t* runs,
+                        int64_t num_runs, const int32_t* base_rows, int64_t num_rows,
+                        int64_t seq_len, int64_t window, int64_t sinks, int64_t page_len,
+                        int64_t cache_rows, int64_t num_q, int64_t num_kv,
+                        int64_t head_dim, int64_t block_len, int64_t* info);
+
+/* Attention over a bf16 cache that already holds the step's tokens.  workspace:
+ * device memory of info[21] bytes (null where that is 0), written before it is
+ * read in every call; calls that may overlap each need their own. */
+int32_t ifr_window_attention_bf16(const void* image_dev, const int64_t* info, const void* q,
+                                  const void* k_base, const void* v_base, void* output,
+                                  void* workspace, int64_t workspace_bytes, int64_t num_q,
+                                  int64_t num_kv, int64_t head_dim, int64_t kv_stride,
+                                  float scale, uint64_t stream);
+
+/* The 8-bit cache: codes [row][kv_stride] of 1 byte, OCP e4m3 or int8, and f32
+ * scales [row / block_len][num_kv], zero or a power of two; the value is code *
+ * scale. */
+#define IFR_KV8_E4M3 1
+#define IFR_KV8_INT8 2
+
+/* RoPE of q into q_out (which may be q_src) and of k_src, and the quantising
+ * write of the step's k and v at their slots.  Rotated k is quantised from f32.
+ * For each block of a page that the step writes to, and each kv head:
+ *   need = the smallest power of two with amax <= Q * need (Q = 448 or 127) over
+ *          the finite values that the step writes there, 0 if they are all 0,
+ *          2^-126 at least otherwise
+ *   scale = need if the step writes the block's first row; else max(need, the
+ *          scale it has), and where that grows, the rows before the step's first
+ *          become rounde(code * old / new) (e4m3: exact above its subnormals)
+ *   code = the value / scale, rounded to nearest even; infinities become the
+ *          largest code, NaN stays NaN in e4m3 and becomes 0 in int8
+ * Rows behind the step's tokens keep their bytes.  Refused where two of the
+ * step's runs write to the same rows.  half and pair_stride: multiples of 8. */
+int32_t ifr_kv8_cache_write(const void* image_dev, const int64_t* info, const void* q_src,
+                            const void* k_src, const void* v_src, void* q_out, void* k_cache,
+                            float* k_scale, void* v_cache, float* v_scale,
+                            const float* cos_table, const float* sin_table, int64_t num_q,
+                            int64_t num_kv, int64_t seq_len, int64_t half,
+                            int64_t pair_stride, int64_t head_dim, int64_t kv_stride,
+                            int64_t kv_format, uint64_t stream);
+
+/* ifr_window_attention_bf16 over that cache (window 0: full attention). */
+int32_t ifr_kv8_attention(const void* image_dev, const int64_t* info, const void* q,
+                          const void* k_base, const float* k_scale, const void* v_base,
+                          const float* v_scale, void* output, void* workspace,
+                          int64_t workspace_bytes, int64_t num_q, int64_t num_kv,
+                          int64_t head_dim, int64_t kv_stride, float scale,
+                          int64_t kv_format, uint64_t stream);
 
 #ifdef __cplusplus
 }

@@ -16,7 +16,10 @@ P_I64 = C.POINTER(C.c_int64)
 P_F32 = C.POINTER(C.c_float)
 
 INFO_LEN = 16
+WINDOW_INFO_LEN = 32
 PLAN_SPLIT_MERGE, PLAN_TOKEN_DIRECT, PLAN_TOKEN_MERGE = 0, 1, 2
+PLAN_WINDOW = 3
+KV8_FORMATS = {"e4m3": 1, "int8": 2}
 
 # name -> (restype, argtypes)
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -82,6 +85,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                             U64]),
     "ifr_gemm_cols_workspace_bytes": (I64, [I64, I64, I64]),
     "ifr_dispatch_gemm_cols": (I32, [VP, VP, VP, I64, I64, I64, VP, I64, U64]),
+    "ifr_plan_window_bytes": (I64, [I64, I64, I64, I64]),
+    "ifr_plan_window": (I32, [VP, I64, P_I32, I64, P_I32, I64, I64, I64, I64, I64, I64, I64,
+                              I64, I64, I64, P_I64]),
+    "ifr_window_attention_bf16": (I32, [VP, P_I64, VP, VP, VP, VP, VP, I64, I64, I64, I64, I64,
+                                        F32, U64]),
+    "ifr_kv8_cache_write": (I32, [VP, P_I64, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, I64, I64,
+                                  I64, I64, I64, I64, I64, I64, U64]),
+    "ifr_kv8_attention": (I32, [VP, P_I64, VP, VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, I64,
+                                F32, I64, U64]),
     # ---- host-side page state (include/inferno_host.h) ----
     "ifr_splitmix64": (U64, [U64]),
     "ifr_hash_token_block": (U64, [VP, I64, I64]),

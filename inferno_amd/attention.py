@@ -11,8 +11,9 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import P_I64, check, lib
-from .kv import FULL, SLIDING, AttentionPlan, KVRunTable, flash_partial_stride
+from ._lib import KV8_FORMATS, P_I64, check, lib
+from .kv import (FULL, SLIDING, AttentionPlan, KVRunTable, WindowPlan,
+                 flash_partial_stride)
 
 
 def _stream() -> int:
@@ -321,8 +322,114 @@ def dispatch_bq_block_quant(src, x_i8, x_sa, *, cols: int, block: int, seq_len: 
                                    _stream()))
 
 
+def window_workspace(plan: WindowPlan):
+    """f32 workspace of window_attention_bf16 and kv8_attention on this plan (None
+    if unneeded).  Calls on one stream may share it."""
+    import torch
+
+    n = plan.workspace_bytes
+    return torch.empty(n // 4, dtype=torch.float32, device=plan.device) if n else None
+
+
+def _buffer(plan: WindowPlan, name: str, t, numel: int, itemsize: int) -> int:
+    """The address of a contiguous buffer of at least numel elements on the plan's
+    device (the kernels see addresses alone)."""
+    if t.device != plan.device:
+        raise ValueError(f"{name} is on {t.device}, the plan on {plan.device}")
+    if t.element_size() != itemsize or not t.is_contiguous() or t.numel() < numel:
+        raise ValueError(f"{name} must be contiguous, of {itemsize}-byte elements and at least "
+                         f"{numel} of them (has {t.numel()} of {t.element_size()} bytes, "
+                         f"strides {tuple(t.stride())})")
+    return t.data_ptr()
+
+
+def _window_stream(plan: WindowPlan) -> int:
+    import torch
+
+    if plan.device.index != torch.cuda.current_device():
+        raise ValueError(f"the plan is on {plan.device}, the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+    return _stream()
+
+
+def _kv8_format(name: str) -> int:
+    if name not in KV8_FORMATS:
+        raise ValueError(f"kv_format must be one of {sorted(KV8_FORMATS)}, not {name!r}")
+    return KV8_FORMATS[name]
+
+
+def _workspace(plan: WindowPlan, workspace):
+    if workspace is None:
+        return None, 0
+    return _buffer(plan, "workspace", workspace, 0, 4), workspace.numel() * 4
+
+
+def _cache_numel(plan: WindowPlan, num_kv: int, head_dim: int, kv_stride: int) -> int:
+    return (plan.cache_rows - 1) * kv_stride + num_kv * head_dim
+
+
+def _scales_numel(plan: WindowPlan, num_kv: int) -> int:
+    return -(-plan.cache_rows // max(plan.block_len, 1)) * num_kv
+
+
+def window_attention_bf16(plan: WindowPlan, q, k_base, v_base, output, workspace, *, num_q: int,
+                          num_kv: int, head_dim: int, kv_stride: int, scale: float) -> None:
+    """Attention with a window and sinks (or over everything, window 0) over a bf16
+    paged cache that already holds the step's tokens: exact softmax of scale * q.k.
+    No counterpart in the reference."""
+    n = plan.seq_len * num_q * head_dim
+    cache = _cache_numel(plan, num_kv, head_dim, kv_stride)
+    ws, ws_bytes = _workspace(plan, workspace)
+    check(lib().ifr_window_attention_bf16(
+        plan.image.data_ptr(), plan.info_ptr, _buffer(plan, "q", q, n, 2),
+        _buffer(plan, "k_base", k_base, cache, 2), _buffer(plan, "v_base", v_base, cache, 2),
+        _buffer(plan, "output", output, n, 2), ws, ws_bytes, num_q, num_kv, head_dim, kv_stride,
+        scale, _window_stream(plan)))
+
+
+def dispatch_kv8_cache_write(plan: WindowPlan, q_src, k_src, v_src, q_out, k_cache, k_scale,
+                             v_cache, v_scale, cos_table, sin_table, *, num_q: int, num_kv: int,
+                             half: int, pair_stride: int, head_dim: int, kv_format: str,
+                             kv_stride: int | None = None) -> None:
+    """RoPE of q into q_out (q_src itself will do) and of k, and the quantising write of
+    the step's k and v into an 8-bit cache: codes [row][kv_stride] of kv_format "e4m3"
+    or "int8", power-of-two scales [row / block_len][num_kv].  The rules for scales,
+    older rows of a block and special values stand at ifr_kv8_cache_write
+    (include/inferno_hip.h).  No counterpart in the reference."""
+    stride = num_kv * head_dim if kv_stride is None else kv_stride
+    nq, nkv = plan.seq_len * num_q * head_dim, plan.seq_len * num_kv * head_dim
+    cache, scales = _cache_numel(plan, num_kv, head_dim, stride), _scales_numel(plan, num_kv)
+    table = (int(plan.info[13]) + 1) * half
+    check(lib().ifr_kv8_cache_write(
+        plan.image.data_ptr(), plan.info_ptr, _buffer(plan, "q_src", q_src, nq, 2),
+        _buffer(plan, "k_src", k_src, nkv, 2), _buffer(plan, "v_src", v_src, nkv, 2),
+        _buffer(plan, "q_out", q_out, nq, 2), _buffer(plan, "k_cache", k_cache, cache, 1),
+        _buffer(plan, "k_scale", k_scale, scales, 4),
+        _buffer(plan, "v_cache", v_cache, cache, 1),
+        _buffer(plan, "v_scale", v_scale, scales, 4),
+        _buffer(plan, "cos_table", cos_table, table, 4),
+        _buffer(plan, "sin_table", sin_table, table, 4), num_q, num_kv, plan.seq_len, half,
+        pair_stride, head_dim, stride, _kv8_format(kv_format), _window_stream(plan)))
+
+
+def kv8_attention(plan: WindowPlan, q, k_base, k_scale, v_base, v_scale, output, workspace, *,
+                  num_q: int, num_kv: int, head_dim: int, kv_stride: int, scale: float,
+                  kv_format: str) -> None:
+    """window_attention_bf16 over the 8-bit cache that dispatch_kv8_cache_write fills."""
+    n = plan.seq_len * num_q * head_dim
+    cache, scales = _cache_numel(plan, num_kv, head_dim, kv_stride), _scales_numel(plan, num_kv)
+    ws, ws_bytes = _workspace(plan, workspace)
+    check(lib().ifr_kv8_attention(
+        plan.image.data_ptr(), plan.info_ptr, _buffer(plan, "q", q, n, 2),
+        _buffer(plan, "k_base", k_base, cache, 1), _buffer(plan, "k_scale", k_scale, scales, 4),
+        _buffer(plan, "v_base", v_base, cache, 1), _buffer(plan, "v_scale", v_scale, scales, 4),
+        _buffer(plan, "output", output, n, 2), ws, ws_bytes, num_q, num_kv, head_dim, kv_stride,
+        scale, _kv8_format(kv_format), _window_stream(plan)))
+
+
 __all__ = [
-    "SLIDING", "FULL", "KVRunTable", "AttentionPlan", "partials_buffer",
+    "SLIDING", "FULL", "KVRunTable", "AttentionPlan", "WindowPlan", "window_workspace",
+    "window_attention_bf16", "dispatch_kv8_cache_write", "kv8_attention", "partials_buffer",
     "dispatch_rope_cache_write", "attention_bf16", "flash_partials_bf16",
     "merge_flash_partials", "dispatch_sliding_attention",
     "dispatch_full_attention", "dispatch_copy_jobs", "dispatch_gather_rows",

@@ -433,10 +433,12 @@ int32_t plan_impl(int32_t* img, int64_t img_words, const int32_t* runs,
   return ok();
 }
 
-int32_t check_info(const int64_t* info) {
+// window_too: a window plan will do as well (the bf16 appends read its run table, page
+// table and token -> run map alone).
+int32_t check_info(const int64_t* info, bool window_too = false) {
   if (!info) return fail(IFR_EINVAL, "null info");
   if (info[0] < 0 || info[1] < 0 || info[0] > INT32_MAX || info[1] > INT32_MAX ||
-      info[2] < 0 || info[2] > 2 || info[5] <= 0 || info[7] < 0 || info[7] > 30)
+      info[2] < 0 || info[2] > (window_too ? IFR_PLAN_WINDOW : 2) || info[5] <= 0 || info[7] < 0 || info[7] > 30)
     return fail(IFR_EINVAL, "info does not describe a plan");
   return IFR_OK;
 }
@@ -619,7 +621,7 @@ int32_t ifr_rope_cache_write(const void* image_dev, const int64_t* info,
                              int64_t page_mask, int64_t seq_len, int64_t half,
                              int64_t pair_stride, int64_t head_dim,
                              uint64_t stream) {
-  int32_t st = check_info(info);
+  int32_t st = check_info(info, true);
   if (st) return st;
   if (seq_len != info[5]) return fail(IFR_EINVAL, "seq_len differs from the plan");
   if (!image_dev || !q || !k_src || !v_src || !k_cache || !v_cache || !cos_table || !sin_table)
@@ -670,7 +672,7 @@ int32_t ifr_rms_norm_rope_cache_write(const void* image_dev, const int64_t* info
                                       int64_t seq_len, int64_t half, int64_t pair_stride,
                                       int64_t head_dim, float sqrt_n, float n_eps,
                                       uint64_t stream) {
-  int32_t st = check_info(info);
+  int32_t st = check_info(info, true);
   if (st) return st;
   if (seq_len != info[5]) return fail(IFR_EINVAL, "seq_len differs from the plan");
   if (!image_dev || !q || !k_src || !v_src || !k_cache || !v_cache || !cos_table ||

@@ -199,6 +199,43 @@ hipError_t launch_bq_attn_prep(const int32_t* image_dev, int seq_len,
                                int head_dim, int rope_half, int pair_stride,
                                float sqrt_n, float n_eps, hipStream_t stream);
 
+// Attention with a window and sinks, and over 8-bit block-scaled caches (window_api.hip
+// plans and checks; formats, items and units as in window.hpp).
+struct WindowArgs {
+  const int32_t* image;
+  const void *q, *k, *v;
+  const float *k_scale, *v_scale;  // [row >> block_shift][num_kv]
+  void* out;
+  float* partials;  // a column of head_dim values for each (split, kv head, token, q head)
+  float* sums;      // and its maximum and sum
+  int64_t kv_stride;
+  int num_q, num_kv, gqa;
+  int shift, row_mask, block_shift;
+  int window, sinks;
+  float scale_log2;
+};
+hipError_t launch_window_rows(const WindowArgs& a, int format, int head_dim, int off_items,
+                              int64_t num_items, int heads_per_group, hipStream_t stream);
+hipError_t launch_window_prompts(const WindowArgs& a, int format, int head_dim, int off_items,
+                                 int64_t num_items, hipStream_t stream);
+hipError_t launch_window_merge(const WindowArgs& a, int head_dim, int off_units,
+                               int64_t num_units, hipStream_t stream);
+
+// RoPE and the quantising write into an 8-bit block-scaled cache (kv8_write.hip).
+struct Kv8WriteArgs {
+  const int32_t* image;
+  const void *q, *k, *v;
+  void *q_out, *k_cache, *v_cache;
+  float *k_scale, *v_scale;
+  const float *cos_table, *sin_table;
+  int64_t kv_stride;
+  int num_q, num_kv, seq_len;
+  int half, pair_stride, block_shift;
+  int off_writes;
+  int64_t num_writes;
+};
+hipError_t launch_kv8_write(const Kv8WriteArgs& a, int format, int head_dim, hipStream_t stream);
+
 // Copy chunks: int64 [n][4] = {src_off, dst_off, bytes, 0}.
 hipError_t launch_copy_chunks(void* arena, const int64_t* chunks_dev, int num_chunks,
                               hipStream_t stream);

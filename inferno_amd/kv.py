@@ -13,7 +13,7 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from ._lib import INFO_LEN, P_I32, P_I64, check, lib
+from ._lib import INFO_LEN, P_I32, P_I64, WINDOW_INFO_LEN, check, lib
 
 SLIDING, FULL = 0, 1
 
@@ -119,3 +119,46 @@ class AttentionPlan:
         off = int(self.host[12])
         n = int(self.info[1])
         return self.host[off:off + 4 * n].reshape(n, 4)[:, :3].copy()
+
+
+class WindowPlan:
+    """A step planned for window_attention_bf16, kv8_attention and
+    dispatch_kv8_cache_write (ifr_plan_window), uploaded to the device; every
+    layer of the step with these heads shares it.
+
+    table: the run table of a full-attention plan.  Only pages that hold a
+    position some query sees are read, so with a window the base rows of the
+    pages in between may be anything (-1).
+    window: positions that a query sees, its own included; 0 for all earlier ones.
+    sinks: first positions that stay visible beside the window.
+    block_len: 0 for a bf16 cache, else the rows of a scale block of an 8-bit one.
+
+    It also serves dispatch_rope_cache_write and
+    dispatch_rms_norm_rope_cache_write, which append to a bf16 cache.
+    """
+
+    def __init__(self, table: KVRunTable, seq_len: int, *, window: int = 0, sinks: int = 0,
+                 page_len: int, cache_rows: int, num_q: int, num_kv: int, head_dim: int,
+                 block_len: int = 0, device=None) -> None:
+        import torch
+
+        runs, rows = table.arrays()
+        nbytes = int(lib().ifr_plan_window_bytes(runs.shape[0], rows.shape[0], max(seq_len, 0),
+                                                 max(block_len, 0)))
+        self.host = np.zeros(max(nbytes // 4, 16), dtype=np.int32)
+        self.info = (C.c_int64 * WINDOW_INFO_LEN)()
+        check(lib().ifr_plan_window(
+            self.host.ctypes.data, self.host.nbytes, runs.ctypes.data_as(P_I32), runs.shape[0],
+            rows.ctypes.data_as(P_I32), rows.shape[0], seq_len, window, sinks, page_len,
+            cache_rows, num_q, num_kv, head_dim, block_len, self.info))
+        self.info_ptr = C.cast(self.info, P_I64)
+        used = int(self.info[4]) // 4
+        dev = device if device is not None else torch.device("cuda")
+        self.image = torch.from_numpy(self.host[:used].copy()).to(dev)
+        self.device = self.image.device
+        self.seq_len = seq_len
+        self.window, self.sinks = window, sinks
+        self.page_len, self.cache_rows, self.block_len = page_len, cache_rows, block_len
+        self.page_mask, self.page_shift = -1, pow2_shift(page_len)
+        self.num_q, self.num_kv, self.head_dim = num_q, num_kv, head_dim
+        self.workspace_bytes = int(self.info[21])
