@@ -98,7 +98,8 @@ __device__ __forceinline__ f32x4_t add_infinities(f32x4_t acc, const Parts& v, b
 
 // Whether a query at position p sees position j.
 __device__ __forceinline__ bool sees(int p, int j, int window, int sinks) {
-  return j <= p && (window == 0 || j > p - window || j < sinks);
+  const int before = window == 0 ? -1 : p - window;  // no short circuits: they would be branches
+  return (j <= p) & ((j > before) | (j < sinks));
 }
 // 1 for each of a lane's eight positions of a tile that a query at p sees, as P^T lies.
 __device__ __forceinline__ bf16x8_t seen_ones(int p, int pos0, int g, int window, int sinks) {

@@ -26,30 +26,96 @@ namespace {
 
 using namespace window;
 using prefill::lds_barrier;
+using prefill::raw_max;
 using prefill::load_lds2;
 using prefill::load_lds4;
 using prefill::lds_s16x4_t;
 using prefill::s16x4_t;
 using prefill::wait_loads;
 
-constexpr float kSlack = 8.0f;  // how far scores may pass the maximum in use, in powers of two
+// One 1 KiB load into LDS (see load_lds4).
+__device__ __forceinline__ void load_lds1(const char* base, uint32_t off, const uint8_t* lds) {
+  uint32_t m0;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
+      "global_load_lds_dwordx4 %2, %3\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(m0)
+      : "s"(prefill::lds_addr(lds)), "v"(off), "s"(base)
+      : "memory");
+}
+__device__ __forceinline__ float max4(const float* v) { return raw_max(prefill::max3_raw(v[0], v[1], v[2]), v[3]); }
 
+// A wave's sums, 16x16 blocks of O^T, in accumulation registers from the first product to
+// the last.  Held as ordinary values, the compiler moves them between the two halves of the
+// register file for every tile, as the rare multiplication by a correction and the store
+// are VALU work; so all that touches them is written as instructions here.  The compiler
+// does not know that these are MFMAs: what VALU instructions wrote is read two wait states
+// later at the earliest (the s_nop 1 ahead of each run of them), and the sums are read
+// behind accs_settled().
+__device__ __forceinline__ void acc_zero(f32x4_t& acc) {
+  const u32x4_t none = u32x4_t{0u, 0u, 0u, 0u};
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %1, 0" : "=a"(acc) : "v"(none));
+}
+__device__ __forceinline__ void acc_mfma(f32x4_t& acc, bf16x8_t x, bf16x8_t y) {
+  asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(x), "v"(y));
+}
+__device__ __forceinline__ void accs_settled() { asm volatile("s_nop 15\n\ts_nop 15"); }
+// Four blocks to ordinary registers, and back, over 4 KiB of LDS that the wave has to
+// itself (at: this lane's 16 bytes).
+__device__ __forceinline__ void accs_out(f32x4_t* v, const f32x4_t& a0, const f32x4_t& a1, const f32x4_t& a2,
+                                         const f32x4_t& a3, uint32_t at) {
+  asm volatile(
+      "ds_write_b128 %4, %5\n\tds_write_b128 %4, %6 offset:1024\n\t"
+      "ds_write_b128 %4, %7 offset:2048\n\tds_write_b128 %4, %8 offset:3072\n\t"
+      "s_waitcnt lgkmcnt(0)\n\t"
+      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\t"
+      "ds_read_b128 %2, %4 offset:2048\n\tds_read_b128 %3, %4 offset:3072\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+      : "v"(at), "a"(a0), "a"(a1), "a"(a2), "a"(a3)
+      : "memory");
+}
+__device__ __forceinline__ void accs_in(f32x4_t& a0, f32x4_t& a1, f32x4_t& a2, f32x4_t& a3, const f32x4_t* v,
+                                        uint32_t at) {
+  asm volatile(
+      "ds_write_b128 %4, %5\n\tds_write_b128 %4, %6 offset:1024\n\t"
+      "ds_write_b128 %4, %7 offset:2048\n\tds_write_b128 %4, %8 offset:3072\n\t"
+      "s_waitcnt lgkmcnt(0)\n\t"
+      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\t"
+      "ds_read_b128 %2, %4 offset:2048\n\tds_read_b128 %3, %4 offset:3072\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&a"(a0), "=&a"(a1), "=&a"(a2), "=&a"(a3)
+      : "v"(at), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3])
+      : "memory");
+}
+
+constexpr float kSlack = 24.0f;  // how far scores may pass the maximum in use, in powers of two
+
+// One block.  False if a sum came out that is not finite: the block is then done again with
+// kCareful, which stores over it (two functions, so that the registers of one do not weigh
+// on the other).
 template <int kD, int kFormat>
-__global__ __launch_bounds__(64 * prompt_waves(kD)) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void window_prompt_kernel(const WindowArgs a, int off_items) {
-  constexpr int kWaves = prompt_waves(kD);
-  constexpr int kNc = 512 / kD;                 // column tiles of a wave
-  constexpr int kRowBytes = 2 * kD;             // of a tile row in LDS
-  constexpr int kTileBytes = kTileKeys * kRowBytes;
+struct Prompt {
+  static constexpr int kNc = prompt_col_tiles(kD);        // column tiles of a wave
+  static constexpr int kRowBytes = 2 * kD;                // of a tile row in LDS
+  static constexpr int kTileBytes = kTileKeys * kRowBytes;
+  // bf16: two tiles of K and V.  8-bit: one, and behind it the codes of the next.
+  static constexpr int kTiles = kFormat == kBf16 ? 4 * kTileBytes : 3 * kTileBytes;
+  static constexpr int kLds = kTiles + kPromptWaves * 4096;  // and what accs_out and accs_in use
+};
+
+template <int kD, int kFormat, bool kCareful>
+__device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items, uint8_t* lds, int* odd_flag) {
+  using P = Prompt<kD, kFormat>;
+  constexpr int kWaves = kPromptWaves;
+  constexpr int kNc = P::kNc, kRowBytes = P::kRowBytes, kTileBytes = P::kTileBytes;
   constexpr int kSteps = kD / 32, kBlocks = kD / 16;
-  constexpr int kWaveRows = kTileKeys / kWaves; // rows that a wave stages
-  constexpr int kLoads = kWaveRows * kRowBytes / 1024;
-  constexpr int kRowLanes = kRowBytes / 16;     // lanes of a row in one staging load
-  constexpr int kCodes = kTileKeys * kD / (64 * kWaves);  // 8-bit: codes of a thread
-  static_assert(kFormat != kBf16 || kLoads == 4 || kLoads == 2, "a staging load of this count");
-  __shared__ __align__(16) uint8_t kbuf[2 * kTileBytes];
-  __shared__ __align__(16) uint8_t vbuf[2 * kTileBytes];
-  __shared__ int again;
+  constexpr int kEsz = elt_bytes(kFormat);
+  constexpr int kStageBytes = kTileKeys * kD * kEsz;      // of K, or V, as it comes from the cache
+  constexpr int kLoads = kStageBytes / kWaves / 1024;     // 1 KiB loads of a wave
+  constexpr int kRowLanes = kD * kEsz / 16;               // lanes of a row in one of them
+  constexpr bool kMayFail = !kCareful && kFormat != kInt8;  // int8 codes are finite
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -64,22 +130,21 @@ void window_prompt_kernel(const WindowArgs a, int off_items) {
 
   // Columns; those past the last token repeat it and are not stored.
   const int wave_col = wave * 16 * kNc;
-  const bool wave_live = wave_col / a.gqa < ntok;
   const int wp0 = p0 + min(wave_col / a.gqa, ntok - 1);  // the wave's first and last position
   const int wp1 = p0 + min((wave_col + 16 * kNc - 1) / a.gqa, ntok - 1);
+  auto column = [&](int n, bool* live) {  // the row of q and of the output
+    const int col = wave_col + 16 * n + c;
+    const int tok = col / a.gqa;
+    *live = tok < ntok;
+    return static_cast<int64_t>(t0 + min(tok, ntok - 1)) * a.num_q + h * a.gqa + (*live ? col - tok * a.gqa : 0);
+  };
   int pos_of[kNc];
-  int64_t q_row[kNc];
-  bool live[kNc];
   u32x4_t qf[kNc][kSteps];
 #pragma unroll
   for (int n = 0; n < kNc; ++n) {
-    const int col = wave_col + 16 * n + c;
-    const int tok = col / a.gqa;
-    live[n] = tok < ntok;
-    const int tk = min(tok, ntok - 1);
-    pos_of[n] = p0 + tk;
-    q_row[n] = static_cast<int64_t>(t0 + tk) * a.num_q + h * a.gqa + (live[n] ? col - tok * a.gqa : 0);
-    const uint16_t* qr = static_cast<const uint16_t*>(a.q) + q_row[n] * kD + 8 * g;
+    bool live;
+    const uint16_t* qr = static_cast<const uint16_t*>(a.q) + column(n, &live) * kD + 8 * g;
+    pos_of[n] = p0 + min((wave_col + 16 * n + c) / a.gqa, ntok - 1);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) qf[n][s] = *reinterpret_cast<const u32x4_t*>(qr + 32 * s);
   }
@@ -91,19 +156,17 @@ void window_prompt_kernel(const WindowArgs a, int off_items) {
   auto tile_pos = [&](int vt) { return kTileKeys * (vt < span.n_sink ? vt : vt - span.n_sink + span.first); };
 
   // ---- staging ----
-  // bf16: load i of a wave moves its rows i * 64 / kRowLanes + lane / kRowLanes; LDS is
-  // filled in order, so the swizzle is in the chunk that a lane fetches.
+  // Load i of a wave moves its rows i * 64 / kRowLanes + lane / kRowLanes of the tile.  LDS
+  // is filled in order, so bf16's swizzle is in the chunk that a lane fetches.
   // Rows that no query of the block sees: K's scores are masked, V's row is another one
   // that is seen (its weights are 0).
-  auto stage_bf16 = [&](int vt, int buf) {
-    const int pos0 = tile_pos(vt);
-    const int64_t row = tile_row(rows, pos0, a.shift, a.row_mask);
-    const int w_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
+  const int w_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
+  auto stage = [&](int pos0, int64_t row, uint8_t* kd, uint8_t* vd) {
     const bool unseen = pos0 + kTileKeys - 1 > p1 || (pos0 < w_lo && pos0 + kTileKeys - 1 >= a.sinks);
     uint32_t ko[kLoads], vo[kLoads];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int r = wave * kWaveRows + i * (64 / kRowLanes) + lane / kRowLanes;
+      const int r = (wave * kLoads + i) * (64 / kRowLanes) + lane / kRowLanes;
       const uint32_t x = lane % kRowLanes;
       int rv = r;
       if (unseen) {
@@ -111,92 +174,88 @@ void window_prompt_kernel(const WindowArgs a, int off_items) {
         if (j > p1) rv = p1 - pos0;
         else if (j < w_lo && j >= a.sinks) rv = (w_lo < pos0 + kTileKeys ? w_lo : a.sinks - 1) - pos0;
       }
-      const uint32_t shift = 1024u * (3 - i);  // the instruction's offset counts on both sides
-      ko[i] = static_cast<uint32_t>(r) * rb32 + 16u * (x ^ (r & 15)) + shift;
-      vo[i] = static_cast<uint32_t>(rv) * rb32 + 16u * (x ^ (2 * (r & 7))) + shift;
+      const uint32_t both = 1024u * ((kLoads < 4 ? 1 : 3) - (i & 3));  // the instruction's offset counts on both sides
+      ko[i] = static_cast<uint32_t>(r) * rb32 + 16u * (kFormat == kBf16 ? x ^ (r & 15) : x) + both;
+      vo[i] = static_cast<uint32_t>(rv) * rb32 + 16u * (kFormat == kBf16 ? x ^ (2 * (r & 7)) : x) + both;
     }
-    const char* kt = kb + row * row_bytes - 3072;
-    const char* vt_ = vb + row * row_bytes - 3072;
-    uint8_t* kd = kbuf + buf * kTileBytes + wave * kWaveRows * kRowBytes;
-    uint8_t* vd = vbuf + buf * kTileBytes + wave * kWaveRows * kRowBytes;
-    if constexpr (kLoads == 4) {
-      load_lds4(kt, ko[0], ko[1], ko[2], ko[3], kd);
-      load_lds4(vt_, vo[0], vo[1], vo[2], vo[3], vd);
-    } else {
-      load_lds2(kt, ko[0], ko[1], kd);
-      load_lds2(vt_, vo[0], vo[1], vd);
-    }
-  };
-  // 8-bit: a thread's kCodes codes of one row, to registers and later to LDS.
-  constexpr int kRowThreads = kD / kCodes;
-  const int sr = threadIdx.x / kRowThreads, sx = threadIdx.x % kRowThreads;
-  u32x4_t kc[kCodes / 16], vc[kCodes / 16];
-  auto fetch_codes = [&](int vt) {
-    const int pos0 = tile_pos(vt);
-    const int64_t row = tile_row(rows, pos0, a.shift, a.row_mask);
-    const uint32_t off = static_cast<uint32_t>(sr) * rb32 + static_cast<uint32_t>(kCodes) * sx;
-    const char* kt = kb + row * row_bytes;
-    const char* vt_ = vb + row * row_bytes;
+    const char* kt = kb + row * row_bytes - 1024 * (kLoads < 4 ? 1 : 3);
+    const char* vt = vb + row * row_bytes - 1024 * (kLoads < 4 ? 1 : 3);
+    kd += wave * kLoads * 1024;
+    vd += wave * kLoads * 1024;
+    if constexpr (kLoads >= 4) {
 #pragma unroll
-    for (int i = 0; i < kCodes / 16; ++i) {
-      kc[i] = *reinterpret_cast<const u32x4_t*>(kt + off + 16 * i);
-      vc[i] = *reinterpret_cast<const u32x4_t*>(vt_ + off + 16 * i);
-    }
-  };
-  auto store_codes = [&](int vt, int buf) {
-    const bool seen = any_seen(p0, p1, tile_pos(vt) + sr, 1, a.window, a.sinks);
-    uint8_t* kd = kbuf + buf * kTileBytes + sr * kRowBytes;
-    uint8_t* vd = vbuf + buf * kTileBytes + sr * kRowBytes;
-#pragma unroll
-    for (int i = 0; i < kCodes / 16; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int x = sx * (kCodes / 8) + 2 * i + e;
-        const u32x2_t k0 = codes4_bf16<kFormat>(kc[i][2 * e]), k1 = codes4_bf16<kFormat>(kc[i][2 * e + 1]);
-        const u32x2_t v0 = codes4_bf16<kFormat>(seen ? vc[i][2 * e] : 0u), v1 = codes4_bf16<kFormat>(seen ? vc[i][2 * e + 1] : 0u);
-        *reinterpret_cast<u32x4_t*>(kd + 16 * (x ^ (sr & 15))) = u32x4_t{k0[0], k0[1], k1[0], k1[1]};
-        *reinterpret_cast<u32x4_t*>(vd + 16 * (x ^ (2 * (sr & 7)))) = u32x4_t{v0[0], v0[1], v1[0], v1[1]};
+      for (int i = 0; i < kLoads; i += 4) {
+        load_lds4(kt, ko[i], ko[i + 1], ko[i + 2], ko[i + 3], kd + 1024 * i);
+        load_lds4(vt, vo[i], vo[i + 1], vo[i + 2], vo[i + 3], vd + 1024 * i);
       }
+    } else if constexpr (kLoads == 2) {
+      load_lds2(kt, ko[0], ko[1], kd);
+      load_lds2(vt, vo[0], vo[1], vd);
+    } else {
+      static_assert(kLoads == 1);
+      load_lds1(kt + 1024, ko[0] - 1024, kd);
+      load_lds1(vt + 1024, vo[0] - 1024, vd);
+    }
+  };
+  // 8-bit: the staged codes become bf16 rows.  A thread takes 16 codes at a time.
+  uint8_t* codes = lds + 2 * kTileBytes;
+  auto convert = [&]() {
+    constexpr int kTurns = kStageBytes / 16 / (64 * kWaves);
+    u32x4_t w[2][kTurns];
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i)
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+        w[v][i] = *reinterpret_cast<const u32x4_t*>(codes + v * kStageBytes + 16 * (threadIdx.x + 64 * kWaves * i));
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const int at = threadIdx.x + 64 * kWaves * i;
+      const int r = at / kRowLanes, x = 2 * (at % kRowLanes);
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const u32x2_t y = codes4_bf16<kFormat>(w[v][i][2 * e]), z = codes4_bf16<kFormat>(w[v][i][2 * e + 1]);
+          *reinterpret_cast<u32x4_t*>(lds + v * kTileBytes + r * kRowBytes + 16 * ((x + e) ^ (v ? 2 * (r & 7) : r & 15))) =
+              u32x4_t{y[0], y[1], z[0], z[1]};
+        }
+    }
   };
 
+  const uint32_t own = prefill::lds_addr(lds + P::kTiles + 4096 * wave + 16 * lane);
+
   // ---- LDS reads ----
-  // K fragment of half tile u, step s: chunk 4 s + g of row 16 u + c.
-  int k_at[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) k_at[i] = c * kRowBytes + 16 * ((4 * i + g) ^ c);
-  // V^T fragment of dims 16 b ..: rows 4 g + c / 4 of both halves, 8 bytes at dim 4 (c % 4).
-  int v_at[8];
-  {
-    const int r = 4 * g + (c >> 2);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v_at[i] = r * kRowBytes + 16 * ((2 * i + ((c & 3) >> 1)) ^ (2 * (r & 7))) + 8 * (c & 1);
-  }
+  // K fragment of half tile u, step s: chunk 4 s + g of row 16 u + c, that is k_at ^ 64 s.
+  // V^T fragment of dims 16 b ..: rows 4 g + c / 4 of both halves, 8 bytes at dim 4 (c % 4),
+  // that is v_at ^ 32 b.
+  const int k_at = c * kRowBytes + 16 * (g ^ c);
+  const int v_row = 4 * g + (c >> 2);
+  const int v_at = v_row * kRowBytes + 16 * (((c & 3) >> 1) ^ (2 * (v_row & 7))) + 8 * (c & 1);
 
   float m[kNc], l[kNc];
   f32x4_t acc[kBlocks][kNc];
 
-  // careful: the second walk of a block whose first one ended with a sum that is not finite.
-  auto compute = [&](auto careful, int vt, int buf) {
-    constexpr bool kCareful = decltype(careful)::value;
-    const int pos0 = tile_pos(vt);
-    if (!wave_live || !any_seen(wp0, wp1, pos0, kTileKeys, a.window, a.sinks)) return;  // wave-uniform
-    const bool masked = !all_seen(wp0, wp1, pos0, kTileKeys, a.window, a.sinks);
-    float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f};
+  // No wave leaves out a tile that none of its columns sees: the others keep the block
+  // there anyway, and the branch around the accumulators would cost a copy of them.
+  // ---- a tile: scores of the K at LDS kt, then weights and sums over the V at vt ----
+  constexpr int kAhead = 4;  // fragments that LDS reads run ahead of their MFMAs
+  float sc[kNc][8], cs[2], vs[2], top[kNc];
+  // True if some column's maximum has to be moved first.
+  auto scores = [&](int pos0, int64_t row, const uint8_t* kt) {
+    const bool masked = !all_seen(wp0, wp1, pos0, kTileKeys, a.window, a.sinks);  // wave-uniform
+    cs[0] = cs[1] = a.scale_log2;
+    vs[0] = vs[1] = 1.0f;
     if constexpr (kFormat != kBf16) {
-      const int64_t row = tile_row(rows, pos0, a.shift, a.row_mask);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        ks[u] = vs[u] = 0.0f;
-        if (!masked || any_seen(wp0, wp1, pos0 + 16 * u, 16, a.window, a.sinks)) {
+        cs[u] = vs[u] = 1.0f;  // of a half that the block does not see
+        if (any_seen(p0, p1, pos0 + 16 * u, 16, a.window, a.sinks)) {
           const int64_t s = ((row + 16 * u) >> a.block_shift) * a.num_kv + h;
-          ks[u] = sload_f32(a.k_scale + s);
+          cs[u] = a.scale_log2 * sload_f32(a.k_scale + s);
           vs[u] = sload_f32(a.v_scale + s);
         }
       }
     }
-    const uint8_t* kt = kbuf + buf * kTileBytes;
-    const uint8_t* vt_ = vbuf + buf * kTileBytes;
     f32x4_t s4[2][kNc];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -206,41 +265,90 @@ void window_prompt_kernel(const WindowArgs a, int off_items) {
     for (int s = 0; s < kSteps; ++s)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kt + k_at[s & 3] + (s >> 2) * 256 + u * 16 * kRowBytes);
+        const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kt + (k_at ^ (64 * (s & 3))) + (s >> 2) * 256 + u * 16 * kRowBytes);
 #pragma unroll
         for (int n = 0; n < kNc; ++n)
           s4[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, __builtin_bit_cast(bf16x8_t, qf[n][s]), s4[u][n], 0, 0, 0);
       }
+    // Left alone, the scheduler puts all reads first and runs out of registers.
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < 2 * kSteps - kAhead; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, kNc, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, kAhead * kNc, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    // The maxima below are taken by instructions that the compiler does not look into, so
+    // it puts no wait states between them and the MFMAs.
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int n = 0; n < kNc; ++n) asm volatile("" : "+v"(s4[u][n]));
+    asm volatile("s_nop 15");
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int n = 0; n < kNc; ++n) {
+        asm volatile("" : "+v"(s4[u][n]));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[n][4 * u + r] = s4[u][n][r];
+      }
+    if (masked) {
+      asm volatile("");  // keeps this a branch: few tiles take it
+#pragma unroll
+      for (int n = 0; n < kNc; ++n)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float& x = sc[n][j];
+          x = sees(pos_of[n], pos0 + 16 * (j >> 2) + 4 * g + (j & 3), a.window, a.sinks) ? x : -INFINITY;
+        }
+    }
+    bool move = false;
+#pragma unroll
+    for (int n = 0; n < kNc; ++n) {
+      top[n] = prefill::groups_max(raw_max(max4(sc[n]) * cs[0], max4(sc[n] + 4) * cs[1]));
+      move |= top[n] > m[n] + kSlack;
+    }
+    return __builtin_amdgcn_ballot_w64(move) != 0;  // wave-uniform
+  };
+  auto move_maxima = [&](bool first) {
+#pragma unroll
+    for (int n = 0; n < kNc; ++n) {
+      const float m_new = top[n] > m[n] + kSlack ? top[n] : m[n];
+      const float corr = m_new == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - m_new);
+      m[n] = m_new;
+      l[n] *= corr;
+      if (first) continue;  // the sums are 0
+      if constexpr (kCareful) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) acc[b][n] *= corr;
+      } else {
+        accs_settled();
+#pragma unroll
+        for (int b = 0; b < kBlocks; b += 4) {
+          f32x4_t v[4];
+          accs_out(v, acc[b][n], acc[b + 1][n], acc[b + 2][n], acc[b + 3][n], own);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] *= corr;
+          accs_in(acc[b][n], acc[b + 1][n], acc[b + 2][n], acc[b + 3][n], v, own);
+        }
+      }
+    }
+  };
+  auto sums = [&](int pos0, const uint8_t* vt) {
     bf16x8_t pf[kNc];
 #pragma unroll
     for (int n = 0; n < kNc; ++n) {
-      float sc[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sc[j] = s4[j >> 2][n][j & 3] * (a.scale_log2 * ks[j >> 2]);
-      if (masked) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          sc[j] = sees(pos_of[n], pos0 + 16 * (j >> 2) + 4 * g + (j & 3), a.window, a.sinks) ? sc[j] : -INFINITY;
-      }
-      float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
-      mx = groups_max(mx);
-      if (__builtin_amdgcn_ballot_w64(mx > m[n] + kSlack) != 0) {  // wave-uniform
-        const float m_new = mx > m[n] + kSlack ? mx : m[n];
-        const float corr = m_new == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - m_new);
-        m[n] = m_new;
-        l[n] *= corr;
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) acc[b][n] *= corr;
-      }
       const float ref = m[n] == -INFINITY ? 0.0f : m[n];
       float w[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        w[j] = __builtin_amdgcn_exp2f(sc[j] - ref);
+        w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][j], cs[j >> 2], -ref));
         l[n] += w[j];
         if constexpr (kFormat != kBf16) w[j] *= vs[j >> 2];
       }
-      // Rounded to bf16 for the product: off by 2^-9 of each weight at most, which
+      // Rounded to bf16 for the product: off by 2^-8 of each weight at most, which
       // independent values average to less than the result's own rounding.
       u32x4_t ph;
 #pragma unroll
@@ -248,7 +356,7 @@ void window_prompt_kernel(const WindowArgs a, int off_items) {
       pf[n] = __builtin_bit_cast(bf16x8_t, ph);
     }
     auto v_frag = [&](int b) {
-      const uint8_t* at = vt_ + v_at[b & 7] + (b >> 3) * 256;
+      const uint8_t* at = vt + (v_at ^ (32 * (b & 7))) + (b >> 3) * 256;
       const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)at);
       const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(at + 16 * kRowBytes));
       return __builtin_bit_cast(u32x4_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -269,81 +377,125 @@ void window_prompt_kernel(const WindowArgs a, int off_items) {
       }
       return;
     }
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4_t vf[kAhead];
+#pragma unroll
+    for (int b = 0; b < kAhead; ++b) vf[b] = v_frag(b);
+    asm volatile("s_nop 1");
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
-      const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, v_frag(b));
+      __builtin_amdgcn_sched_barrier(0);
+      const bf16x8_t x = __builtin_bit_cast(bf16x8_t, vf[b % kAhead]);
 #pragma unroll
-      for (int n = 0; n < kNc; ++n) acc[b][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n], acc[b][n], 0, 0, 0);
+      for (int n = 0; n < kNc; ++n) acc_mfma(acc[b][n], x, pf[n]);
+      if (b + kAhead < kBlocks) vf[b % kAhead] = v_frag(b + kAhead);
     }
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  auto walk = [&](auto careful) {
 #pragma unroll
-    for (int n = 0; n < kNc; ++n) {
-      m[n] = -INFINITY;
-      l[n] = 0.0f;
+  for (int n = 0; n < kNc; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.0f;
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) acc[b][n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int b = 0; b < kBlocks; ++b) {
+      if constexpr (kCareful) acc[b][n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      else acc_zero(acc[b][n]);
     }
-    if constexpr (kFormat == kBf16) {
-      stage_bf16(lo, 0);
-    } else {
-      fetch_codes(lo);
-      store_codes(lo, 0);
-    }
+  }
+  if (kMayFail && threadIdx.x == 0) *odd_flag = 0;
+  auto row_of = [&](int vt) { return tile_row(rows, tile_pos(vt), a.shift, a.row_mask); };
+  int64_t row = row_of(lo), next = row;
+  // The next tile of a bf16 cache goes to the other of two buffers, which is filled again
+  // after the barrier that ended its reads; the codes of the next tile of an 8-bit one to
+  // their own place, once the tile before has become bf16 rows.
+  if constexpr (kFormat == kBf16) {
+    stage(tile_pos(lo), row, lds, lds + kTileBytes);
+    if (lo + 1 < hi) next = row_of(lo + 1);
     wait_loads<0>();
     lds_barrier();
-    // One barrier a tile: a buffer is filled again after the barrier that ended its reads.
-    for (int vt = lo; vt < hi; ++vt) {
-      const int buf = (vt - lo) & 1;
-      const bool more = vt + 1 < hi;
-      if (more) {
-        if constexpr (kFormat == kBf16) stage_bf16(vt + 1, buf ^ 1);
-        else fetch_codes(vt + 1);
-      }
-      compute(careful, vt, buf);
-      if constexpr (kFormat != kBf16)
-        if (more) store_codes(vt + 1, buf ^ 1);
+  } else {
+    stage(tile_pos(lo), row, codes, codes + kStageBytes);
+  }
+  for (int vt = lo; vt < hi; ++vt) {
+    uint8_t* at = kFormat == kBf16 ? lds + 2 * kTileBytes * ((vt - lo) & 1) : lds;
+    if constexpr (kFormat == kBf16) {
+      uint8_t* to = lds + 2 * kTileBytes * ((vt - lo + 1) & 1);
+      if (vt + 1 < hi) stage(tile_pos(vt + 1), next, to, to + kTileBytes);
+      row = next;
+      if (vt + 2 < hi) next = row_of(vt + 2);
+    } else {
+      if (vt > lo) row = next;
+      if (vt + 1 < hi) next = row_of(vt + 1);
+      wait_loads<0>();
+      lds_barrier();  // the codes are there, and the tile before has no reader left
+      convert();
+      lds_barrier();
+      if (vt + 1 < hi) stage(tile_pos(vt + 1), next, codes, codes + kStageBytes);
+    }
+    if (scores(tile_pos(vt), row, at)) move_maxima(vt == lo);
+    sums(tile_pos(vt), at + kTileBytes);
+    if constexpr (kFormat == kBf16) {
       wait_loads<0>();
       lds_barrier();
     }
-  };
-  if (threadIdx.x == 0) again = 0;  // ahead of the walk's first barrier
-  walk(std::false_type{});
-  if constexpr (kFormat != kInt8) {  // int8 codes are finite
-    bool odd = false;
-#pragma unroll
-    for (int n = 0; n < kNc; ++n)
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) odd |= !all_finite(acc[b][n]);
-    if (odd) again = 1;
-    lds_barrier();
-    // Read by every wave ahead of the second walk, which does not write it.
-    if (__builtin_amdgcn_readfirstlane(again) != 0) walk(std::true_type{});
   }
+  if constexpr (kFormat != kBf16) lds_barrier();  // ahead of a second walk
 
   // ---- the result, or a partial column: value r of block b is dim 16 b + 4 g + r ----
+  if constexpr (!kCareful) accs_settled();
+  bool odd = false;
 #pragma unroll
   for (int n = 0; n < kNc; ++n) {
     const float sum = groups_sum(l[n]);
-    if (!live[n]) continue;
-    if (col0 < 0) {
-      const float inv = 1.0f / sum;
-      uint16_t* dst = static_cast<uint16_t*>(a.out) + q_row[n] * kD + 4 * g;
+    bool live;
+    const int64_t out_row = column(n, &live);
+    const int64_t col = col0 + static_cast<int64_t>(h) * prompt_cols(kD) + wave_col + 16 * n + c;
+    const float inv = 1.0f / sum;
+    uint16_t* dst = static_cast<uint16_t*>(a.out) + out_row * kD + 4 * g;
+    float* part = a.partials + col * kD + 4 * g;
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-        *reinterpret_cast<u32x2_t*>(dst + 16 * b) = u32x2_t{pack_bf16(acc[b][n][0] * inv, acc[b][n][1] * inv),
-                                                            pack_bf16(acc[b][n][2] * inv, acc[b][n][3] * inv)};
-    } else {
-      const int64_t col = col0 + static_cast<int64_t>(h) * prompt_cols(kD) + wave_col + 16 * n + c;
-      float* dst = a.partials + col * kD + 4 * g;
+    for (int b = 0; b < kBlocks; b += 4) {
+      f32x4_t v[4];
+      if constexpr (kCareful) {
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) *reinterpret_cast<f32x4_t*>(dst + 16 * b) = acc[b][n];
-      if (g == 0) {
-        a.sums[2 * col] = m[n];
-        a.sums[2 * col + 1] = sum;
+        for (int i = 0; i < 4; ++i) v[i] = acc[b + i][n];
+      } else {
+        accs_out(v, acc[b][n], acc[b + 1][n], acc[b + 2][n], acc[b + 3][n], own);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        odd |= !all_finite(v[i]);
+        if (!live) continue;
+        if (col0 < 0)
+          *reinterpret_cast<u32x2_t*>(dst + 16 * (b + i)) =
+              u32x2_t{pack_bf16(v[i][0] * inv, v[i][1] * inv), pack_bf16(v[i][2] * inv, v[i][3] * inv)};
+        else
+          *reinterpret_cast<f32x4_t*>(part + 16 * (b + i)) = v[i];
       }
     }
+    if (live && col0 >= 0 && g == 0) {
+      a.sums[2 * col] = m[n];
+      a.sums[2 * col + 1] = sum;
+    }
+  }
+  if constexpr (kMayFail) {
+    if (odd) *odd_flag = 1;
+    lds_barrier();
+    return __builtin_amdgcn_readfirstlane(*odd_flag) == 0;
+  }
+  return true;
+}
+
+template <int kD, int kFormat>
+__global__ __launch_bounds__(64 * kPromptWaves)
+__attribute__((amdgpu_waves_per_eu(1, 1)))
+void window_prompt_kernel(const WindowArgs a, int off_items) {
+  __shared__ __align__(16) uint8_t lds[Prompt<kD, kFormat>::kLds];
+  __shared__ int odd_flag;
+  if (!prompt_block<kD, kFormat, false>(a, off_items, lds, &odd_flag)) {
+    lds_barrier();  // every wave has read the flag
+    prompt_block<kD, kFormat, true>(a, off_items, lds, &odd_flag);
   }
 }
 
@@ -351,7 +503,7 @@ template <int kD>
 hipError_t prompts_of(const WindowArgs& a, int format, int off_items, int64_t num_items, hipStream_t stream) {
   const int64_t groups = num_items * a.num_kv;
   if (groups > kMaxGroups) return hipErrorInvalidConfiguration;
-  const dim3 grid(static_cast<uint32_t>(groups)), block(64 * prompt_waves(kD));
+  const dim3 grid(static_cast<uint32_t>(groups)), block(64 * kPromptWaves);
   if (format == kBf16) window_prompt_kernel<kD, kBf16><<<grid, block, 0, stream>>>(a, off_items);
   else if (format == kE4m3) window_prompt_kernel<kD, kE4m3><<<grid, block, 0, stream>>>(a, off_items);
   else window_prompt_kernel<kD, kInt8><<<grid, block, 0, stream>>>(a, off_items);
