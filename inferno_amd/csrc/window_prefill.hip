@@ -16,6 +16,9 @@
 // The maximum of a column's softmax is only moved when a score passes it by 2^8: the
 // weights are then at most 2^8, which f32 sums and bf16's exponent hold with room, and the
 // accumulators are rarely multiplied.
+#ifndef DEPTH
+#define DEPTH 2
+#endif
 #include <type_traits>
 
 #include "prefill_waves.hpp"
@@ -44,49 +47,53 @@ __device__ __forceinline__ void load_lds1(const char* base, uint32_t off, const 
       : "s"(prefill::lds_addr(lds)), "v"(off), "s"(base)
       : "memory");
 }
+template <int n>
+__device__ __forceinline__ void wait_all_but() {
+  if constexpr (n == 2) asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+  else wait_loads<n>();
+}
 __device__ __forceinline__ float max4(const float* v) { return raw_max(prefill::max3_raw(v[0], v[1], v[2]), v[3]); }
 
 // A wave's sums, 16x16 blocks of O^T, in accumulation registers from the first product to
 // the last.  Held as ordinary values, the compiler moves them between the two halves of the
 // register file for every tile, as the rare multiplication by a correction and the store
 // are VALU work; so all that touches them is written as instructions here.  The compiler
-// does not know that these are MFMAs: what VALU instructions wrote is read two wait states
-// later at the earliest (the s_nop 1 ahead of each run of them), and the sums are read
-// behind accs_settled().
+// does not know that these are MFMAs: what VALU instructions wrote (a move of an operand
+// that the compiler put there among them) is read two wait states later at the earliest,
+// hence the s_nop 1, and the sums are read behind accs_settled().
 __device__ __forceinline__ void acc_zero(f32x4_t& acc) {
   const u32x4_t none = u32x4_t{0u, 0u, 0u, 0u};
   asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %1, 0" : "=a"(acc) : "v"(none));
 }
 __device__ __forceinline__ void acc_mfma(f32x4_t& acc, bf16x8_t x, bf16x8_t y) {
-  asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(x), "v"(y));
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(x), "v"(y));
+}
+// Scores, in ordinary registers: as the compiler's own MFMAs they would be given accumulation
+// registers, and the sums pushed out of them.
+__device__ __forceinline__ void score_first(f32x4_t& s, bf16x8_t x, bf16x8_t y) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(x), "v"(y));
+}
+__device__ __forceinline__ void score_mfma(f32x4_t& s, bf16x8_t x, bf16x8_t y) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(x), "v"(y));
 }
 __device__ __forceinline__ void accs_settled() { asm volatile("s_nop 15\n\ts_nop 15"); }
-// Four blocks to ordinary registers, and back, over 4 KiB of LDS that the wave has to
-// itself (at: this lane's 16 bytes).
-__device__ __forceinline__ void accs_out(f32x4_t* v, const f32x4_t& a0, const f32x4_t& a1, const f32x4_t& a2,
-                                         const f32x4_t& a3, uint32_t at) {
+// Two blocks to ordinary registers, and back, over 2 KiB of LDS that the wave has to itself
+// (at: this lane's 16 bytes).
+constexpr int kOwnBytes = 2048;
+__device__ __forceinline__ void accs_out(f32x4_t* v, const f32x4_t& a0, const f32x4_t& a1, uint32_t at) {
   asm volatile(
-      "ds_write_b128 %4, %5\n\tds_write_b128 %4, %6 offset:1024\n\t"
-      "ds_write_b128 %4, %7 offset:2048\n\tds_write_b128 %4, %8 offset:3072\n\t"
-      "s_waitcnt lgkmcnt(0)\n\t"
-      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\t"
-      "ds_read_b128 %2, %4 offset:2048\n\tds_read_b128 %3, %4 offset:3072\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
-      : "v"(at), "a"(a0), "a"(a1), "a"(a2), "a"(a3)
+      "ds_write_b128 %2, %3\n\tds_write_b128 %2, %4 offset:1024\n\ts_waitcnt lgkmcnt(0)\n\t"
+      "ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:1024\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1])
+      : "v"(at), "a"(a0), "a"(a1)
       : "memory");
 }
-__device__ __forceinline__ void accs_in(f32x4_t& a0, f32x4_t& a1, f32x4_t& a2, f32x4_t& a3, const f32x4_t* v,
-                                        uint32_t at) {
+__device__ __forceinline__ void accs_in(f32x4_t& a0, f32x4_t& a1, const f32x4_t* v, uint32_t at) {
   asm volatile(
-      "ds_write_b128 %4, %5\n\tds_write_b128 %4, %6 offset:1024\n\t"
-      "ds_write_b128 %4, %7 offset:2048\n\tds_write_b128 %4, %8 offset:3072\n\t"
-      "s_waitcnt lgkmcnt(0)\n\t"
-      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\t"
-      "ds_read_b128 %2, %4 offset:2048\n\tds_read_b128 %3, %4 offset:3072\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&a"(a0), "=&a"(a1), "=&a"(a2), "=&a"(a3)
-      : "v"(at), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3])
+      "ds_write_b128 %2, %3\n\tds_write_b128 %2, %4 offset:1024\n\ts_waitcnt lgkmcnt(0)\n\t"
+      "ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:1024\n\ts_waitcnt lgkmcnt(0)"
+      : "=&a"(a0), "=&a"(a1)
+      : "v"(at), "v"(v[0]), "v"(v[1])
       : "memory");
 }
 
@@ -100,19 +107,21 @@ struct Prompt {
   static constexpr int kNc = prompt_col_tiles(kD);        // column tiles of a wave
   static constexpr int kRowBytes = 2 * kD;                // of a tile row in LDS
   static constexpr int kTileBytes = kTileKeys * kRowBytes;
-  // bf16: two tiles of K and V.  8-bit: one, and behind it the codes of the next.
-  static constexpr int kTiles = kFormat == kBf16 ? 4 * kTileBytes : 3 * kTileBytes;
-  static constexpr int kLds = kTiles + kPromptWaves * 4096;  // and what accs_out and accs_in use
+  // bf16: two tiles of K and V.  8-bit: one, and behind it the codes of two.
+  static constexpr int kDepth = DEPTH;
+  static constexpr int kStageBytes = kTileKeys * kD * elt_bytes(kFormat);  // of K, or V, as it comes from the cache
+  static constexpr int kTiles = kFormat == kBf16 ? kDepth * 2 * kTileBytes : 2 * kTileBytes + kDepth * 2 * kStageBytes;
+  static constexpr int kLds = kTiles + prompt_waves(kD) * kOwnBytes;  // and what accs_out and accs_in use
 };
 
 template <int kD, int kFormat, bool kCareful>
 __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items, uint8_t* lds, int* odd_flag) {
   using P = Prompt<kD, kFormat>;
-  constexpr int kWaves = kPromptWaves;
+  constexpr int kWaves = prompt_waves(kD);
   constexpr int kNc = P::kNc, kRowBytes = P::kRowBytes, kTileBytes = P::kTileBytes;
   constexpr int kSteps = kD / 32, kBlocks = kD / 16;
   constexpr int kEsz = elt_bytes(kFormat);
-  constexpr int kStageBytes = kTileKeys * kD * kEsz;      // of K, or V, as it comes from the cache
+  constexpr int kStageBytes = P::kStageBytes, kDepth = P::kDepth;
   constexpr int kLoads = kStageBytes / kWaves / 1024;     // 1 KiB loads of a wave
   constexpr int kRowLanes = kD * kEsz / 16;               // lanes of a row in one of them
   constexpr bool kMayFail = !kCareful && kFormat != kInt8;  // int8 codes are finite
@@ -198,8 +207,7 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
     }
   };
   // 8-bit: the staged codes become bf16 rows.  A thread takes 16 codes at a time.
-  uint8_t* codes = lds + 2 * kTileBytes;
-  auto convert = [&]() {
+  auto convert = [&](const uint8_t* codes) {
     constexpr int kTurns = kStageBytes / 16 / (64 * kWaves);
     u32x4_t w[2][kTurns];
 #pragma unroll
@@ -222,7 +230,7 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
     }
   };
 
-  const uint32_t own = prefill::lds_addr(lds + P::kTiles + 4096 * wave + 16 * lane);
+  const uint32_t own = prefill::lds_addr(lds + P::kTiles + kOwnBytes * wave + 16 * lane);
 
   // ---- LDS reads ----
   // K fragment of half tile u, step s: chunk 4 s + g of row 16 u + c, that is k_at ^ 64 s.
@@ -257,30 +265,27 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
       }
     }
     f32x4_t s4[2][kNc];
+    // Fragment i: half tile i % 2 of step i / 2, kAhead reads ahead of its products.
+    auto k_frag = [&](int i) {
+      const int s = i >> 1, u = i & 1;
+      return *reinterpret_cast<const bf16x8_t*>(kt + (k_at ^ (64 * (s & 3))) + (s >> 2) * 256 + u * 16 * kRowBytes);
+    };
+    bf16x8_t kf[kAhead];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int i = 0; i < kAhead; ++i) kf[i] = k_frag(i);
 #pragma unroll
-      for (int n = 0; n < kNc; ++n) s4[u][n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < 2 * kSteps; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kt + (k_at ^ (64 * (s & 3))) + (s >> 2) * 256 + u * 16 * kRowBytes);
-#pragma unroll
-        for (int n = 0; n < kNc; ++n)
-          s4[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, __builtin_bit_cast(bf16x8_t, qf[n][s]), s4[u][n], 0, 0, 0);
+      for (int n = 0; n < kNc; ++n) {
+        const bf16x8_t y = __builtin_bit_cast(bf16x8_t, qf[n][i >> 1]);
+        if (i < 2) score_first(s4[i][n], kf[i % kAhead], y);
+        else score_mfma(s4[i & 1][n], kf[i % kAhead], y);
       }
-    // Left alone, the scheduler puts all reads first and runs out of registers.
-    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
-#pragma unroll
-    for (int i = 0; i < 2 * kSteps - kAhead; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, kNc, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if (i + kAhead < 2 * kSteps) kf[i % kAhead] = k_frag(i + kAhead);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, kAhead * kNc, 0);
     __builtin_amdgcn_sched_barrier(0);
-    // The maxima below are taken by instructions that the compiler does not look into, so
-    // it puts no wait states between them and the MFMAs.
+    // The compiler knows nothing of the wait states between these MFMAs and their readers.
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -326,12 +331,12 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
       } else {
         accs_settled();
 #pragma unroll
-        for (int b = 0; b < kBlocks; b += 4) {
-          f32x4_t v[4];
-          accs_out(v, acc[b][n], acc[b + 1][n], acc[b + 2][n], acc[b + 3][n], own);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] *= corr;
-          accs_in(acc[b][n], acc[b + 1][n], acc[b + 2][n], acc[b + 3][n], v, own);
+        for (int b = 0; b < kBlocks; b += 2) {
+          f32x4_t v[2];
+          accs_out(v, acc[b][n], acc[b + 1][n], own);
+          v[0] *= corr;
+          v[1] *= corr;
+          accs_in(acc[b][n], acc[b + 1][n], v, own);
         }
       }
     }
@@ -381,7 +386,6 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
     u32x4_t vf[kAhead];
 #pragma unroll
     for (int b = 0; b < kAhead; ++b) vf[b] = v_frag(b);
-    asm volatile("s_nop 1");
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
       __builtin_amdgcn_sched_barrier(0);
@@ -404,43 +408,40 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
     }
   }
   if (kMayFail && threadIdx.x == 0) *odd_flag = 0;
-  auto row_of = [&](int vt) { return tile_row(rows, tile_pos(vt), a.shift, a.row_mask); };
-  int64_t row = row_of(lo), next = row;
-  // The next tile of a bf16 cache goes to the other of two buffers, which is filled again
-  // after the barrier that ended its reads; the codes of the next tile of an 8-bit one to
-  // their own place, once the tile before has become bf16 rows.
-  if constexpr (kFormat == kBf16) {
-    stage(tile_pos(lo), row, lds, lds + kTileBytes);
-    if (lo + 1 < hi) next = row_of(lo + 1);
-    wait_loads<0>();
-    lds_barrier();
-  } else {
-    stage(tile_pos(lo), row, codes, codes + kStageBytes);
-  }
+  // Staged tiles go round kDepth buffers, kDepth - 1 of them ahead of the one at hand; a
+  // buffer is filled again after the barrier that ended its reads.
+  auto row_of = [&](int vt) { return vt < hi ? tile_row(rows, tile_pos(vt), a.shift, a.row_mask) : 0; };
+  uint8_t* ring = kFormat == kBf16 ? lds : lds + 2 * kTileBytes;
+  auto stage_tile = [&](int vt, int64_t r, int buf) {
+    if (vt < hi) stage(tile_pos(vt), r, ring + buf * 2 * kStageBytes, ring + buf * 2 * kStageBytes + kStageBytes);
+  };
+  int64_t row[kDepth];  // of the tile at hand and those that are staged
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i) row[i] = row_of(lo + i);
+#pragma unroll
+  for (int i = 0; i < kDepth - 1; ++i) stage_tile(lo + i, row[i], i);
+  int buf = 0;
   for (int vt = lo; vt < hi; ++vt) {
-    uint8_t* at = kFormat == kBf16 ? lds + 2 * kTileBytes * ((vt - lo) & 1) : lds;
-    if constexpr (kFormat == kBf16) {
-      uint8_t* to = lds + 2 * kTileBytes * ((vt - lo + 1) & 1);
-      if (vt + 1 < hi) stage(tile_pos(vt + 1), next, to, to + kTileBytes);
-      row = next;
-      if (vt + 2 < hi) next = row_of(vt + 2);
-    } else {
-      if (vt > lo) row = next;
-      if (vt + 1 < hi) next = row_of(vt + 1);
-      wait_loads<0>();
-      lds_barrier();  // the codes are there, and the tile before has no reader left
-      convert();
+    // Of the loads in flight, those of the tiles behind the one at hand may stay so.
+    if (kDepth == 3 && vt + 1 < hi) wait_all_but<2 * kLoads>();
+    else wait_loads<0>();
+    lds_barrier();  // the tile is there, and the one before it has no reader left
+    const uint8_t* at = ring + buf * 2 * kStageBytes;
+    if constexpr (kFormat != kBf16) {
+      convert(at);
       lds_barrier();
-      if (vt + 1 < hi) stage(tile_pos(vt + 1), next, codes, codes + kStageBytes);
+      at = lds;
     }
-    if (scores(tile_pos(vt), row, at)) move_maxima(vt == lo);
+    stage_tile(vt + kDepth - 1, row[kDepth - 1], buf == 0 ? kDepth - 1 : buf - 1);
+    const int64_t mine = row[0];
+#pragma unroll
+    for (int i = 0; i < kDepth - 1; ++i) row[i] = row[i + 1];
+    row[kDepth - 1] = row_of(vt + kDepth);
+    if (scores(tile_pos(vt), mine, at)) move_maxima(vt == lo);
     sums(tile_pos(vt), at + kTileBytes);
-    if constexpr (kFormat == kBf16) {
-      wait_loads<0>();
-      lds_barrier();
-    }
+    buf = buf == kDepth - 1 ? 0 : buf + 1;
   }
-  if constexpr (kFormat != kBf16) lds_barrier();  // ahead of a second walk
+  lds_barrier();  // ahead of a second walk
 
   // ---- the result, or a partial column: value r of block b is dim 16 b + 4 g + r ----
   if constexpr (!kCareful) accs_settled();
@@ -455,16 +456,16 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
     uint16_t* dst = static_cast<uint16_t*>(a.out) + out_row * kD + 4 * g;
     float* part = a.partials + col * kD + 4 * g;
 #pragma unroll
-    for (int b = 0; b < kBlocks; b += 4) {
-      f32x4_t v[4];
+    for (int b = 0; b < kBlocks; b += 2) {
+      f32x4_t v[2];
       if constexpr (kCareful) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = acc[b + i][n];
+        v[0] = acc[b][n];
+        v[1] = acc[b + 1][n];
       } else {
-        accs_out(v, acc[b][n], acc[b + 1][n], acc[b + 2][n], acc[b + 3][n], own);
+        accs_out(v, acc[b][n], acc[b + 1][n], own);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 2; ++i) {
         odd |= !all_finite(v[i]);
         if (!live) continue;
         if (col0 < 0)
@@ -488,8 +489,8 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
 }
 
 template <int kD, int kFormat>
-__global__ __launch_bounds__(64 * kPromptWaves)
-__attribute__((amdgpu_waves_per_eu(1, 1)))
+__global__ __launch_bounds__(64 * prompt_waves(kD))
+__attribute__((amdgpu_waves_per_eu(2, 2)))
 void window_prompt_kernel(const WindowArgs a, int off_items) {
   __shared__ __align__(16) uint8_t lds[Prompt<kD, kFormat>::kLds];
   __shared__ int odd_flag;
@@ -503,7 +504,7 @@ template <int kD>
 hipError_t prompts_of(const WindowArgs& a, int format, int off_items, int64_t num_items, hipStream_t stream) {
   const int64_t groups = num_items * a.num_kv;
   if (groups > kMaxGroups) return hipErrorInvalidConfiguration;
-  const dim3 grid(static_cast<uint32_t>(groups)), block(64 * kPromptWaves);
+  const dim3 grid(static_cast<uint32_t>(groups)), block(64 * prompt_waves(kD));
   if (format == kBf16) window_prompt_kernel<kD, kBf16><<<grid, block, 0, stream>>>(a, off_items);
   else if (format == kE4m3) window_prompt_kernel<kD, kE4m3><<<grid, block, 0, stream>>>(a, off_items);
   else window_prompt_kernel<kD, kInt8><<<grid, block, 0, stream>>>(a, off_items);
