@@ -79,8 +79,10 @@ static_assert(kInSharedWrites < IFR_WINDOW_INFO_LEN, "info holds every word");
 // gives it; prompt blocks take 8 to 16 times the columns and the cache through LDS.  A run
 // of few columns would leave most of a prompt block idle.
 constexpr int64_t kRowItemCols = 32;
-// Workgroups that run at once: two of four waves on each of 256 CUs, at head_dim 512 one.
+// Workgroups that run at once, of row items: two of four waves on each of 256 CUs, at
+// head_dim 512 one; of prompt blocks: one of eight waves.
 constexpr int64_t resident_groups(int64_t head_dim) { return head_dim == 512 ? 256 : 512; }
+constexpr int64_t kPromptGroups = 256;
 constexpr int64_t kSplitGroups = 2 * 512;  // workgroups that splits aim at, at most
 
 struct Work {
@@ -246,7 +248,7 @@ int32_t plan(int32_t* img, int64_t img_words, const int32_t* runs, int64_t num_r
   }
   // Prompt blocks are split only where they do not fill the card.
   const int64_t want = static_cast<int64_t>(many.size()) * num_kv;
-  const int64_t many_chunk = want >= groups ? INT32_MAX : std::max<int64_t>(8, ceil_div(many_tiles * num_kv, groups));
+  const int64_t many_chunk = want >= kPromptGroups ? INT32_MAX : std::max<int64_t>(8, ceil_div(many_tiles * num_kv, kPromptGroups));
   for (const Part& p : many) {
     const int64_t n = std::min<int64_t>(ceil_div(p.tiles, many_chunk), kMaxStripes);
     b.put(b.prompts, p.t0, p.ntok, rows_base + runs[4 * p.run + 2], p.p0, std::max<int64_t>(n, 1), block_cols);

@@ -53,6 +53,20 @@ __device__ __forceinline__ u32x2_t codes4_bf16(uint32_t w) {
   }
 }
 
+// The same, times a power of two (or 0).
+template <int kFormat>
+__device__ __forceinline__ u32x2_t codes4_scaled(uint32_t w, float scale) {
+  if constexpr (kFormat == kE4m3) {
+    return u32x2_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))};
+  } else {
+    return u32x2_t{pack_bf16(static_cast<float>(static_cast<int8_t>(w)) * scale,
+                             static_cast<float>(static_cast<int8_t>(w >> 8)) * scale),
+                   pack_bf16(static_cast<float>(static_cast<int8_t>(w >> 16)) * scale,
+                             static_cast<float>(static_cast<int8_t>(w >> 24)) * scale)};
+  }
+}
+
 // Non-finite values of V.  In a product of matrices they reach every column, also those
 // that do not see them, as 0 * inf, and a weight's second part turns inf into NaN.  The
 // sums show that; the walk is then done again with each fragment of V taken apart: its

@@ -16,9 +16,6 @@
 // The maximum of a column's softmax is only moved when a score passes it by 2^8: the
 // weights are then at most 2^8, which f32 sums and bf16's exponent hold with room, and the
 // accumulators are rarely multiplied.
-#ifndef DEPTH
-#define DEPTH 2
-#endif
 #include <type_traits>
 
 #include "prefill_waves.hpp"
@@ -47,10 +44,13 @@ __device__ __forceinline__ void load_lds1(const char* base, uint32_t off, const 
       : "s"(prefill::lds_addr(lds)), "v"(off), "s"(base)
       : "memory");
 }
-template <int n>
-__device__ __forceinline__ void wait_all_but() {
-  if constexpr (n == 2) asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
-  else wait_loads<n>();
+// The lane, counted anew: what follows from it in a tile would otherwise be kept in registers
+// from the first tile on, and, as there are too few, in scratch memory.  Its reloads would
+// wait for every load of the next tiles in flight.
+__device__ __forceinline__ int lane_now() {
+  int n;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=&v"(n));
+  return n;
 }
 __device__ __forceinline__ float max4(const float* v) { return raw_max(prefill::max3_raw(v[0], v[1], v[2]), v[3]); }
 
@@ -107,21 +107,23 @@ struct Prompt {
   static constexpr int kNc = prompt_col_tiles(kD);        // column tiles of a wave
   static constexpr int kRowBytes = 2 * kD;                // of a tile row in LDS
   static constexpr int kTileBytes = kTileKeys * kRowBytes;
-  // bf16: two tiles of K and V.  8-bit: one, and behind it the codes of two.
-  static constexpr int kDepth = DEPTH;
+  static constexpr int kGroup = kD == 512 ? 1 : 2;        // tiles between two barriers
   static constexpr int kStageBytes = kTileKeys * kD * elt_bytes(kFormat);  // of K, or V, as it comes from the cache
-  static constexpr int kTiles = kFormat == kBf16 ? kDepth * 2 * kTileBytes : 2 * kTileBytes + kDepth * 2 * kStageBytes;
-  static constexpr int kLds = kTiles + prompt_waves(kD) * kOwnBytes;  // and what accs_out and accs_in use
+  // bf16: the tiles at hand and the next ones.  8-bit: the tiles at hand, and their codes
+  // and the next ones'.
+  static constexpr int kRows = kGroup * 2 * kTileBytes, kRing = 2 * kGroup * 2 * kStageBytes;
+  static constexpr int kTiles = kFormat == kBf16 ? kRing : kRows + kRing;
+  static constexpr int kLds = kTiles + kPromptWaves * kOwnBytes;  // and what accs_out and accs_in use
 };
 
 template <int kD, int kFormat, bool kCareful>
 __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items, uint8_t* lds, int* odd_flag) {
   using P = Prompt<kD, kFormat>;
-  constexpr int kWaves = prompt_waves(kD);
+  constexpr int kWaves = kPromptWaves;
   constexpr int kNc = P::kNc, kRowBytes = P::kRowBytes, kTileBytes = P::kTileBytes;
   constexpr int kSteps = kD / 32, kBlocks = kD / 16;
   constexpr int kEsz = elt_bytes(kFormat);
-  constexpr int kStageBytes = P::kStageBytes, kDepth = P::kDepth;
+  constexpr int kStageBytes = P::kStageBytes, kGroup = P::kGroup;
   constexpr int kLoads = kStageBytes / kWaves / 1024;     // 1 KiB loads of a wave
   constexpr int kRowLanes = kD * kEsz / 16;               // lanes of a row in one of them
   constexpr bool kMayFail = !kCareful && kFormat != kInt8;  // int8 codes are finite
@@ -170,76 +172,85 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
   // Rows that no query of the block sees: K's scores are masked, V's row is another one
   // that is seen (its weights are 0).
   const int w_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
+  auto seen_row = [&](int pos0, int r) {  // r, or the row that stands in for it
+    const bool all = pos0 + kTileKeys - 1 <= p1 && (pos0 >= w_lo || pos0 + kTileKeys - 1 < a.sinks);
+    if (all) return r;  // wave-uniform
+    const int j = pos0 + r;
+    const int gap = (w_lo < pos0 + kTileKeys ? w_lo : a.sinks - 1) - pos0;
+    return j > p1 ? p1 - pos0 : (j < w_lo && j >= a.sinks) ? gap : r;
+  };
   auto stage = [&](int pos0, int64_t row, uint8_t* kd, uint8_t* vd) {
-    const bool unseen = pos0 + kTileKeys - 1 > p1 || (pos0 < w_lo && pos0 + kTileKeys - 1 >= a.sinks);
-    uint32_t ko[kLoads], vo[kLoads];
+    const bool both = kLoads > 0;  // else the first half of the waves loads K, the second V
+    constexpr int kN = kLoads > 0 ? kLoads : 1;
+    constexpr uint32_t kAt = 1024u * (kN < 2 ? 0 : kN < 4 ? 1 : 3);
+    const int first = both ? wave * kN : wave % (kWaves / 2);
+    const int lane = lane_now();
+    uint32_t ko[kN], vo[kN];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int r = (wave * kLoads + i) * (64 / kRowLanes) + lane / kRowLanes;
+    for (int i = 0; i < kN; ++i) {
+      const int r = (first + i) * (64 / kRowLanes) + lane / kRowLanes;
       const uint32_t x = lane % kRowLanes;
-      int rv = r;
-      if (unseen) {
-        const int j = pos0 + r;
-        if (j > p1) rv = p1 - pos0;
-        else if (j < w_lo && j >= a.sinks) rv = (w_lo < pos0 + kTileKeys ? w_lo : a.sinks - 1) - pos0;
-      }
-      const uint32_t both = 1024u * ((kLoads < 4 ? 1 : 3) - (i & 3));  // the instruction's offset counts on both sides
-      ko[i] = static_cast<uint32_t>(r) * rb32 + 16u * (kFormat == kBf16 ? x ^ (r & 15) : x) + both;
-      vo[i] = static_cast<uint32_t>(rv) * rb32 + 16u * (kFormat == kBf16 ? x ^ (2 * (r & 7)) : x) + both;
+      const int rv = seen_row(pos0, r);
+      const uint32_t on = kAt - 1024u * (i & 3);  // the instruction's offset counts on both sides
+      ko[i] = static_cast<uint32_t>(r) * rb32 + 16u * (kFormat == kBf16 ? x ^ (r & 15) : x) + on;
+      vo[i] = static_cast<uint32_t>(rv) * rb32 + 16u * (kFormat == kBf16 ? x ^ (2 * (r & 7)) : x) + on;
     }
-    const char* kt = kb + row * row_bytes - 1024 * (kLoads < 4 ? 1 : 3);
-    const char* vt = vb + row * row_bytes - 1024 * (kLoads < 4 ? 1 : 3);
-    kd += wave * kLoads * 1024;
-    vd += wave * kLoads * 1024;
-    if constexpr (kLoads >= 4) {
-#pragma unroll
-      for (int i = 0; i < kLoads; i += 4) {
-        load_lds4(kt, ko[i], ko[i + 1], ko[i + 2], ko[i + 3], kd + 1024 * i);
-        load_lds4(vt, vo[i], vo[i + 1], vo[i + 2], vo[i + 3], vd + 1024 * i);
-      }
+    const char* kt = kb + row * row_bytes - kAt;
+    const char* vt = vb + row * row_bytes - kAt;
+    kd += first * 1024;
+    vd += first * 1024;
+    if constexpr (kLoads == 4) {
+      load_lds4(kt, ko[0], ko[1], ko[2], ko[3], kd);
+      load_lds4(vt, vo[0], vo[1], vo[2], vo[3], vd);
     } else if constexpr (kLoads == 2) {
       load_lds2(kt, ko[0], ko[1], kd);
       load_lds2(vt, vo[0], vo[1], vd);
     } else {
-      static_assert(kLoads == 1);
-      load_lds1(kt + 1024, ko[0] - 1024, kd);
-      load_lds1(vt + 1024, vo[0] - 1024, vd);
+      static_assert(kLoads == 1 || (kLoads == 0 && kStageBytes / 1024 == kWaves / 2));
+      if (both || wave < kWaves / 2) load_lds1(kt, ko[0], kd);
+      if (both || wave >= kWaves / 2) load_lds1(vt, vo[0], vd);
     }
   };
-  // 8-bit: the staged codes become bf16 rows.  A thread takes 16 codes at a time.
-  auto convert = [&](const uint8_t* codes) {
-    constexpr int kTurns = kStageBytes / 16 / (64 * kWaves);
-    u32x4_t w[2][kTurns];
-#pragma unroll
-    for (int i = 0; i < kTurns; ++i)
-#pragma unroll
-      for (int v = 0; v < 2; ++v)
-        w[v][i] = *reinterpret_cast<const u32x4_t*>(codes + v * kStageBytes + 16 * (threadIdx.x + 64 * kWaves * i));
+  // 8-bit: the staged codes become bf16 rows, times their blocks' scales (powers of two, so
+  // exactly).  A thread takes 16 codes at a time, and has loaded their scale with them.
+  constexpr int kTurns = kFormat == kBf16 ? 1 : 2 * kStageBytes / 16 / (64 * kWaves);
+  auto fetch_scales = [&](int pos0, int64_t row, float* scale) {
+    const int thread = 64 * wave + lane_now();
 #pragma unroll
     for (int i = 0; i < kTurns; ++i) {
-      const int at = threadIdx.x + 64 * kWaves * i;
-      const int r = at / kRowLanes, x = 2 * (at % kRowLanes);
+      const int at = thread + 64 * kWaves * i;
+      const bool is_v = at >= kStageBytes / 16;
+      const int r = at / kRowLanes % kTileKeys;
+      const int64_t block = (row + (is_v ? seen_row(pos0, r) : r)) >> a.block_shift;
+      scale[i] = (is_v ? a.v_scale : a.k_scale)[block * a.num_kv + h];
+    }
+  };
+  auto convert = [&](const uint8_t* codes, uint8_t* to, const float* scale) {
+    const int thread = 64 * wave + lane_now();
+    u32x4_t w[kTurns];
 #pragma unroll
-      for (int v = 0; v < 2; ++v)
+    for (int i = 0; i < kTurns; ++i)
+      w[i] = *reinterpret_cast<const u32x4_t*>(codes + 16 * (thread + 64 * kWaves * i));
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const u32x2_t y = codes4_bf16<kFormat>(w[v][i][2 * e]), z = codes4_bf16<kFormat>(w[v][i][2 * e + 1]);
-          *reinterpret_cast<u32x4_t*>(lds + v * kTileBytes + r * kRowBytes + 16 * ((x + e) ^ (v ? 2 * (r & 7) : r & 15))) =
-              u32x4_t{y[0], y[1], z[0], z[1]};
-        }
+    for (int i = 0; i < kTurns; ++i) {
+      const int at = thread + 64 * kWaves * i;
+      const int v = at >= kStageBytes / 16 ? 1 : 0;  // of K, of V
+      const int r = at / kRowLanes % kTileKeys, x = 2 * (at % kRowLanes);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const u32x2_t y = codes4_scaled<kFormat>(w[i][2 * e], scale[i]), z = codes4_scaled<kFormat>(w[i][2 * e + 1], scale[i]);
+        *reinterpret_cast<u32x4_t*>(to + v * kTileBytes + r * kRowBytes + 16 * ((x + e) ^ (v ? 2 * (r & 7) : r & 15))) =
+            u32x4_t{y[0], y[1], z[0], z[1]};
+      }
     }
   };
 
-  const uint32_t own = prefill::lds_addr(lds + P::kTiles + kOwnBytes * wave + 16 * lane);
+  auto own_now = [&] { return prefill::lds_addr(lds + P::kTiles + kOwnBytes * wave) + 16 * lane_now(); };
 
   // ---- LDS reads ----
   // K fragment of half tile u, step s: chunk 4 s + g of row 16 u + c, that is k_at ^ 64 s.
   // V^T fragment of dims 16 b ..: rows 4 g + c / 4 of both halves, 8 bytes at dim 4 (c % 4),
   // that is v_at ^ 32 b.
-  const int k_at = c * kRowBytes + 16 * (g ^ c);
-  const int v_row = 4 * g + (c >> 2);
-  const int v_at = v_row * kRowBytes + 16 * (((c & 3) >> 1) ^ (2 * (v_row & 7))) + 8 * (c & 1);
-
   float m[kNc], l[kNc];
   f32x4_t acc[kBlocks][kNc];
 
@@ -247,24 +258,17 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
   // there anyway, and the branch around the accumulators would cost a copy of them.
   // ---- a tile: scores of the K at LDS kt, then weights and sums over the V at vt ----
   constexpr int kAhead = 4;  // fragments that LDS reads run ahead of their MFMAs
-  float sc[kNc][8], cs[2], vs[2], top[kNc];
+  float sc[kNc][8], top[kNc];
+  // Tiles whose first position lies in [seen_first, seen_last], or up to seen_sink, are seen
+  // whole by every column of the wave.
+  const int seen_last = wp0 - (kTileKeys - 1), seen_sink = a.sinks - kTileKeys;
+  const int seen_first = a.window > 0 ? wp1 - a.window + 1 : 0;
   // True if some column's maximum has to be moved first.
-  auto scores = [&](int pos0, int64_t row, const uint8_t* kt) {
-    const bool masked = !all_seen(wp0, wp1, pos0, kTileKeys, a.window, a.sinks);  // wave-uniform
-    cs[0] = cs[1] = a.scale_log2;
-    vs[0] = vs[1] = 1.0f;
-    if constexpr (kFormat != kBf16) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        cs[u] = vs[u] = 1.0f;  // of a half that the block does not see
-        if (any_seen(p0, p1, pos0 + 16 * u, 16, a.window, a.sinks)) {
-          const int64_t s = ((row + 16 * u) >> a.block_shift) * a.num_kv + h;
-          cs[u] = a.scale_log2 * sload_f32(a.k_scale + s);
-          vs[u] = sload_f32(a.v_scale + s);
-        }
-      }
-    }
+  auto scores = [&](int pos0, const uint8_t* kt) {
+    const bool masked = pos0 > seen_last || (pos0 < seen_first && pos0 > seen_sink);  // wave-uniform
     f32x4_t s4[2][kNc];
+    const int lane = lane_now();
+    const int k_at = (lane & 15) * kRowBytes + 16 * ((lane >> 4) ^ (lane & 15));
     // Fragment i: half tile i % 2 of step i / 2, kAhead reads ahead of its products.
     auto k_frag = [&](int i) {
       const int s = i >> 1, u = i & 1;
@@ -273,6 +277,7 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
     bf16x8_t kf[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) kf[i] = k_frag(i);
+    __builtin_amdgcn_s_setprio(1);  // products ahead of the other wave's softmax
 #pragma unroll
     for (int i = 0; i < 2 * kSteps; ++i) {
       __builtin_amdgcn_sched_barrier(0);
@@ -285,6 +290,7 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
       if (i + kAhead < 2 * kSteps) kf[i % kAhead] = k_frag(i + kAhead);
     }
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
     // The compiler knows nothing of the wait states between these MFMAs and their readers.
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -300,19 +306,19 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
         for (int r = 0; r < 4; ++r) sc[n][4 * u + r] = s4[u][n][r];
       }
     if (masked) {
-      asm volatile("");  // keeps this a branch: few tiles take it
+      const int j0 = pos0 + 4 * (lane_now() >> 4);  // also keeps this a branch: few tiles take it
 #pragma unroll
       for (int n = 0; n < kNc; ++n)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float& x = sc[n][j];
-          x = sees(pos_of[n], pos0 + 16 * (j >> 2) + 4 * g + (j & 3), a.window, a.sinks) ? x : -INFINITY;
+          x = sees(pos_of[n], j0 + 16 * (j >> 2) + (j & 3), a.window, a.sinks) ? x : -INFINITY;
         }
     }
     bool move = false;
 #pragma unroll
     for (int n = 0; n < kNc; ++n) {
-      top[n] = prefill::groups_max(raw_max(max4(sc[n]) * cs[0], max4(sc[n] + 4) * cs[1]));
+      top[n] = prefill::groups_max(raw_max(max4(sc[n]), max4(sc[n] + 4)) * a.scale_log2);
       move |= top[n] > m[n] + kSlack;
     }
     return __builtin_amdgcn_ballot_w64(move) != 0;  // wave-uniform
@@ -330,6 +336,7 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
         for (int b = 0; b < kBlocks; ++b) acc[b][n] *= corr;
       } else {
         accs_settled();
+        const uint32_t own = own_now();
 #pragma unroll
         for (int b = 0; b < kBlocks; b += 2) {
           f32x4_t v[2];
@@ -349,9 +356,8 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
       float w[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][j], cs[j >> 2], -ref));
+        w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][j], a.scale_log2, -ref));
         l[n] += w[j];
-        if constexpr (kFormat != kBf16) w[j] *= vs[j >> 2];
       }
       // Rounded to bf16 for the product: off by 2^-8 of each weight at most, which
       // independent values average to less than the result's own rounding.
@@ -360,6 +366,8 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
       for (int j = 0; j < 4; ++j) ph[j] = pack_bf16(w[2 * j], w[2 * j + 1]);
       pf[n] = __builtin_bit_cast(bf16x8_t, ph);
     }
+    const int lane = lane_now(), v_row = lane >> 2;  // 4 g + c / 4
+    const int v_at = v_row * kRowBytes + 16 * (((lane & 3) >> 1) ^ (2 * (v_row & 7))) + 8 * (lane & 1);
     auto v_frag = [&](int b) {
       const uint8_t* at = vt + (v_at ^ (32 * (b & 7))) + (b >> 3) * 256;
       const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)at);
@@ -369,7 +377,7 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
     if constexpr (kCareful) {
       bf16x8_t ones[kNc];
 #pragma unroll
-      for (int n = 0; n < kNc; ++n) ones[n] = seen_ones(pos_of[n], pos0, g, a.window, a.sinks);
+      for (int n = 0; n < kNc; ++n) ones[n] = seen_ones(pos_of[n], pos0, lane >> 4, a.window, a.sinks);
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
         __builtin_amdgcn_sched_barrier(0);  // one fragment at a time: registers
@@ -386,6 +394,7 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
     u32x4_t vf[kAhead];
 #pragma unroll
     for (int b = 0; b < kAhead; ++b) vf[b] = v_frag(b);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
       __builtin_amdgcn_sched_barrier(0);
@@ -395,6 +404,7 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
       if (b + kAhead < kBlocks) vf[b % kAhead] = v_frag(b + kAhead);
     }
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
   };
 
 #pragma unroll
@@ -408,43 +418,51 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
     }
   }
   if (kMayFail && threadIdx.x == 0) *odd_flag = 0;
-  // Staged tiles go round kDepth buffers, kDepth - 1 of them ahead of the one at hand; a
-  // buffer is filled again after the barrier that ended its reads.
+  // Groups of tiles go to two places in turn, which are filled again after the barrier that
+  // ended their reads: a group is loaded during the work on the one before it.
   auto row_of = [&](int vt) { return vt < hi ? tile_row(rows, tile_pos(vt), a.shift, a.row_mask) : 0; };
-  uint8_t* ring = kFormat == kBf16 ? lds : lds + 2 * kTileBytes;
-  auto stage_tile = [&](int vt, int64_t r, int buf) {
-    if (vt < hi) stage(tile_pos(vt), r, ring + buf * 2 * kStageBytes, ring + buf * 2 * kStageBytes + kStageBytes);
+  uint8_t* ring = kFormat == kBf16 ? lds : lds + P::kRows;
+  int64_t next[kGroup];  // rows of the group to be loaded
+  float scale[kGroup][kTurns];
+  auto stage_group = [&](int vt, uint8_t* to) {
+#pragma unroll
+    for (int e = 0; e < kGroup; ++e)
+      if (vt + e < hi) {
+        const int pos0 = tile_pos(vt + e);
+        if constexpr (kFormat != kBf16) fetch_scales(pos0, next[e], scale[e]);
+        stage(pos0, next[e], to + e * 2 * kStageBytes, to + e * 2 * kStageBytes + kStageBytes);
+        next[e] = row_of(vt + kGroup + e);
+      }
   };
-  int64_t row[kDepth];  // of the tile at hand and those that are staged
 #pragma unroll
-  for (int i = 0; i < kDepth; ++i) row[i] = row_of(lo + i);
-#pragma unroll
-  for (int i = 0; i < kDepth - 1; ++i) stage_tile(lo + i, row[i], i);
-  int buf = 0;
-  for (int vt = lo; vt < hi; ++vt) {
-    // Of the loads in flight, those of the tiles behind the one at hand may stay so.
-    if (kDepth == 3 && vt + 1 < hi) wait_all_but<2 * kLoads>();
-    else wait_loads<0>();
-    lds_barrier();  // the tile is there, and the one before it has no reader left
-    const uint8_t* at = ring + buf * 2 * kStageBytes;
+  for (int e = 0; e < kGroup; ++e) next[e] = row_of(lo + e);
+  stage_group(lo, ring);
+  int place = 0;
+  for (int vt = lo; vt < hi; vt += kGroup) {
+    wait_loads<0>();
+    lds_barrier();  // the group is there, and the one before it has no reader left
+    const uint8_t* at = ring + place * (P::kRing / 2);
+    place ^= 1;
     if constexpr (kFormat != kBf16) {
-      convert(at);
+#pragma unroll
+      for (int e = 0; e < kGroup; ++e)
+        if (vt + e < hi) convert(at + e * 2 * kStageBytes, lds + e * 2 * kTileBytes, scale[e]);
       lds_barrier();
       at = lds;
     }
-    stage_tile(vt + kDepth - 1, row[kDepth - 1], buf == 0 ? kDepth - 1 : buf - 1);
-    const int64_t mine = row[0];
-#pragma unroll
-    for (int i = 0; i < kDepth - 1; ++i) row[i] = row[i + 1];
-    row[kDepth - 1] = row_of(vt + kDepth);
-    if (scores(tile_pos(vt), mine, at)) move_maxima(vt == lo);
-    sums(tile_pos(vt), at + kTileBytes);
-    buf = buf == kDepth - 1 ? 0 : buf + 1;
+    stage_group(vt + kGroup, ring + place * (P::kRing / 2));
+#pragma unroll 1
+    for (int e = 0; e < kGroup && vt + e < hi; ++e) {
+      const int pos0 = tile_pos(vt + e);
+      if (scores(pos0, at + e * 2 * kTileBytes)) move_maxima(vt + e == lo);
+      sums(pos0, at + e * 2 * kTileBytes + kTileBytes);
+    }
   }
   lds_barrier();  // ahead of a second walk
 
   // ---- the result, or a partial column: value r of block b is dim 16 b + 4 g + r ----
   if constexpr (!kCareful) accs_settled();
+  const uint32_t own = own_now();
   bool odd = false;
 #pragma unroll
   for (int n = 0; n < kNc; ++n) {
@@ -489,7 +507,7 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
 }
 
 template <int kD, int kFormat>
-__global__ __launch_bounds__(64 * prompt_waves(kD))
+__global__ __launch_bounds__(64 * kPromptWaves)
 __attribute__((amdgpu_waves_per_eu(2, 2)))
 void window_prompt_kernel(const WindowArgs a, int off_items) {
   __shared__ __align__(16) uint8_t lds[Prompt<kD, kFormat>::kLds];
@@ -504,7 +522,7 @@ template <int kD>
 hipError_t prompts_of(const WindowArgs& a, int format, int off_items, int64_t num_items, hipStream_t stream) {
   const int64_t groups = num_items * a.num_kv;
   if (groups > kMaxGroups) return hipErrorInvalidConfiguration;
-  const dim3 grid(static_cast<uint32_t>(groups)), block(64 * prompt_waves(kD));
+  const dim3 grid(static_cast<uint32_t>(groups)), block(64 * kPromptWaves);
   if (format == kBf16) window_prompt_kernel<kD, kBf16><<<grid, block, 0, stream>>>(a, off_items);
   else if (format == kE4m3) window_prompt_kernel<kD, kE4m3><<<grid, block, 0, stream>>>(a, off_items);
   else window_prompt_kernel<kD, kInt8><<<grid, block, 0, stream>>>(a, off_items);
