@@ -7,6 +7,9 @@
 
 #include <algorithm>
 #include <array>
+#include <functional>
+#include <queue>
+#include <utility>
 #include <vector>
 
 #include "../../include/inferno_hip.h"
@@ -83,6 +86,8 @@ constexpr int64_t kRowItemCols = 32;
 // head_dim 512 one; of prompt blocks: one of eight waves.
 constexpr int64_t resident_groups(int64_t head_dim) { return head_dim == 512 ? 256 : 512; }
 constexpr int64_t kPromptGroups = 256;
+constexpr int64_t kBlockTiles = 3, kPieceTiles = 7;  // what a prompt block, and a piece of one, costs besides its tiles
+constexpr int64_t kLeastPiece = 4;                   // tiles
 constexpr int64_t kSplitGroups = 2 * 512;  // workgroups that splits aim at, at most
 
 struct Work {
@@ -132,6 +137,55 @@ struct Builder {
 struct Part {
   int64_t run, t0, ntok, p0, tiles;
 };
+
+// How many pieces each prompt block's tiles are split into.  One workgroup of prompt blocks
+// fits a CU, so what counts is the longest sum of pieces that one CU gets: 256 workgroups
+// of n tiles take as long as n tiles, 257 twice that.  Splits that bring the pieces up to one
+// or two workgroups a CU are compared with none, at their lengths and what a piece costs
+// besides (its start, and where it is split its sums in memory and their merging).
+std::vector<int64_t> prompt_splits(const std::vector<Part>& parts, int64_t num_kv) {
+  const std::vector<int64_t> whole(parts.size(), 1);
+  std::vector<int64_t> best = whole;
+  const int64_t want = static_cast<int64_t>(parts.size()) * num_kv;
+  if (parts.empty() || want >= 2 * kPromptGroups) return best;
+  auto makespan = [&](const std::vector<int64_t>& n) {
+    std::vector<int64_t> pieces;
+    for (size_t i = 0; i < parts.size(); ++i)
+      for (int64_t s = 0; s < n[i]; ++s)
+        pieces.push_back(parts[i].tiles * (s + 1) / n[i] - parts[i].tiles * s / n[i] + (n[i] > 1 ? kPieceTiles : kBlockTiles));
+    std::sort(pieces.begin(), pieces.end(), std::greater<int64_t>());
+    std::priority_queue<int64_t, std::vector<int64_t>, std::greater<int64_t>> cus;
+    for (int64_t i = 0; i < kPromptGroups; ++i) cus.push(0);
+    int64_t end = 0;
+    for (int64_t piece : pieces)
+      for (int64_t h = 0; h < num_kv; ++h) {
+        const int64_t t = cus.top() + piece;
+        cus.pop();
+        cus.push(t);
+        end = std::max(end, t);
+      }
+    return end;
+  };
+  int64_t least = makespan(best);
+  for (int64_t most : {kPromptGroups, 2 * kPromptGroups}) {
+    std::vector<int64_t> n = whole;
+    std::priority_queue<std::pair<int64_t, int64_t>> longest;  // piece, and the smaller index first
+    for (size_t i = 0; i < parts.size(); ++i) longest.push({parts[i].tiles, -static_cast<int64_t>(i)});
+    for (int64_t total = want; total + num_kv <= most; total += num_kv) {
+      const auto [len, i] = longest.top();
+      if (len < 2 * kLeastPiece) break;
+      longest.pop();
+      if (++n[-i] < kMaxStripes) longest.push({ceil_div(parts[-i].tiles, n[-i]), i});
+      if (longest.empty()) break;
+    }
+    const int64_t t = makespan(n);
+    if (t < least) {
+      least = t;
+      best = n;
+    }
+  }
+  return best;
+}
 
 // Longest first: workgroups start in order as earlier ones end.
 void longest_first(std::vector<Work>& v) {
@@ -246,13 +300,9 @@ int32_t plan(int32_t* img, int64_t img_words, const int32_t* runs, int64_t num_r
     const int64_t n = std::min<int64_t>(ceil_div(p.tiles, few_chunk), kMaxStripes);
     b.put(b.items, p.t0, p.ntok, rows_base + runs[4 * p.run + 2], p.p0, std::max<int64_t>(n, 1), kRowCols);
   }
-  // Prompt blocks are split only where they do not fill the card.
-  const int64_t want = static_cast<int64_t>(many.size()) * num_kv;
-  const int64_t many_chunk = want >= kPromptGroups ? INT32_MAX : std::max<int64_t>(8, ceil_div(many_tiles * num_kv, kPromptGroups));
-  for (const Part& p : many) {
-    const int64_t n = std::min<int64_t>(ceil_div(p.tiles, many_chunk), kMaxStripes);
-    b.put(b.prompts, p.t0, p.ntok, rows_base + runs[4 * p.run + 2], p.p0, std::max<int64_t>(n, 1), block_cols);
-  }
+  const std::vector<int64_t> splits = prompt_splits(many, num_kv);
+  for (size_t i = 0; i < many.size(); ++i)
+    b.put(b.prompts, many[i].t0, many[i].ntok, rows_base + runs[4 * many[i].run + 2], many[i].p0, splits[i], block_cols);
   longest_first(b.items);
   longest_first(b.prompts);
 
