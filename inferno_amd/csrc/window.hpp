@@ -32,10 +32,11 @@ constexpr int64_t kMaxGroups = (1 << 23) - 1;  // a launch's threads fit 32 bits
 constexpr int kMaxStripes = 64;  // splits of a token: one lane each in the merge kernel
 constexpr int kRowCols = 16;     // columns of a row item: (token, q head of the kv head)
 
-// A prompt block: eight waves, each with 16 columns times its column tiles.
+// A prompt block: eight waves, each with some tiles of 32 columns, at head_dim 512 of 16.
 constexpr int kPromptWaves = 8;
-constexpr int prompt_col_tiles(int head_dim) { return head_dim == 128 ? 3 : 512 / head_dim; }
-constexpr int prompt_cols(int head_dim) { return kPromptWaves * 16 * prompt_col_tiles(head_dim); }
+constexpr int prompt_tile_cols(int head_dim) { return head_dim == 512 ? 16 : 32; }
+constexpr int prompt_col_tiles(int head_dim) { return head_dim == 128 ? 2 : 1; }
+constexpr int prompt_cols(int head_dim) { return kPromptWaves * prompt_tile_cols(head_dim) * prompt_col_tiles(head_dim); }
 
 struct Span {
   int n_sink;  // sink tiles ahead of the window's first tile

@@ -53,17 +53,20 @@ __device__ __forceinline__ u32x2_t codes4_bf16(uint32_t w) {
   }
 }
 
-// The same, times a power of two (or 0).
+// The same, times a power of two (or 0).  int8 as unsigned bytes of 128 more, one conversion
+// each: the fma takes 128 off again, exactly, as its result has 8 significant bits.
 template <int kFormat>
 __device__ __forceinline__ u32x2_t codes4_scaled(uint32_t w, float scale) {
   if constexpr (kFormat == kE4m3) {
     return u32x2_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false)),
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))};
   } else {
-    return u32x2_t{pack_bf16(static_cast<float>(static_cast<int8_t>(w)) * scale,
-                             static_cast<float>(static_cast<int8_t>(w >> 8)) * scale),
-                   pack_bf16(static_cast<float>(static_cast<int8_t>(w >> 16)) * scale,
-                             static_cast<float>(static_cast<int8_t>(w >> 24)) * scale)};
+    const uint32_t u = w ^ 0x80808080u;
+    const float off = -128.0f * scale;
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(static_cast<float>((u >> (8 * i)) & 0xFFu), scale, off);
+    return u32x2_t{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
   }
 }
 
@@ -98,16 +101,20 @@ __device__ __forceinline__ Parts taken_apart(const u32x4_t& v) {
   }
   return Parts{__builtin_bit_cast(bf16x8_t, f), __builtin_bit_cast(bf16x8_t, u), __builtin_bit_cast(bf16x8_t, d)};
 }
-__device__ __forceinline__ f32x4_t add_infinities(f32x4_t acc, const Parts& v, bf16x8_t seen) {
-  const f32x4_t none = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  const f32x4_t up = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v.up, seen, none, 0, 0, 0);
-  const f32x4_t down = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v.down, seen, none, 0, 0, 0);
+template <typename Acc>
+__device__ __forceinline__ Acc with_infinities(Acc acc, const Acc& up, const Acc& down) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
+  for (int r = 0; r < static_cast<int>(sizeof(Acc) / 4); ++r) {
     acc[r] += up[r] > 0.0f ? INFINITY : 0.0f;
     acc[r] += down[r] > 0.0f ? -INFINITY : 0.0f;
   }
   return acc;
+}
+__device__ __forceinline__ f32x4_t add_infinities(f32x4_t acc, const Parts& v, bf16x8_t seen) {
+  const f32x4_t none = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const f32x4_t up = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v.up, seen, none, 0, 0, 0);
+  const f32x4_t down = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v.down, seen, none, 0, 0, 0);
+  return with_infinities(acc, up, down);
 }
 
 // Whether a query at position p sees position j.

@@ -65,7 +65,7 @@ def test_items_cover_every_visible_tile_once(shape, step):
     pos_of = np.concatenate([np.arange(c, c + n) for c, n in lens])
     covered = [[] for _ in range(case.seq)]
     columns = {}
-    for off, n, most in ((16, info[0], ROW_COLS), (info[22], info[14], {128: 384, 256: 256, 512: 128}[d])):
+    for off, n, most in ((16, info[0], ROW_COLS), (info[22], info[14], {128: 512, 256: 256, 512: 128}[d])):
         lengths = []
         for t0, ntok, rows_off, p0, lo, hi, col, _ in items_of(img, off, n):
             assert 0 < ntok and ntok * gqa <= most and p0 == pos_of[t0] and lo < hi
