@@ -88,6 +88,9 @@ constexpr int64_t resident_groups(int64_t head_dim) { return head_dim == 512 ? 2
 constexpr int64_t kPromptGroups = 256;
 constexpr int64_t kBlockTiles = 3, kPieceTiles = 7;  // what a prompt block, and a piece of one, costs besides its tiles
 constexpr int64_t kLeastPiece = 4;                   // tiles
+constexpr int64_t kItemTiles = 4;                    // what a row item costs besides a wave's tiles
+constexpr int64_t kMergePieces = 8;                  // pieces of a token whose merging costs as much as a tile
+constexpr int64_t kMaxRounds = 4;
 constexpr int64_t kSplitGroups = 2 * 512;  // workgroups that splits aim at, at most
 
 struct Work {
@@ -183,6 +186,40 @@ std::vector<int64_t> prompt_splits(const std::vector<Part>& parts, int64_t num_k
       least = t;
       best = n;
     }
+  }
+  return best;
+}
+
+// Tiles of a row item at most.  Workgroups run `slots` at a time, so the time is about the rounds
+// that they come to times an item's tiles (a wave's share of them) and what it costs besides, and
+// the merging of the most pieces that a token has.  For each number of rounds the shortest items
+// that keep to it are tried, and such of twice and four times the tiles.
+int64_t row_chunk(const std::vector<Part>& parts, int64_t heads, int64_t subs, int64_t slots) {
+  int64_t longest = subs;
+  for (const Part& p : parts) longest = std::max(longest, p.tiles);
+  auto rounds = [&](int64_t chunk) {
+    int64_t n = 0;
+    for (const Part& p : parts) n += std::min<int64_t>(ceil_div(p.tiles, chunk), kMaxStripes);
+    return ceil_div(n * heads, slots);
+  };
+  int64_t best = longest, least = INT64_MAX;
+  for (int64_t r = 1; r <= kMaxRounds; ++r) {
+    int64_t lo = subs, hi = longest;  // the shortest chunk of r rounds, if there is one
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (rounds(mid) <= r) hi = mid;
+      else lo = mid + 1;
+    }
+    if (rounds(lo) > r) continue;
+    for (int64_t chunk = lo; chunk <= 4 * lo; chunk *= 2) {
+      const int64_t pieces = ceil_div(longest, chunk);
+      const int64_t cost = rounds(chunk) * (ceil_div(chunk, subs) + kItemTiles) + (pieces > 1 ? 1 + pieces / kMergePieces : 0);
+      if (cost < least) {
+        least = cost;
+        best = chunk;
+      }
+    }
+    if (lo == subs) break;  // no shorter items
   }
   return best;
 }
@@ -294,7 +331,7 @@ int32_t plan(int32_t* img, int64_t img_words, const int32_t* runs, int64_t num_r
   int64_t per_group = 1;
   if (few_tiles * num_kv >= 16 * 4 * groups) per_group = num_kv % 4 == 0 ? 4 : num_kv % 2 == 0 ? 2 : 1;
   const int64_t subs = 4 / per_group;
-  const int64_t few_chunk = std::max<int64_t>(2 * subs, ceil_div(few_tiles * (num_kv / per_group), 2 * groups));
+  const int64_t few_chunk = row_chunk(few, num_kv / per_group, subs, groups);
   const int64_t rows_base = 0;  // filled below: offsets are relative to the row table
   for (const Part& p : few) {
     const int64_t n = std::min<int64_t>(ceil_div(p.tiles, few_chunk), kMaxStripes);

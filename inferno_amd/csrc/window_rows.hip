@@ -407,7 +407,7 @@ void window_rows_kernel(const WindowArgs a, int off_items, int per_group) {
 template <int kD>
 __global__ __launch_bounds__(64 * kWaves) void window_merge_kernel(const WindowArgs a, int off_units) {
   constexpr int kN = kD / 64;
-  constexpr int kAhead = 8;  // splits' loads in flight together
+  constexpr int kAhead = kD == 512 ? 8 : 16;  // splits' loads in flight together
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int groups = (a.num_q + kWaves - 1) / kWaves;
@@ -418,11 +418,22 @@ __global__ __launch_bounds__(64 * kWaves) void window_merge_kernel(const WindowA
   const int64_t step = sload(un + kUnStep);
   const int kv = head / a.gqa;
   const int64_t col = static_cast<int64_t>(sload(un + kUnCol)) + static_cast<int64_t>(kv) * sload(un + kUnHstep) + (head - kv * a.gqa);
+  const float* src = a.partials + col * kD + lane * kN;
+  float x[kAhead][kN];
+  auto fetch = [&](int s0) {
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      const float* ps = src + min(s0 + e, n - 1) * step * kD;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) x[e][i] = ps[i];
+    }
+  };
   float ms = -INFINITY, ls = 0.0f;
   if (lane < n) {
     ms = a.sums[2 * (col + lane * step)];
     ls = a.sums[2 * (col + lane * step) + 1];
   }
+  fetch(0);  // ahead of the wait for the factors
   const float top = wave_max_ref(ms);
   const float f = ms == top ? 1.0f : __builtin_amdgcn_exp2f(ms - top);
   float sum = lane < n ? ls * f : 0.0f;
@@ -431,15 +442,8 @@ __global__ __launch_bounds__(64 * kWaves) void window_merge_kernel(const WindowA
   float v[kN];
 #pragma unroll
   for (int i = 0; i < kN; ++i) v[i] = 0.0f;
-  const float* src = a.partials + col * kD + lane * kN;
   for (int s0 = 0; s0 < n; s0 += kAhead) {
-    float x[kAhead][kN];
-#pragma unroll
-    for (int e = 0; e < kAhead; ++e) {
-      const float* ps = src + min(s0 + e, n - 1) * step * kD;
-#pragma unroll
-      for (int i = 0; i < kN; ++i) x[e][i] = ps[i];
-    }
+    if (s0 > 0) fetch(s0);
 #pragma unroll
     for (int e = 0; e < kAhead; ++e) {
       if (s0 + e >= n) break;
