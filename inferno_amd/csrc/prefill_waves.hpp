@@ -94,7 +94,6 @@ __device__ __forceinline__ void load_lds2(const char* base, uint32_t o0, uint32_
 template <int n>
 __device__ __forceinline__ void wait_loads() {
   if constexpr (n == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  else if constexpr (n == 1) asm volatile("s_waitcnt vmcnt(1)" ::: "memory");
   else if constexpr (n == 2) asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
   else if constexpr (n == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
   else if constexpr (n == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");

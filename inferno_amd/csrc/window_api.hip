@@ -79,9 +79,16 @@ static_assert(kInSharedWrites < IFR_WINDOW_INFO_LEN, "info holds every word");
 // The work of a step in row items and prompt blocks.
 //
 // Row items take 16 columns, a (token, q head) each, and the cache at the rate that HBM
-// gives it; prompt blocks take 8 to 16 times the columns and the cache through LDS.  A run
-// of few columns would leave most of a prompt block idle.
-constexpr int64_t kRowItemCols = 32;
+// gives it; prompt blocks take 8 to 32 times the columns and the cache through LDS.  A run
+// of few columns would leave most of a prompt block idle, and one of many would have row items
+// read the cache once for each 16 of them.  Runs of up to kRowItemCols columns are row items
+// always, runs of up to kRowItemMost if what all of those read stays below kRowItemBytes.
+// Measured as row items and as prompt blocks, on 4,096 positions of an e4m3 cache (us):
+//   head_dim 256, 8 kv heads, 1 run:   32 columns 20 and 37, 64 columns 28 and 38, 128 columns 30 and 39
+//   the same, 16 runs:                 32 columns 111 and 162, 64 columns (1.1 GB) 195 and 165
+//   head_dim 128, 4 kv heads, 16 runs: 32 columns 35 and 93, 64 columns (270 MB) 60 and 94, 128 (550 MB) 105 and 95
+constexpr int64_t kRowItemCols = 32, kRowItemMost = 128;
+constexpr int64_t kRowItemBytes = int64_t{400} << 20;
 // Workgroups that run at once, of row items: two of four waves on each of 256 CUs, at
 // head_dim 512 one; of prompt blocks: one of eight waves.
 constexpr int64_t resident_groups(int64_t head_dim) { return head_dim == 512 ? 256 : 512; }
@@ -91,7 +98,8 @@ constexpr int64_t kLeastPiece = 4;                   // tiles
 constexpr int64_t kItemTiles = 4;                    // what a row item costs besides a wave's tiles
 constexpr int64_t kMergePieces = 8;                  // pieces of a token whose merging costs as much as a tile
 constexpr int64_t kMaxRounds = 4;
-constexpr int64_t kSplitGroups = 2 * 512;  // workgroups that splits aim at, at most
+// Pieces at most that splits make: of row items all rounds, of prompt blocks two a CU more than there are.
+constexpr int64_t kSplitPieces = kMaxRounds * resident_groups(256) + 2 * kPromptGroups;
 
 struct Work {
   std::array<int32_t, kWorkWords> words;
@@ -230,8 +238,8 @@ void longest_first(std::vector<Work>& v) {
 }
 
 int64_t most_words(int64_t num_runs, int64_t num_rows, int64_t seq_len, int64_t block_len) {
-  // A part a token at most; splits add what fills the card (kSplitGroups items a kv head).
-  const int64_t items = std::min(seq_len * kMaxStripes, seq_len + 2 * kSplitGroups);
+  // A part a token at most; splits add kSplitPieces (with one kv head).
+  const int64_t items = std::min(seq_len * kMaxStripes, seq_len + kSplitPieces);
   const int64_t writes = block_len > 0 ? seq_len / block_len + 2 * num_runs + 1 : 0;
   return ifr::kHdrWords + kWorkWords * items + 4 * num_runs + num_rows + seq_len + kMergeWords * seq_len + kWriteBlockWords * writes;
 }
@@ -312,24 +320,39 @@ int32_t plan(int32_t* img, int64_t img_words, const int32_t* runs, int64_t num_r
   const int64_t block_tokens = block_cols / gqa;
   Builder b{num_kv, gqa, window, sinks, {}, {}, {}, 0};
   std::vector<Part> few, many;
-  int64_t few_tiles = 0, many_tiles = 0;
+  int64_t few_tiles = 0, between = 0;
+  const int64_t tile_bytes = 2 * kTileKeys * head_dim * (block_len > 0 ? 1 : 2);
+  for (int64_t i = 0; i < num_runs; ++i) {
+    const int64_t n = (i + 1 < num_runs ? runs[4 * (i + 1)] : seq_len) - runs[4 * i], cols = n * gqa;
+    if (cols > kRowItemCols && cols <= kRowItemMost)
+      between += b.tiles(runs[4 * i + 1], n) * ceil_div(cols, kRowCols) * num_kv * tile_bytes;
+  }
+  const int64_t row_cols = between <= kRowItemBytes ? kRowItemMost : kRowItemCols;
   for (int64_t i = 0; i < num_runs; ++i) {
     const int64_t start = runs[4 * i], base = runs[4 * i + 1];
     const int64_t n = (i + 1 < num_runs ? runs[4 * (i + 1)] : seq_len) - start;
-    const bool rows = n * gqa <= kRowItemCols;
+    const bool rows = n * gqa <= row_cols;
     const int64_t width = rows ? row_tokens : block_tokens;
     for (int64_t t = 0; t < n; t += width) {
       const int64_t c = std::min(width, n - t);
       const Part p{i, start + t, c, base + t, b.tiles(base + t, c)};
       (rows ? few : many).push_back(p);
-      (rows ? few_tiles : many_tiles) += p.tiles;
+      few_tiles += rows ? p.tiles : 0;
     }
   }
-  // A row item's four waves either take a kv head each or share one head's tiles; sharing
-  // costs a sum over LDS, and gives items of a quarter the length.
+  // A row item's four waves take a kv head each, or two of them or all four share the tiles of one.
+  // Sharing costs a sum over LDS, and gives items of a half or a quarter the length.  Single tokens,
+  // 1, 2 and 4 heads an item (us), by tiles times kv heads for each workgroup that runs at once:
+  //   2 (1 sequence of 4,096, e4m3, 256 dims)     16, 18 and 22
+  //   32 (16 of 4,096; 64 of 1,024)               56, 54 and 57; 53, 51 and 52
+  //   33 (33 of 700 to 20,000, window 4,096, bf16, 512 dims, 2 heads)   149 and 155
+  //   48 (48 of 4,096, int8, 512 dims, 2 heads)   94 and 82
+  //   129 (64 of 4,096)                           188, 177 and 170
   const int64_t groups = resident_groups(head_dim);
+  const int64_t load = few_tiles * num_kv / groups;
   int64_t per_group = 1;
-  if (few_tiles * num_kv >= 16 * 4 * groups) per_group = num_kv % 4 == 0 ? 4 : num_kv % 2 == 0 ? 2 : 1;
+  if (load >= 64 && num_kv % 4 == 0) per_group = 4;
+  else if (load >= 40 && num_kv % 2 == 0) per_group = 2;
   const int64_t subs = 4 / per_group;
   const int64_t few_chunk = row_chunk(few, num_kv / per_group, subs, groups);
   const int64_t rows_base = 0;  // filled below: offsets are relative to the row table

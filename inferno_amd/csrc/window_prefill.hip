@@ -19,15 +19,17 @@
 // accumulators are rarely multiplied.
 //
 // Measured: 4 prompts of 2,048 new tokens, 16 q and 8 kv heads of 256, on up to 7,693 positions of
-// an int8 cache: 742 us, 930 TFLOP/s of what the mask leaves; with a window of 1,024 on a bf16
-// cache 191 us.  Without its products the first would take 430 us, without the softmax 690, without
-// loading and converting 560: the parts come one after the other, as the two waves of a SIMD do the
-// same thing at the same time, at the rate of the pipe that does it (two waves is what 256 registers
-// each leave).  Tried and slower: the halves of the block half a step apart, with a second barrier
-// in each step (790 us); scores of the next tile between the weights of this one (810 us); 16x16x32
-// products with two or three column tiles a wave (815 us); a group of two tiles a barrier made no
-// difference, nor did fewer instructions for addresses.  Stores of whole cache lines over LDS save
-// 15 us of the second's 206.
+// an int8 cache: 769 us, 890 TFLOP/s of what the mask leaves; with a window of 1,024 on a bf16 cache
+// 177 us.  The time is the sum of its parts (repeated calls, 735 us: without the products 430, without
+// the softmax 690, without loading and converting 560), as the two waves of a SIMD do the same thing
+// at the same time, at the rate of the pipe that does it; two waves is what 256 registers each leave.
+// Tried: the second half of the waves with its barrier behind the scores instead of ahead of them, so
+// that one wave's products meet the other's softmax: 5 % faster here, 6 to 8 % slower for short pieces
+// and at head_dim 128 (a longer start, more registers); the halves apart by a second barrier in each
+// step: 790 us against 735; scores of the next tile between the weights of this one: 810; 16x16x32
+// products with two or three column tiles a wave: 815.  A group of two tiles a barrier made no
+// difference, nor did fewer instructions for addresses.  Stores of whole cache lines over LDS save 15
+// us of the second's 206.
 #include <float.h>
 
 #include <type_traits>

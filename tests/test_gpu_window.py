@@ -131,7 +131,7 @@ def test_prompts(shape, kv):
     that start inside a block, sinks ahead of and inside the window."""
     announce(f"window prompts {shape} {kv}")
     gqa = shape[0] // shape[1]
-    n = 33 // gqa + 1
+    n = 128 // gqa + 1
     for lens, window, sinks in [([(0, n)], 0, 0), ([(45, n + 30), (3, n)], 0, 0), ([(130, n + 9)], 1, 0),
                                 ([(130, n + 9)], 40, 5), ([(0, n + 90)], 37, 64), ([(200, n + 3)], 150, 50)]:
         case = make_case(21, lens, window=window, sinks=sinks)
@@ -162,16 +162,16 @@ def test_prompt_blocks_and_splits(kv):
 @pytest.mark.parametrize("kv", KINDS)
 def test_pages_and_blocks(kv, page, block):
     announce(f"window pages {kv} {page} {block}")
-    case = make_case(29, [(95, 1), (31, 1), (320, 1), (64, 40)], page=page)
+    case = make_case(29, [(95, 1), (31, 1), (320, 1), (64, 100)], page=page)
     Step(case, kv, (4, 2, 128), 30, block=block).check("full")
-    case = make_case(31, [(95, 1), (31, 1), (320, 1), (64, 40)], page=page, window=70, sinks=33)
+    case = make_case(31, [(95, 1), (31, 1), (320, 1), (64, 100)], page=page, window=70, sinks=33)
     Step(case, kv, (4, 2, 128), 32, block=block).check("window")
 
 
 @pytest.mark.parametrize("kv", KINDS)
 def test_rows_wider_than_their_heads(kv):
     announce(f"window stride {kv}")
-    case = make_case(33, [(95, 1), (310, 2), (64, 40)])
+    case = make_case(33, [(95, 1), (310, 2), (64, 100)])
     for shape in [(4, 2, 128), (4, 2, 256), (8, 1, 512)]:
         Step(case, kv, shape, 34, gap=48).check(f"{shape}")
 
@@ -182,7 +182,7 @@ def test_score_ranges(kv, size, scale):
     """Scores of hundreds (one weight takes all) and of nothing (all weights alike), with
     maxima that move from tile to tile."""
     announce(f"window scores {kv} {size} {scale}")
-    case = make_case(35, [(400, 1), (150, 40)])
+    case = make_case(35, [(400, 1), (150, 100)])
     for shape in [(4, 2, 128), (2, 1, 256)]:
         Step(case, kv, shape, 36, q_size=size).check(f"{shape}", scale=scale)
 
@@ -190,7 +190,7 @@ def test_score_ranges(kv, size, scale):
 def test_a_rising_and_a_falling_row():
     """Scores that rise (or fall) by more than 2^8 from tile to tile."""
     announce("window rising scores")
-    case = make_case(37, [(300, 1), (200, 60)])
+    case = make_case(37, [(300, 1), (200, 100)])
     for sign in (1.0, -1.0):
         step = Step(case, "bf16", (4, 2, 128), 38)
         for r, (c, n) in enumerate(case.lens):
@@ -276,7 +276,7 @@ def test_rows_past_four_gigabytes(kv):
     nq, nkv, d, page = 4, 2, 128, 64
     stride = 1 << 14
     rows = (5 << 30) // (stride * (2 if kv == "bf16" else 1)) // page * page
-    case = make_case(43, [(150, 1), (20, 50)])
+    case = make_case(43, [(150, 1), (20, 80)])
     near = Step(case, kv, (nq, nkv, d), 44, gap=stride - nkv * d)
     want, _ = near.run()
     shift = rows - case.rows

@@ -308,3 +308,13 @@ def test_wrappers_check_their_buffers():
             A.dispatch_kv8_cache_write(plan_, q, a["k"], src, q, a["kc"], scales, codes, a["vs"], a["cos"],
                                        table, num_q=16, num_kv=8, half=128, pair_stride=128,
                                        head_dim=256, kv_format="e4m3")
+
+
+def test_splits_fit_the_image_that_was_asked_for():
+    # One kv head: the rounds of row items and the pieces of a prompt block, at their most.
+    for tokens in (1, 5, 33, 65):
+        for ctx in (40, 3000, 30000):
+            case = make_case(11, [(ctx + 17 * i, 1) for i in range(tokens)] + [(ctx, 3), (ctx, 40)])
+            for nq, d in ((16, 128), (16, 512), (1, 256)):
+                st, img, info = plan(case, nq=nq, nkv=1, d=d)
+                assert st == 0, _lib.last_error()
