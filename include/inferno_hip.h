@@ -453,7 +453,7 @@ int32_t ifr_window_attention_bf16(const void* image_dev, const int64_t* info, co
  *          2^-126 at least otherwise
  *   scale = need if the step writes the block's first row; else max(need, the
  *          scale it has), and where that grows, the rows before the step's first
- *          become rounde(code * old / new) (e4m3: exact above its subnormals)
+ *          become code * old / new, to nearest even (e4m3: exact above its subnormals)
  *   code = the value / scale, rounded to nearest even; infinities become the
  *          largest code, NaN stays NaN in e4m3 and becomes 0 in int8
  * Rows behind the step's tokens keep their bytes.  Refused where two of the

@@ -485,7 +485,8 @@ int32_t attention(int format, const void* image, const int64_t* info, const void
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(output, 16))
     return fail(IFR_EINVAL, "q, the caches and output must be 16-byte aligned");
   if (format != kBf16 && info[kInBlock] == 0) return fail(IFR_EINVAL, "the plan has no block_len: it was made for a bf16 cache");
-  if (!(scale > 0.0f) || !isfinite(scale)) return fail(IFR_EINVAL, "scale must be positive and finite");
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!(scale > 0.0f) || !isfinite(scale_log2)) return fail(IFR_EINVAL, "scale must be positive, and finite times log2 e");
   if (info[kInWorkspace] > 0) {
     if (!workspace || workspace_bytes < info[kInWorkspace])
       return fail(IFR_ESPACE, "workspace of %lld bytes, the plan needs %lld", (long long)(workspace ? workspace_bytes : 0),
@@ -511,7 +512,7 @@ int32_t attention(int format, const void* image, const int64_t* info, const void
   a.block_shift = info[kInBlock] > 0 ? static_cast<int>(shift_of(info[kInBlock])) : 0;
   a.window = static_cast<int>(info[kInWindow]);
   a.sinks = static_cast<int>(info[kInSinks]);
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale_log2;
   const hipStream_t s = reinterpret_cast<hipStream_t>(static_cast<uintptr_t>(stream));
   const int dim = static_cast<int>(head_dim);
   hipError_t e = hipSuccess;

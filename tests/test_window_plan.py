@@ -318,3 +318,10 @@ def test_splits_fit_the_image_that_was_asked_for():
             for nq, d in ((16, 128), (16, 512), (1, 256)):
                 st, img, info = plan(case, nq=nq, nkv=1, d=d)
                 assert st == 0, _lib.last_error()
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+def test_a_scale_that_overflows_with_log2_e_is_refused(kv8):
+    case = make_case(12, [(100, 1)])
+    _, img, info = plan(case, block=64 if kv8 else 0)
+    assert _attend(info, img, kv8, scale=3.0e38) == -1
