@@ -19,17 +19,16 @@
 // accumulators are rarely multiplied.
 //
 // Measured: 4 prompts of 2,048 new tokens, 16 q and 8 kv heads of 256, on up to 7,693 positions of
-// an int8 cache: 769 us, 890 TFLOP/s of what the mask leaves; with a window of 1,024 on a bf16 cache
-// 177 us.  The time is the sum of its parts (repeated calls, 735 us: without the products 430, without
-// the softmax 690, without loading and converting 560), as the two waves of a SIMD do the same thing
-// at the same time, at the rate of the pipe that does it; two waves is what 256 registers each leave.
-// Tried: the second half of the waves with its barrier behind the scores instead of ahead of them, so
-// that one wave's products meet the other's softmax: 5 % faster here, 6 to 8 % slower for short pieces
-// and at head_dim 128 (a longer start, more registers); the halves apart by a second barrier in each
-// step: 790 us against 735; scores of the next tile between the weights of this one: 810; 16x16x32
-// products with two or three column tiles a wave: 815.  A group of two tiles a barrier made no
-// difference, nor did fewer instructions for addresses.  Stores of whole cache lines over LDS save 15
-// us of the second's 206.
+// an int8 cache: 700 us, 970 TFLOP/s of what the mask leaves; with a window of 1,024 on a bf16 cache
+// 178 us.  With all waves at the same thing at the same time the first takes 769 to 785 us, the sum
+// of its parts, each at the rate of the pipe that does it (repeated calls, 735 us: without the products
+// 430, without the softmax 690, without loading and converting 560); two waves a SIMD is what 256
+// registers each leave.  The halves of the waves apart (see the walk) cost a longer start, 3 % of a
+// piece of 29 tiles; at head_dim 128 they are not, as the registers that it takes there cost 2 to 5 %.
+// Tried and slower: a second barrier in each step between the halves' parts (790 us against 735);
+// scores of the next tile between the weights of this one (810); 16x16x32 products with two or three
+// column tiles a wave (815).  A group of two tiles a barrier made no difference, nor did fewer
+// instructions for addresses.  Stores of whole cache lines over LDS save 15 us of the second's 206.
 #include <float.h>
 
 #include <type_traits>
@@ -165,14 +164,16 @@ struct Prompt {
   static constexpr int kRowBytes = 2 * kD;                                     // of a tile row in LDS
   static constexpr int kTileBytes = kTileKeys * kRowBytes;
   static constexpr int kStageBytes = kTileKeys * kD * elt_bytes(kFormat);  // of K, or V, as it comes from the cache
-  // Places of K and V: of rows, and of 8-bit codes.  8-bit at head_dim 512: LDS holds no second
-  // place for the rows, so they are converted between two barriers.
-  static constexpr bool kApart = kFormat != kBf16 && kD == 512;
-  static constexpr int kRowPlaces = kApart ? 1 : kFormat == kBf16 && kD < 512 ? 3 : 2;
-  static constexpr int kCodePlaces = kFormat == kBf16 ? 0 : 2;
+  // How the waves go over the tiles (see the walk): at head_dim 256 in two halves, at 512 the 8-bit
+  // rows between two barriers of their own, as LDS holds no second place for them.
+  static constexpr bool kApart = kFormat != kBf16 && kD == 512, kSkew = kD == 256;
+  // Places of K and V: of rows, and of 8-bit codes.
+  static constexpr int kRowPlaces =
+      kFormat == kBf16 ? (kSkew ? 4 : kD == 512 ? 2 : 3) : kApart ? 1 : kSkew ? 3 : 2;
+  static constexpr int kCodePlaces = kFormat == kBf16 ? 0 : kSkew ? 3 : 2;
   // A step on one tile loads the tile this far behind it, into the place of a tile whose readers
-  // the barrier at its start has seen end.
-  static constexpr int kLead = kFormat == kBf16 ? kRowPlaces - 1 : kApart ? 1 : 2;
+  // a barrier has seen end.
+  static constexpr int kLead = kSkew ? (kFormat == kBf16 ? 3 : 4) : kFormat == kBf16 ? kRowPlaces - 1 : kApart ? 1 : 2;
   static constexpr int kCodesAt = 2 * kRowPlaces * kTileBytes;
   static constexpr int kPosAt = kCodesAt + 2 * kCodePlaces * kStageBytes;  // the columns' positions
   static constexpr int kLds = kPosAt + kPromptWaves * 256 * kNc;
@@ -590,8 +591,18 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
   } else {
     // Between the products of a step's scores the loads of a later tile are started, and between
     // those of its sums the codes of the next tile become rows.
+    //
+    // At head_dim 256 the second half of the waves, the others of the first half's SIMDs, has its
+    // barrier of a step behind the scores instead of ahead of them, so that one wave of a SIMD has
+    // products to do while the other is at its softmax.  Between barriers t and t + 1 the first half
+    // reads K and V of tile t, the second V of tile t and K of tile t + 1.  What is written there,
+    // between the products of the sums: bf16, the loads of tile t + 3, to the place of tile t - 1,
+    // whole by barrier t + 2; 8-bit, the rows of tile t + 2, to the place of tile t - 1, from codes
+    // that were whole by barrier t, and the loads of the codes of tile t + 4, to the place of those of
+    // tile t + 1.
     constexpr int kLead = P::kLead;
-    constexpr bool kCodes = kFormat != kBf16, kApart = P::kApart;
+    constexpr bool kCodes = kFormat != kBf16, kApart = P::kApart, kSkew = P::kSkew;
+    constexpr int kTileLoads = 2 * kLoads;  // of a wave
     constexpr int kLoadPlaces = kCodes ? P::kCodePlaces : P::kRowPlaces;
     int32_t row = row_at(0, entry_at(0)), row_next = row;  // of the tile loaded next; of the one that a step converts
     int32_t entry = entry_at(1);
@@ -602,36 +613,58 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
     };
     int load_place = 0, row_place = 0;
     auto next_place = [](int& place, int places) { place = place + 1 == places ? 0 : place + 1; };
-    int32_t row_0 = row;
-#pragma unroll
-    for (int t = 0; t < kLead; ++t) {
-      load_k(t, row, t);
-      load_v(t, row, t);
+    auto load_next = [&](int t) {
+      load_k(t, row, load_place);
+      load_v(t, row, load_place);
       advance(t);
-    }
-    load_place = kLead % kLoadPlaces;
-    if constexpr (kCodes && !kApart) {
-      begin();
-      rows_from(0, 0, row_0, 0);
-    }
-
-    for (int t = 0; t < num; ++t) {
-      // All loads that this step needs: all but those of the step before, if they were started.
-      if (kLead == 2 && !kCodes && t + 1 < num) wait_loads<2 * kLoads>();
+      next_place(load_place, kLoadPlaces);
+    };
+#pragma unroll
+    for (int t = 0; t < (kLead < 3 ? kLead : 3); ++t) load_next(t);
+    if constexpr (kSkew) {  // the first two tiles have come
+      if (2 < num) wait_loads<kTileLoads>();
       else wait_loads<0>();
       lds_barrier();
+    } else if constexpr (kCodes && !kApart) {
+      begin();
+    }
+    if constexpr (kCodes && !kApart) {
+      rows_from(0, 0, row_at(0, entry_at(0)), 0);
+      if constexpr (kSkew) {
+        rows_from(1, 1, row_at(1, entry_at(1)), 1);
+        lds_barrier();
+        load_next(3);
+      }
+    }
+    int32_t entry_2 = kCodes && kSkew ? entry_at(2) : 0;  // of the tile that a step converts
+    // What a step needs has come: all loads but those of the last tile, if they were started.
+    auto step_begin = [&](int t) {
+      constexpr int kMore = kSkew ? (kCodes ? 3 : 2) : kLead == 2 && !kCodes ? 1 : 0;
+      if (kMore > 0 && t + kMore < num) wait_loads<kTileLoads>();
+      else wait_loads<0>();
+      lds_barrier();
+    };
+    const bool late = kSkew && wave >= kWaves / 2;
+
+    for (int t = 0; t < num; ++t) {
+      if (!late) step_begin(t);
       if constexpr (kApart) {
-        load_k(t + 1, row, load_place);
-        load_v(t + 1, row, load_place);
-        rows_from(load_place ^ 1, 0, row_next, t);
-        advance(t + 1);
+        const int32_t row_here = row_next;
+        load_next(t + 1);
+        rows_from(load_place, 0, row_here, t);
         lds_barrier();
       }
       Scores x;
       Scales ks{}, vs{};
       score_tile(rows_at(false, row_place), x, [&](auto number) {
         constexpr int i = number;
-        if constexpr (!kApart) {
+        if constexpr (kSkew && kCodes && i == 4) {
+          const int32_t row_2 = row_at(t + 2, entry_2);
+          ks = scales_of(false, row_2);
+          vs = scales_of(true, row_2);
+          entry_2 = entry_at(t + 3);
+        }
+        if constexpr (!kSkew && !kApart) {
           if constexpr (i == 1) load_k(t + kLead, row, load_place);
           if constexpr (i == 3) load_v(t + kLead, row, load_place);
           if constexpr (i == 4) {
@@ -643,6 +676,7 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
           }
         }
       });
+      if (late) step_begin(t);
       Weights w;
       soften(x, w, t);
       Turn turn;
@@ -653,16 +687,25 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
           // A word of a turn's four at a time, two products behind their read.
           static_assert(kFrags >= 6 * kTurns);
           constexpr int kTurn = i / 6, kWord = i % 6 - 2;
+          const int tile = kSkew ? t + 2 : t + 1;
+          const int rows = kSkew ? (row_place == 0 ? 2 : row_place - 1) : row_place ^ 1;
+          const int codes = kSkew ? rows : load_place ^ 1;  // both rings of three: tile t + 2's place is that of t - 1
           if constexpr (kTurn < kTurns && kWord == -2)
-            turn = take(kTurn, codes_at(false, load_place ^ 1), codes_at(true, load_place ^ 1), ks, vs, pos_at(t + 1));
+            turn = take(kTurn, codes_at(false, codes), codes_at(true, codes), ks, vs, pos_at(tile));
           if constexpr (kTurn < kTurns && kWord >= 0) {
             const u32x2_t y = codes4_scaled<kFormat>(turn.code[kWord], turn.scale);
             if constexpr (kWord % 2 == 0) half = y;
-            else put_row(kTurn, kWord / 2, turn, half, y, rows_at(false, row_place ^ 1), rows_at(true, row_place ^ 1));
+            else put_row(kTurn, kWord / 2, turn, half, y, rows_at(false, rows), rows_at(true, rows));
           }
         }
+        if constexpr (kSkew) {
+          constexpr int kFrom = kCodes ? 6 * kTurns : 1;
+          if constexpr (i == kFrom) load_k(t + kLead, row, load_place);
+          if constexpr (i == kFrom + 1) load_v(t + kLead, row, load_place);
+          if constexpr (i == kFrags - 1) advance(t + kLead);
+        }
       });
-      next_place(load_place, kLoadPlaces);
+      if constexpr (!kApart) next_place(load_place, kLoadPlaces);
       next_place(row_place, P::kRowPlaces);
     }
   }
