@@ -218,8 +218,9 @@ __global__ __launch_bounds__(kThreads) void kv8_write_kernel(const Kv8WriteArgs 
     if (r < count) write(r, held[i]);
   }
   for (int r = kHeld * kRows + tr; r < count; r += kRows) write(r, values(r));
-  // Older rows under a scale that grew.
-  if (old > 0.0f && now > old) {
+  // Older rows under a scale that grew.  From 0 it makes their codes 0: they were worth that (an
+  // infinity among rows of zeros has the largest code).
+  if (before > 0 && now > old) {
     const float ratio = old * inv;
     for (int r = tr; r < before; r += kRows) {
       const int64_t row = row0 - before + r;
