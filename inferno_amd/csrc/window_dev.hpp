@@ -53,19 +53,17 @@ __device__ __forceinline__ u32x2_t codes4_bf16(uint32_t w) {
   }
 }
 
-// The same, times a power of two (or 0).  int8 as unsigned bytes of 128 more, one conversion
-// each: the fma takes 128 off again, exactly, as its result has 8 significant bits.
+// The same, times a power of two (or 0): exact where the product is a bf16 number, which a finite one
+// above 2^-126 is.
 template <int kFormat>
 __device__ __forceinline__ u32x2_t codes4_scaled(uint32_t w, float scale) {
   if constexpr (kFormat == kE4m3) {
     return u32x2_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false)),
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))};
   } else {
-    const uint32_t u = w ^ 0x80808080u;
-    const float off = -128.0f * scale;
     float x[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(static_cast<float>((u >> (8 * i)) & 0xFFu), scale, off);
+    for (int i = 0; i < 4; ++i) x[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i))) * scale;
     return u32x2_t{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
   }
 }

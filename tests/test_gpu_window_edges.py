@@ -1,9 +1,12 @@
-"""The window and 8-bit cache operators where their numbers are at an end: blocks that grow from a scale of 0."""
+"""The window and 8-bit cache operators where their numbers are at an end: blocks that grow from a scale of 0, scales
+at the top of f32's range.  Against the definition in 64 bits."""
 import numpy as np
 import pytest
+import torch
 
 from tests.gpu_util import announce
 from tests.test_gpu_kv8_write import Cache, make_plan, same_codes, tables, write
+from tests.test_gpu_window import Step
 from tests.window_util import bf16, code_values, make_case, round_code, to_codes
 
 pytestmark = pytest.mark.gpu
@@ -46,3 +49,49 @@ def test_a_block_that_grows_from_a_scale_of_zero(kv):
         s = float(scales[row[0] // 32, 0])
         if i == 1:
             same_codes(raw[row[2]], to_codes(round_code(token[0, 0] / np.float64(s), kv), kv), kv, "token")
+
+
+def values_of(step):
+    """k and v of a Step as its codes and scales have them now (8 bits)."""
+    out = []
+    for raw, scales in zip(step.raw, step.scales):
+        codes = code_values(raw[:, :step.nkv * step.d].cpu().numpy(), step.kv).reshape(-1, step.nkv, step.d)
+        out.append(codes * np.repeat(scales.cpu().numpy(), step.block, 0)[:, :, None])
+    return out
+
+
+def faint_queries(step, seed):
+    """Queries of a few values of 2^-126 and the next ones, of any sign, and for the first token all 0."""
+    rng = np.random.default_rng(seed)
+    q = rng.integers(-2, 3, step.q.shape) * (rng.random(step.q.shape) < 1 / 16) * 2.0 ** -126
+    q[0] = 0.0
+    step.q = q.astype(np.float32)
+    step.q_dev = torch.from_numpy(step.q).to(torch.bfloat16).cuda()
+
+
+@pytest.mark.parametrize("shape", [(2, 1, 128), (2, 1, 256), (4, 1, 512)])
+def test_int8_prompts_under_the_largest_scales(shape):
+    """Scales of 2^121 and 2^122 (the largest that the write makes), in v and in k."""
+    announce(f"window int8 largest scales {shape}")
+    n, d = 80, shape[2]
+    rng = np.random.default_rng(4)
+    for e, most in ((121, 127), (122, 63)):
+        # One visible position: the result is the row.
+        case = make_case(5, [(70, n)], window=1)
+        step = Step(case, "int8", shape, 6)
+        codes = rng.integers(-most, most + 1, (case.rows, shape[1] * d)).astype(np.int8)
+        step.raw[1] = torch.from_numpy(codes).view(torch.uint8).cuda()
+        step.scales[1][:] = 2.0 ** e
+        got, plan = step.run()
+        assert plan.info[14] > 0
+        at = case.row(0, np.arange(70, 70 + n))
+        want = (codes[at].astype(np.float64) * 2.0 ** e).reshape(n, 1, d)
+        assert np.array_equal(got, np.broadcast_to(want, got.shape)), e
+        # The same in k.
+        step = Step(make_case(7, [(70, n)]), "int8", shape, 8)
+        codes = rng.integers(-most, most + 1, (step.case.rows, shape[1] * d)).astype(np.int8)
+        step.raw[0] = torch.from_numpy(codes).view(torch.uint8).cuda()
+        step.scales[0][:] = 2.0 ** e
+        step.k = values_of(step)[0]
+        faint_queries(step, 9)
+        step.check(f"k 2^{e}", scale=1.0 / 16)
