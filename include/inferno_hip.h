@@ -441,7 +441,7 @@ int32_t ifr_window_attention_bf16(const void* image_dev, const int64_t* info, co
 
 /* The 8-bit cache: codes [row][kv_stride] of 1 byte, OCP e4m3 or int8, and f32
  * scales [row / block_len][num_kv], zero or a power of two; the value is code *
- * scale. */
+ * scale, which f32 has to hold. */
 #define IFR_KV8_E4M3 1
 #define IFR_KV8_INT8 2
 
@@ -454,8 +454,10 @@ int32_t ifr_window_attention_bf16(const void* image_dev, const int64_t* info, co
  *   scale = need if the step writes the block's first row; else max(need, the
  *          scale it has), and where that grows, the rows before the step's first
  *          become code * old / new, to nearest even (e4m3: exact above its subnormals)
- *   code = the value / scale, rounded to nearest even; infinities become the
- *          largest code, NaN stays NaN in e4m3 and becomes 0 in int8
+ *   code = the value / scale, rounded to nearest even, and of the codes whose
+ *          product with the scale f32 holds (all but those above 240 under 2^120
+ *          in e4m3, above 63 under 2^122 in int8); infinities become the largest
+ *          of them, NaN stays NaN in e4m3 and becomes 0 in int8
  * Rows behind the step's tokens keep their bytes.  Refused where two of the
  * step's runs write to the same rows.  half and pair_stride: multiples of 8. */
 int32_t ifr_kv8_cache_write(const void* image_dev, const int64_t* info, const void* q_src,

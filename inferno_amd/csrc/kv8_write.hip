@@ -14,6 +14,8 @@
 //
 // Bound by HBM for prompts (k, v, q once, codes once): 2 x 2,048 tokens of 16 q and 8 kv heads of 256
 // take 25 us, 4.9 TB/s; by a launch's latency for single tokens: 64 of them 8 us.
+#include <float.h>
+
 #include "window_dev.hpp"
 
 namespace ifr {
@@ -78,14 +80,22 @@ __device__ __forceinline__ uint32_t scale_bits(float amax) {
   return static_cast<uint32_t>(max(e, 1)) << 23;
 }
 
-// x (already divided by the scale) to a code: nearest even, saturating; NaN stays (e4m3) or
+// The largest code times `scale`, inv = 1 / scale, that f32 (and so bf16) holds: 240 under 2^120
+// in e4m3, 63 under 2^122 in int8, where the nearest code of the largest bf16 values stands for 2^128.
+template <int kFormat>
+__device__ __forceinline__ float top_code(float inv) {
+  if constexpr (kFormat == kE4m3) return fminf(448.0f, 0x1.Ep127f * inv);  // 240 * 2^120: 448 * 2^119 is less
+  else return fminf(127.0f, __builtin_floorf(FLT_MAX * inv));
+}
+
+// x (already divided by the scale) to a code: nearest even, at most top; NaN stays (e4m3) or
 // becomes 0 (int8).
 template <int kFormat>
-__device__ __forceinline__ uint32_t codes4(const float* x) {
+__device__ __forceinline__ uint32_t codes4(const float* x, float top) {
   if constexpr (kFormat == kE4m3) {
     float y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_fmed3f(x[i], -448.0f, 448.0f);
+    for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_fmed3f(x[i], -top, top);
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
     w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
     uint32_t r = static_cast<uint32_t>(w);
@@ -97,7 +107,7 @@ __device__ __forceinline__ uint32_t codes4(const float* x) {
     uint32_t r = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float y = x[i] == x[i] ? __builtin_rintf(__builtin_amdgcn_fmed3f(x[i], -127.0f, 127.0f)) : 0.0f;
+      const float y = x[i] == x[i] ? __builtin_rintf(__builtin_amdgcn_fmed3f(x[i], -top, top)) : 0.0f;
       r |= (static_cast<uint32_t>(static_cast<int32_t>(y)) & 0xFFu) << (8 * i);
     }
     return r;
@@ -200,10 +210,11 @@ __global__ __launch_bounds__(kThreads) void kv8_write_kernel(const Kv8WriteArgs 
 
   // A power of two of at most 2^126: exact.  Under a scale of 0 every finite value is 0.
   const float inv = now > 0.0f ? 1.0f / now : 1.0f;
+  const float top = top_code<kFormat>(inv);
   auto store = [&](int64_t row, const float* x) {
     u32x2_t w;
-    w[0] = codes4<kFormat>(x);
-    w[1] = codes4<kFormat>(x + 4);
+    w[0] = codes4<kFormat>(x, top);
+    w[1] = codes4<kFormat>(x + 4, top);
     *reinterpret_cast<u32x2_t*>(cache + row * a.kv_stride) = w;
   };
   auto write = [&](int r, const Chunk& c) {

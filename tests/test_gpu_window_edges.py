@@ -95,3 +95,41 @@ def test_int8_prompts_under_the_largest_scales(shape):
         step.k = values_of(step)[0]
         faint_queries(step, 9)
         step.check(f"k 2^{e}", scale=1.0 / 16)
+
+
+TOP = float(np.float32(255 * 2.0 ** 120))  # the largest bf16
+
+
+@pytest.mark.parametrize("kv", ["e4m3", "int8"])
+def test_what_is_written_reads_as_finite_values(kv):
+    """The largest bf16 values, and infinities beside them: where the nearest code times the scale is 2^128, the code below."""
+    announce(f"kv8 top of the range {kv}")
+    first = bf16(np.random.default_rng(10).standard_normal((2, 1, 128)))
+    for dim, x in ((20, TOP), (21, -TOP), (22, 2.0 ** 127), (23, 248 * 2.0 ** 120), (24, -2.0 ** 126)):
+        first[0, 0, dim] = x
+    first[1, 0, 25], first[1, 0, 26] = np.inf, -np.inf
+    want = {"e4m3": [240, -240, 128, 240, -64, 240, -240], "int8": [63, -63, 32, 62, -16, 63, -63]}[kv]
+    scale = 2.0 ** (120 if kv == "e4m3" else 122)
+    cos, sin = tables(make_case(1, [(0, 64)]), 8)
+    cache = Cache(4 * 64, 1, 128, kv, 32, 11)
+    whole = steps_of([(32, 2)], WRITE, kv, cache, cos, sin, (first, first))
+    row = whole.row(0, np.arange(32, 35))
+    for i in range(2):
+        raw, scales = cache.got(i)
+        assert scales[row[0] // 32, 0] == scale
+        held = code_values(raw[row[:2]], kv)
+        assert [*held[0, 20:25], *held[1, 25:27]] == want, held[:, 20:27]
+        with np.errstate(over="ignore"):
+            assert np.isfinite(held * np.float32(scale)).all()
+    # A block of the next smaller scale and its largest code, which grows.
+    old = np.zeros((1, 1, 128), dtype=np.float32)
+    old[0, 0, 30] = 448 * 2.0 ** 119 if kv == "e4m3" else 127 * 2.0 ** 121
+    old[0, 0, 31] = -old[0, 0, 30]
+    cache = Cache(4 * 64, 1, 128, kv, 32, 12)
+    steps_of([(32, 1), (33, 1)], WRITE, kv, cache, cos, sin, (old, old), (first[:1], first[:1]))
+    for i in range(2):
+        raw, scales = cache.got(i)
+        assert scales[row[0] // 32, 0] == scale
+        held = code_values(raw[row[:2]], kv)
+        assert list(held[0, 30:32]) == ([224, -224] if kv == "e4m3" else [63, -63])
+        assert list(held[1, 20:25]) == want[:5]
