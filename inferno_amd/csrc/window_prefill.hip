@@ -438,18 +438,25 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
   struct Weights {
     u32x4_t p[S::kParts][kNc];
   };
+  // Rounded to bf16 for the product, each off by 2^-8 of itself at most.  The sum of weights takes them
+  // rounded too: the result is the exact softmax of the rounded weights, off by 2^-8 sum p |v - o| at
+  // most.  With the weights as they were in the sum a row of which one weight is nearly all, 2^x with any
+  // x below kSlack, was off by that weight's own rounding, up to another 2^-8 of the whole result.
   auto weigh = [&](const Scores& x, Weights& w) {
+    const bf16x2_t ones = bf16x2_t{1.0f, 1.0f};
 #pragma unroll
     for (int n = 0; n < kNc; ++n) {
       float even = 0.0f;
 #pragma unroll
       for (int j = 0; j < S::kScores; ++j) {
         const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x.get(n, j), a.scale_log2, -m[n]));
-        l[n] += v;
-        // Rounded to bf16 for the product: off by 2^-8 of each weight at most, which
-        // independent values average to less than the result's own rounding.
-        if (j & 1) w.p[j >> 3][n][(j & 7) >> 1] = pack_bf16(even, v);
-        else even = v;
+        if (j & 1) {
+          const uint32_t two = pack_bf16(even, v);
+          w.p[j >> 3][n][(j & 7) >> 1] = two;
+          l[n] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, two), ones, l[n], false);
+        } else {
+          even = v;
+        }
       }
     }
   };

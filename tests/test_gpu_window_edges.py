@@ -1,5 +1,7 @@
 """The window and 8-bit cache operators where their numbers are at an end: blocks that grow from a scale of 0, scales
-at the top of f32's range.  Against the definition in 64 bits."""
+at the top of f32's range, rows of weights of which one has nearly all.  Against the definition in 64 bits."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -11,6 +13,7 @@ from tests.window_util import bf16, code_values, make_case, round_code, to_codes
 
 pytestmark = pytest.mark.gpu
 
+KINDS = ["bf16", "e4m3", "int8"]
 WRITE = (2, 1, 128, 8, 64)  # q and kv heads, head_dim, rotated pairs of dims 0-7 and 64-71
 
 
@@ -133,3 +136,70 @@ def test_what_is_written_reads_as_finite_values(kv):
         held = code_values(raw[row[:2]], kv)
         assert list(held[0, 30:32]) == ([224, -224] if kv == "e4m3" else [63, -63])
         assert list(held[1, 20:25]) == want[:5]
+
+
+def shared_rounding64(case, q, k, v, scale, gqa, step):
+    """(o, bound) where numerator and denominator take the same rounded weights, each off by `step` of itself at most.
+
+    o' = sum p (1 + e) v / sum p (1 + e), |e| <= step:  o' - o = sum p e (v - o) / sum p (1 + e), at most
+    step / (1 - step) sum p |v - o|, and 1 / (1 - step) < 1 + 2 step.  The rest as in attention64: 2^-8 |o|, the result's own
+    rounding; (2 (ds + n 2^-24) + 2^-18) sum p |v|; n 2^-116 (1 + max |v|)."""
+    o, bound = (np.zeros(q.shape) for _ in range(2))
+    t = 0
+    for r, (c, n) in enumerate(case.lens):
+        rows = case.row(r, np.arange(c + n))
+        for h in range(q.shape[1]):
+            kk, vv = k[rows, h // gqa].astype(np.float64), v[rows, h // gqa].astype(np.float64)
+            for i in range(n):
+                kp, vp, qq = kk[:c + i + 1], vv[:c + i + 1], q[t + i, h].astype(np.float64)
+                s = kp @ qq * scale
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                x = w @ vp
+                ds = (q.shape[2] + 4) * 2.0 ** -24 * scale * (np.abs(kp) @ np.abs(qq)).max()
+                m = len(s)
+                o[t + i, h] = x
+                bound[t + i, h] = (2.0 ** -8 * np.abs(x) + step * (1 + 2 * step) * (w @ np.abs(vp - x))
+                                   + (2 * (ds + m * 2.0 ** -24) + 2.0 ** -18) * (w @ np.abs(vp)) + m * 2.0 ** -116 * (1 + np.abs(vp).max()))
+        t += n
+    return o, bound
+
+
+def one_sharp_position(step, at, lo, hi, seed, v_size=1.0):
+    """Scores near 0 in powers of two, but for position `at` of each run, which is at lo to hi, another for each query; v times
+    v_size."""
+    rng = np.random.default_rng(seed)
+    step.k, step.v = bf16(step.k * 2.0 ** -7), bf16(step.v * v_size)
+    step.k[:, :, 0] = 0.0
+    step.k[[int(step.case.row(r, at)) for r in range(len(step.case.lens))], :, 0] = 1.0
+    step.q = bf16(step.q / 2.0)
+    scale = 1 / math.sqrt(step.d)
+    step.q[:, :, 0] = bf16(rng.uniform(lo, hi, step.q.shape[:2]) * math.log(2.0) / scale)
+    step.q_dev = torch.from_numpy(step.q).to(torch.bfloat16).cuda()
+    for i, x in enumerate((step.k, step.v)):
+        if step.kv == "bf16":
+            step.raw[i] = step.wide(torch.from_numpy(x).to(torch.bfloat16))
+            continue
+        s = 2.0 ** -6 if i == 0 else v_size * 2.0 ** -5
+        step.raw[i] = step.wide(torch.from_numpy(to_codes(round_code(x.astype(np.float64) / s, step.kv).reshape(x.shape), step.kv)))
+        step.scales[i][:] = s
+    if step.kv != "bf16":
+        step.k, step.v = values_of(step)
+
+
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("shape", [(4, 2, 128), (4, 2, 256), (4, 1, 512)])
+def test_a_position_that_has_nearly_all_of_the_weight(shape, kv):
+    """A prompt's scores pass the maximum of their first tile by 10 to 20 powers of two: such a weight's rounding is in the sum of
+    weights too, so that next to nothing of it is left in the result."""
+    announce(f"window sharp weights {shape} {kv}")
+    case = make_case(13, [(100, 80), (40, 70)])
+    step = Step(case, kv, shape, 14)
+    one_sharp_position(step, 38, 10.0, 20.0, 15)
+    got, plan = step.run()
+    assert plan.info[14] > 0
+    want, bound = shared_rounding64(case, step.q, step.k, step.v, 1 / math.sqrt(step.d), shape[0] // shape[1], 2.0 ** -8)
+    far = np.abs(got - want)
+    print(f"  {shape} {kv}: {float((far / bound).max()):.3f} of the bound, relative rms {float(np.sqrt((far ** 2).sum() / (want ** 2).sum())):.2e}",
+          flush=True)
+    assert (far <= bound).all()
