@@ -401,7 +401,8 @@ int32_t ifr_bq_block_quant(const void* src, void* x_i8, float* x_sa, int64_t col
  * over j in visible(p), m = max_j s_j; sums and products in f32, the weights of
  * a sum over v in bf16 (decode: two bf16 parts), o rounded once to bf16.  What
  * a position holds that a query does not see does not enter its result, be it
- * infinite or NaN.
+ * infinite or NaN.  The sum of |v| over the positions that a query sees has to
+ * stay in f32's range; weights below 2^-110 of the largest count as 0.
  *
  * head_dim 128, 256 or 512; 1 to 16 q heads a kv head; pages of 32 rows or more.
  * q and output [seq_len][num_q][head_dim] bf16, 16-byte aligned; caches

@@ -14,9 +14,10 @@
 // scales, between the products of the tile before (exactly: a code has at most 8 significant bits
 // and a scale is a power of two).
 //
-// The maximum of a column's softmax is only moved when a score passes it by 24 powers of two: the
-// weights are then at most 2^24, which f32 sums and bf16's exponent hold with room, and the
-// accumulators are rarely multiplied.
+// Weights are 2^(score - m) with an m that lies up to 16 powers of two above the column's largest score
+// so far, and is only moved when a score passes it: the accumulators are rarely multiplied, and the
+// weights are at most 1, so that no sum passes what sum |v| over the positions seen does.  At the
+// other end a weight below 2^-110 of the largest counts as 0, and a result below 2^-110 loses bits.
 //
 // Measured: 4 prompts of 2,048 new tokens, 16 q and 8 kv heads of 256, on up to 7,693 positions of
 // an int8 cache: 700 us, 970 TFLOP/s of what the mask leaves; with a window of 1,024 on a bf16 cache
@@ -153,7 +154,9 @@ __device__ __forceinline__ void score_mfma(f32x16_t& s, bf16x8_t x, bf16x8_t y) 
   asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(x), "v"(y));
 }
 
-constexpr float kSlack = 24.0f;  // how far scores may pass the maximum in use, in powers of two
+// How far m is put above the score that moves it, in powers of two.  4 prompts of 2,048 tokens with a
+// window of 1,024 take 213 us at 10, 205 at 12, 193 at 14 and 189 at 16, as with 24.
+constexpr float kSlack = 16.0f;
 
 // One block.  False if a sum came out that is not finite: the block is then done again with
 // kCareful, which stores over it (two functions, so that the registers of one do not weigh
@@ -407,12 +410,12 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
 #pragma unroll
     for (int i = 0; i < kBlocks * kNc; ++i) asm volatile("" : "+a"(acc[i / kNc][i % kNc]));
   };
-  // Moves the maxima that x passes.
-  auto move_maxima = [&](const float* top, bool first) {
+  // Moves the references that a score passes.
+  auto move_references = [&](const float* top, bool first) {
     float corr[kNc];
 #pragma unroll
     for (int n = 0; n < kNc; ++n) {
-      const float m_new = top[n] > m[n] + kSlack ? top[n] : m[n];
+      const float m_new = top[n] > m[n] ? top[n] + kSlack : m[n];
       corr[n] = m_new == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - m_new);
       m[n] = m_new;
       l[n] *= corr[n];
@@ -440,7 +443,7 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
   };
   // Rounded to bf16 for the product, each off by 2^-8 of itself at most.  The sum of weights takes them
   // rounded too: the result is the exact softmax of the rounded weights, off by 2^-8 sum p |v - o| at
-  // most.  With the weights as they were in the sum a row of which one weight is nearly all, 2^x with any
+  // most.  With the weights as they were in the sum a row of which one weight is nearly all, 2^-x with any
   // x below kSlack, was off by that weight's own rounding, up to another 2^-8 of the whole result.
   auto weigh = [&](const Scores& x, Weights& w) {
     const bf16x2_t ones = bf16x2_t{1.0f, 1.0f};
@@ -555,9 +558,9 @@ __device__ __forceinline__ bool prompt_block(const WindowArgs& a, int off_items,
 #pragma unroll
     for (int n = 0; n < kNc; ++n) {
       top[n] = top_of(x, n);
-      move |= top[n] > m[n] + kSlack;
+      move |= top[n] > m[n];
     }
-    if (__builtin_amdgcn_ballot_w64(move) != 0) move_maxima(top, t == 0);
+    if (__builtin_amdgcn_ballot_w64(move) != 0) move_references(top, t == 0);
     weigh(x, w);
   };
   auto begin = [&] {

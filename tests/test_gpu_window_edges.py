@@ -143,7 +143,8 @@ def shared_rounding64(case, q, k, v, scale, gqa, step):
 
     o' = sum p (1 + e) v / sum p (1 + e), |e| <= step:  o' - o = sum p e (v - o) / sum p (1 + e), at most
     step / (1 - step) sum p |v - o|, and 1 / (1 - step) < 1 + 2 step.  The rest as in attention64: 2^-8 |o|, the result's own
-    rounding; (2 (ds + n 2^-24) + 2^-18) sum p |v|; n 2^-116 (1 + max |v|)."""
+    rounding; (2 (ds + n 2^-24) + 2^-18) sum p |v|.  A prompt's largest weight is 2^-16 at least, and exp2, bf16 and the
+    products take what is below 2^-126 to 0: less than 2^-110 (2 |v| + 1) for each position, and n 2^-108 (1 + max |v|) for all."""
     o, bound = (np.zeros(q.shape) for _ in range(2))
     t = 0
     for r, (c, n) in enumerate(case.lens):
@@ -160,7 +161,7 @@ def shared_rounding64(case, q, k, v, scale, gqa, step):
                 m = len(s)
                 o[t + i, h] = x
                 bound[t + i, h] = (2.0 ** -8 * np.abs(x) + step * (1 + 2 * step) * (w @ np.abs(vp - x))
-                                   + (2 * (ds + m * 2.0 ** -24) + 2.0 ** -18) * (w @ np.abs(vp)) + m * 2.0 ** -116 * (1 + np.abs(vp).max()))
+                                   + (2 * (ds + m * 2.0 ** -24) + 2.0 ** -18) * (w @ np.abs(vp)) + m * 2.0 ** -108 * (1 + np.abs(vp).max()))
         t += n
     return o, bound
 
@@ -203,3 +204,18 @@ def test_a_position_that_has_nearly_all_of_the_weight(shape, kv):
     print(f"  {shape} {kv}: {float((far / bound).max()):.3f} of the bound, relative rms {float(np.sqrt((far ** 2).sum() / (want ** 2).sum())):.2e}",
           flush=True)
     assert (far <= bound).all()
+
+
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("shape", [(4, 2, 128), (4, 2, 256), (4, 1, 512)])
+def test_large_values_under_scores_that_rise(shape, kv):
+    """v of about 2^112, and scores that pass the maximum of their first tile by 17 to 23 powers of two: the sums are finite."""
+    announce(f"window large values {shape} {kv}")
+    case = make_case(16, [(100, 80), (40, 70)])
+    step = Step(case, kv, shape, 17)
+    one_sharp_position(step, 38, 17.0, 23.0, 18, v_size=2.0 ** 112)
+    assert np.isfinite(step.v).all()
+    got, plan = step.run()
+    assert plan.info[14] > 0 and np.isfinite(got).all()
+    want, bound = shared_rounding64(case, step.q, step.k, step.v, 1 / math.sqrt(step.d), shape[0] // shape[1], 2.0 ** -8)
+    assert (np.abs(got - want) <= bound).all()
