@@ -5,7 +5,7 @@
 // 32 positions with the running maximum m and sum l of each column's softmax:
 //
 //   S^T[32 x 16] = K . Q^T          16x16x32 MFMA, K straight from the cache
-//   p = exp2(c s - m), l += p       c = scale * log2 e (* the block's scale)
+//   p = exp2(c s - m), l += p       c = scale * log2 e, s times the block's scale
 //   O^T[D x 16] += V^T . P^T
 //
 // A 16x16x32 MFMA gives lane (c, g) = (lane % 16, lane / 16) the scores of column c at
@@ -184,9 +184,9 @@ void window_rows_kernel(const WindowArgs a, int off_items, int per_group) {
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const float cs = kFormat == kBf16 ? a.scale_log2 : a.scale_log2 * ks[u];
+        // Not times a product of the two factors, which may pass f32's range where the scores do not.
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sc[4 * u + r] = s4[u][r] * cs;
+        for (int r = 0; r < 4; ++r) sc[4 * u + r] = (kFormat == kBf16 ? s4[u][r] : s4[u][r] * ks[u]) * a.scale_log2;
       }
     }
     if (masked) {

@@ -219,3 +219,20 @@ def test_large_values_under_scores_that_rise(shape, kv):
     assert plan.info[14] > 0 and np.isfinite(got).all()
     want, bound = shared_rounding64(case, step.q, step.k, step.v, 1 / math.sqrt(step.d), shape[0] // shape[1], 2.0 ** -8)
     assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("kv,e,most", [("e4m3", 120, 15), ("int8", 122, 63)])
+@pytest.mark.parametrize("shape", [(2, 1, 128), (2, 1, 256), (4, 1, 512)])
+def test_a_scale_of_the_scores_times_the_largest_scale_of_k(shape, kv, e, most):
+    """Their product passes f32's range, the scores do not (of queries of 0 they are 0)."""
+    announce(f"window scale overflow {shape} {kv}")
+    for lens in ([(70, 1), (33, 1)], [(70, 80)]):
+        step = Step(make_case(19, lens), kv, shape, 20)
+        rng = np.random.default_rng(21)
+        codes = rng.integers(-1, 2, (step.case.rows, shape[1] * step.d)).astype(np.float32)
+        codes[:, 1::2] *= most * (rng.random(codes[:, 1::2].shape) < 1 / 64)
+        step.raw[0] = torch.from_numpy(to_codes(codes, kv)).cuda()
+        step.scales[0][:] = 2.0 ** e
+        step.k = values_of(step)[0]
+        faint_queries(step, 22)
+        step.check(f"{lens}", scale=512.0)
