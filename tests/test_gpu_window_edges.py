@@ -236,3 +236,25 @@ def test_a_scale_of_the_scores_times_the_largest_scale_of_k(shape, kv, e, most):
         step.k = values_of(step)[0]
         faint_queries(step, 22)
         step.check(f"{lens}", scale=512.0)
+
+
+@pytest.mark.parametrize("shape", [(2, 1, 128), (2, 1, 256), (2, 1, 512)])
+@pytest.mark.parametrize("kv", ["e4m3", "int8"])
+def test_every_code_in_prompts(shape, kv):
+    """Every code through the prompt kernel, whose conversion is its own: one visible position, so that the result is the row."""
+    announce(f"window all codes in prompts {shape} {kv}")
+    n, d = 80, shape[2]
+    case = make_case(23, [(70, n)], window=1)
+    step = Step(case, kv, shape, 24)
+    raw = np.arange(256, dtype=np.uint8)
+    if kv == "e4m3":
+        raw = np.where((raw & 0x7F) == 0x7F, 0, raw).astype(np.uint8)
+    rng = np.random.default_rng(25)
+    rows = np.stack([rng.permutation(np.resize(np.roll(raw, 128 * i), d)) for i in range(n)])
+    assert len(np.unique(rows)) == (254 if kv == "e4m3" else 256)
+    step.raw[1][torch.from_numpy(case.row(0, np.arange(70, 70 + n))).cuda()] = torch.from_numpy(rows).cuda()
+    step.scales[1][:] = 2.0 ** -5
+    got, plan = step.run()
+    assert plan.info[14] > 0 and plan.info[0] == 0
+    want = code_values(rows, kv).reshape(n, 1, d) * 2.0 ** -5
+    assert np.array_equal(got, np.broadcast_to(want, got.shape))
