@@ -258,3 +258,36 @@ def test_every_code_in_prompts(shape, kv):
     assert plan.info[14] > 0 and plan.info[0] == 0
     want = code_values(rows, kv).reshape(n, 1, d) * 2.0 ** -5
     assert np.array_equal(got, np.broadcast_to(want, got.shape))
+
+
+@pytest.mark.parametrize("kv", KINDS)
+def test_replays_read_the_inputs_of_their_time(kv):
+    """A captured step with other queries in every replay, between eager calls of another step on the same workspace."""
+    announce(f"window replays {kv}")
+    step = Step(make_case(26, [(1500, 1), (40, 1), (300, 90)]), kv, (8, 2, 128), 27)
+    other = Step(make_case(28, [(1200, 1), (100, 70)]), kv, (8, 2, 128), 29)
+    plan, plan2 = step.plan(), other.plan()
+    assert plan.info[0] and plan.info[1] and plan.info[14] and plan2.info[1]
+    ws = torch.empty(max(plan.workspace_bytes, plan2.workspace_bytes) // 4, device="cuda")
+    scale = 1 / math.sqrt(128)
+    queries = [step.q_dev, -step.q_dev, step.q_dev.flip(0).contiguous()]
+    want = []
+    for q in queries:
+        out = torch.empty_like(q)
+        step.attend(plan, out, ws, scale, q)
+        want.append(out)
+    torch.cuda.synchronize()
+    assert not torch.equal(want[0], want[1])
+    out, out2, q = torch.zeros_like(step.q_dev), torch.zeros_like(other.q_dev), step.q_dev.clone()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step.attend(plan, out, ws, scale, q)
+    for r in (1, 0, 2, 1, 1, 2, 0):
+        out.zero_()
+        q.copy_(queries[r])
+        other.attend(plan2, out2, ws, scale)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[r]), r
+    del g
