@@ -1,5 +1,6 @@
-"""The window and 8-bit cache operators where their numbers are at an end: blocks that grow from a scale of 0, scales
-at the top of f32's range, rows of weights of which one has nearly all.  Against the definition in 64 bits."""
+"""The window and 8-bit cache operators where their numbers are at an end (blocks that grow from a scale of 0, scales and values
+at the top of f32's range, rows of weights of which one has nearly all), and in forms that take many sequences or certain lengths
+to be planned.  Against the definition in 64 bits."""
 import math
 
 import numpy as np
@@ -291,3 +292,62 @@ def test_replays_read_the_inputs_of_their_time(kv):
         torch.cuda.synchronize()
         assert torch.equal(out, want[r]), r
     del g
+
+
+def shared_pages_case(lens, page=64, of=3):
+    """Sequences that read the pages of the longest ones of `of` groups."""
+    top = max(c + n for c, n in lens)
+    pool = make_case(30, [(top - 1, 1)] * of, page=page)
+    case = make_case(30, [(0, n) for _, n in lens], page=page)
+    case.lens, case.rows = list(lens), pool.rows
+    case.pages = [pool.pages[r % of][:(c + n - 1) // page + 1] for r, (c, n) in enumerate(lens)]
+    case.table = type(case.table)()
+    t = 0
+    for (c, n), pages in zip(lens, case.pages):
+        case.table.begin_run(t, c)
+        for row in pages:
+            case.table.add_base_row(row)
+        t += n
+    return case
+
+
+# Single sequences, shortest and longest context, kv heads that a work item's waves take, and whether some tokens are split.
+BUSY = [(300, 300, 310, 2, False), (180, 60, 900, 2, True), (256, 500, 520, 4, False), (130, 60, 2500, 4, True)]
+
+
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("shape", [(16, 8, 256), (8, 8, 128), (8, 4, 512)])
+@pytest.mark.parametrize("busy", BUSY)
+def test_busy_decode(busy, shape, kv):
+    """Batches whose work items take two and four kv heads, whole and split, among them runs of a few tokens."""
+    runs, lo, hi, heads, split = busy
+    announce(f"window busy decode {busy} {shape} {kv}")
+    lens = [(int(c), 3 if i % 31 == 7 else 1) for i, c in enumerate(np.linspace(lo, hi, runs))]
+    case = shared_pages_case(lens)
+    step = Step(case, kv, shape, 31)
+    plan = step.plan()
+    assert plan.info[25] == heads and plan.info[14] == 0
+    assert (0 < plan.info[1] < case.seq) if split else plan.info[1] == 0
+    step.check("busy", plan=plan)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("shape", [(16, 8, 256), (8, 8, 128), (8, 4, 512)])
+@pytest.mark.parametrize("busy", [BUSY[0], BUSY[3]])
+def test_busy_decode_of_an_infinite_value(busy, shape, kv):
+    """One dim of one position of v infinite, or NaN: the sequences on that page get it there, and no other value changes a bit."""
+    runs, lo, hi, heads, _ = busy
+    announce(f"window busy decode of infinities {busy} {shape} {kv}")
+    lens = [(int(c), 1) for c in np.linspace(lo, hi, runs)]
+    case = shared_pages_case(lens)
+    step = Step(case, kv, shape, 32)
+    want, plan = step.run()
+    assert plan.info[25] == heads
+    flat = step.raw[1][int(case.row(1, 37))]
+    flat[shape[2] + 3] = float("-inf") if kv == "bf16" else 0x7F  # kv head 1, dim 3
+    got, _ = step.run(plan=plan)
+    gqa = shape[0] // shape[1]
+    hit = np.zeros(got.shape, dtype=bool)
+    hit[1::3, gqa:2 * gqa, 3] = True
+    assert np.array_equal(got[~hit], want[~hit])
+    assert (np.isneginf(got[hit]) if kv == "bf16" else np.isnan(got[hit])).all()
