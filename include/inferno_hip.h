@@ -52,6 +52,7 @@ extern "C" {
 #define IFR_EUNSUPPORTED (-2)  /* shape outside the compiled kernel set */
 #define IFR_EHIP (-3)          /* HIP runtime error */
 #define IFR_ESPACE (-4)        /* caller-provided buffer too small */
+#define IFR_ENOMEM (-5)        /* no host memory (ifr_plan_window) */
 
 #define IFR_ABI_VERSION 1
 

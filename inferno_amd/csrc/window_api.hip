@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <array>
 #include <functional>
+#include <new>
 #include <queue>
 #include <utility>
 #include <vector>
@@ -539,8 +540,12 @@ int32_t ifr_plan_window(void* image, int64_t image_bytes, const int32_t* runs, i
                         int64_t num_rows, int64_t seq_len, int64_t window, int64_t sinks, int64_t page_len,
                         int64_t cache_rows, int64_t num_q, int64_t num_kv, int64_t head_dim, int64_t block_len,
                         int64_t* info) {
-  return plan(static_cast<int32_t*>(image), image_bytes / 4, runs, num_runs, base_rows, num_rows, seq_len, window, sinks,
-              page_len, cache_rows, num_q, num_kv, head_dim, block_len, info);
+  try {
+    return plan(static_cast<int32_t*>(image), image_bytes / 4, runs, num_runs, base_rows, num_rows, seq_len, window, sinks,
+                page_len, cache_rows, num_q, num_kv, head_dim, block_len, info);
+  } catch (const std::bad_alloc&) {  // no exception passes a C entry
+    return fail(IFR_ENOMEM, "no host memory to plan %lld tokens in", (long long)seq_len);
+  }
 }
 
 int32_t ifr_window_attention_bf16(const void* image_dev, const int64_t* info, const void* q, const void* k_base,
