@@ -416,7 +416,9 @@ int32_t ifr_bq_block_quant(const void* src, void* x_i8, float* x_sa, int64_t col
  * be anything (-1, or pages that another run has taken over since).
  * block_len: 0 for a bf16 cache; else the rows of a scale block of an 8-bit
  * cache, a power of two in [16, page_len], every page starting at a block.
- * image: ifr_plan_window_bytes of host memory, of which info[4] bytes are used;
+ * image: ifr_plan_window_bytes of host memory (-1 for arguments that no plan
+ * takes: up to 2^24 tokens and runs, 2^29 - 1 rows), of which info[4] bytes are
+ * used;
  * info[IFR_WINDOW_INFO_LEN]: as for ifr_plan_attention, but info[2] =
  * IFR_PLAN_WINDOW, info[3] partial columns, info[14] prompt blocks, info[15]
  * write blocks, info[16] sinks, info[17..19] num_q, num_kv, head_dim, info[20]

@@ -102,6 +102,8 @@ constexpr int64_t kMaxRounds = 4;
 // Pieces at most that splits make: of row items all rounds, of prompt blocks two a CU more than there are.
 constexpr int64_t kSplitPieces = kMaxRounds * resident_groups(256) + 2 * kPromptGroups;
 
+constexpr int64_t kMostTokens = int64_t{1} << 24, kMostRows = INT32_MAX / 4;  // of a step, and of its run table
+
 struct Work {
   std::array<int32_t, kWorkWords> words;
   int64_t len() const { return words[kItHi] - words[kItLo]; }
@@ -260,9 +262,9 @@ int32_t plan(int32_t* img, int64_t img_words, const int32_t* runs, int64_t num_r
              int64_t num_q, int64_t num_kv, int64_t head_dim, int64_t block_len, int64_t* info) {
   using namespace ifr;
   if (!img || !info) return fail(IFR_EINVAL, "null image or info");
-  if (seq_len <= 0 || seq_len > (int64_t{1} << 24)) return fail(IFR_EINVAL, "seq_len must be in [1, 2^24]");
+  if (seq_len <= 0 || seq_len > kMostTokens) return fail(IFR_EINVAL, "seq_len must be in [1, 2^24]");
   if (num_runs <= 0 || num_runs > seq_len) return fail(IFR_EINVAL, "num_runs must be in [1, seq_len]");
-  if (num_rows < 0 || num_rows > INT32_MAX / 4) return fail(IFR_EINVAL, "num_rows out of range");
+  if (num_rows < 0 || num_rows > kMostRows) return fail(IFR_EINVAL, "num_rows out of range");
   if (!runs || !base_rows) return fail(IFR_EINVAL, "null run table");
   if (window < 0 || window > INT32_MAX / 4) return fail(IFR_EINVAL, "window must be in [0, 2^29)");
   if (sinks < 0 || sinks > INT32_MAX / 4) return fail(IFR_EINVAL, "sinks must be in [0, 2^29)");
@@ -533,6 +535,7 @@ extern "C" {
 
 int64_t ifr_plan_window_bytes(int64_t num_runs, int64_t num_rows, int64_t seq_len, int64_t block_len) {
   if (num_runs < 0 || num_rows < 0 || seq_len < 0 || block_len < 0) return -1;
+  if (num_runs > kMostTokens || num_rows > kMostRows || seq_len > kMostTokens) return -1;  // the plan refuses them
   return 4 * most_words(num_runs, num_rows, seq_len, block_len);
 }
 
