@@ -396,7 +396,10 @@ int32_t ifr_bq_block_quant(const void* src, void* x_i8, float* x_sa, int64_t col
 /* ---- attention with a window and sinks, and the 8-bit block-scaled cache -----
  * No counterpart in the reference.  These operators use the softmax as defined,
  * not the reference's biased exp, and their results do not depend on a worker
- * capacity.  With the queries' positions p:
+ * capacity.  They do depend, within what follows, on the step's other runs: how a
+ * run's work is cut, and so the order of its sums, and for runs of 33 to 128
+ * columns (tokens times q heads a kv head) whether they are taken as decode or as
+ * a prompt.  With the queries' positions p:
  *   visible(p) = { j <= p : window == 0, or j > p - window, or j < sinks }
  *   s_j = scale * q . k_j       o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)
  * over j in visible(p), m = max_j s_j; sums and products in f32, the weights of
@@ -462,8 +465,9 @@ int32_t ifr_window_attention_bf16(const void* image_dev, const int64_t* info, co
  *          product with the scale f32 holds (all but those above 240 under 2^120
  *          in e4m3, above 63 under 2^122 in int8); infinities become the largest
  *          of them, NaN stays NaN in e4m3 and becomes 0 in int8
- * Rows behind the step's tokens keep their bytes.  Refused where two of the
- * step's runs write to the same rows.  half and pair_stride: multiples of 8. */
+ * Rows behind the step's tokens keep their bytes.  Refused where two pages that
+ * the step writes to share rows (two runs on a page, or pages less than page_len
+ * rows apart).  half and pair_stride: multiples of 8. */
 int32_t ifr_kv8_cache_write(const void* image_dev, const int64_t* info, const void* q_src,
                             const void* k_src, const void* v_src, void* q_out, void* k_cache,
                             float* k_scale, void* v_cache, float* v_scale,

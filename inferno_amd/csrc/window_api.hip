@@ -83,7 +83,8 @@ static_assert(kInSharedWrites < IFR_WINDOW_INFO_LEN, "info holds every word");
 // gives it; prompt blocks take 8 to 32 times the columns and the cache through LDS.  A run
 // of few columns would leave most of a prompt block idle, and one of many would have row items
 // read the cache once for each 16 of them.  Runs of up to kRowItemCols columns are row items
-// always, runs of up to kRowItemMost if what all of those read stays below kRowItemBytes.
+// always, runs of up to kRowItemMost if what all of those read stays below kRowItemBytes: so a run
+// of 33 to 128 columns has weights of two bf16 parts or of one by what else is in the step.
 // Measured as row items and as prompt blocks, on 4,096 positions of an e4m3 cache (us):
 //   head_dim 256, 8 kv heads, 1 run:   32 columns 20 and 37, 64 columns 28 and 38, 128 columns 30 and 39
 //   the same, 16 runs:                 32 columns 111 and 162, 64 columns (1.1 GB) 195 and 165
@@ -351,6 +352,7 @@ int32_t plan(int32_t* img, int64_t img_words, const int32_t* runs, int64_t num_r
   //   33 (33 of 700 to 20,000, window 4,096, bf16, 512 dims, 2 heads)   149 and 155
   //   48 (48 of 4,096, int8, 512 dims, 2 heads)   94 and 82
   //   129 (64 of 4,096)                           188, 177 and 170
+  // Two heads from 40 on: at 32 they gain 2 us of 55, at 33 in 512 dims they lose 6 of 149.
   const int64_t groups = resident_groups(head_dim);
   const int64_t load = few_tiles * num_kv / groups;
   int64_t per_group = 1;

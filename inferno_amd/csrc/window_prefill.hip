@@ -2,9 +2,9 @@
 // and 8-bit caches.
 //
 // A block's eight waves share tiles of 32 positions of K and V in LDS.  A wave holds some tiles of
-// columns, (token, q head) pairs, with all head_dim dims of their sums, 128 accumulators a lane at
-// head_dim 128 and 256 and 128 at 512: S^T = K . Q^T and O^T += V^T . P^T in 32x32x16 MFMAs (at
-// head_dim 512, where 32 columns do not fit, 16x16x32).  The weights stay in the lanes that computed
+// columns, (token, q head) pairs, with all head_dim dims of their sums, 128 accumulators a lane at each
+// head_dim: S^T = K . Q^T and O^T += V^T . P^T in 32x32x16 MFMAs (at head_dim 512, where 32 columns
+// do not fit, 16x16x32).  The weights stay in the lanes that computed
 // them (the order of positions inside a product is free, and V^T is read in the order in which the
 // scores lie), K fragments are 16 bytes of an LDS row, V^T fragments two transposing LDS reads.
 //
@@ -20,16 +20,16 @@
 // other end a weight below 2^-110 of the largest counts as 0, and a result below 2^-110 loses bits.
 //
 // Measured: 4 prompts of 2,048 new tokens, 16 q and 8 kv heads of 256, on up to 7,693 positions of
-// an int8 cache: 700 us, 970 TFLOP/s of what the mask leaves; with a window of 1,024 on a bf16 cache
-// 178 us.  With all waves at the same thing at the same time the first takes 769 to 785 us, the sum
+// an int8 cache: 704 us, 966 TFLOP/s of what the mask leaves; with a window of 1,024 on a bf16 cache
+// 183 us.  With all waves at the same thing at the same time the first took 769 to 785 us, the sum
 // of its parts, each at the rate of the pipe that does it (repeated calls, 735 us: without the products
 // 430, without the softmax 690, without loading and converting 560); two waves a SIMD is what 256
 // registers each leave.  The halves of the waves apart (see the walk) cost a longer start, 3 % of a
 // piece of 29 tiles; at head_dim 128 they are not, as the registers that it takes there cost 2 to 5 %.
-// Tried and slower: a second barrier in each step between the halves' parts (790 us against 735);
-// scores of the next tile between the weights of this one (810); 16x16x32 products with two or three
-// column tiles a wave (815).  A group of two tiles a barrier made no difference, nor did fewer
-// instructions for addresses.  Stores of whole cache lines over LDS save 15 us of the second's 206.
+// Tried and slower, in that form: a second barrier in each step between the halves' parts (790 us
+// against 735); scores of the next tile between the weights of this one (810); 16x16x32 products with
+// two or three column tiles a wave (815).  A group of two tiles a barrier made no difference, nor did
+// fewer instructions for addresses.  Stores of whole cache lines over LDS saved 15 us of the second's 206.
 #include <float.h>
 
 #include <type_traits>
@@ -155,12 +155,14 @@ __device__ __forceinline__ void score_mfma(f32x16_t& s, bf16x8_t x, bf16x8_t y) 
 }
 
 // How far m is put above the score that moves it, in powers of two.  4 prompts of 2,048 tokens with a
-// window of 1,024 take 213 us at 10, 205 at 12, 193 at 14 and 189 at 16, as with 24.
+// window of 1,024 take 213 us at 10, 205 at 12, 193 at 14 and 189 at 16, where
+// the moves no longer show.
 constexpr float kSlack = 16.0f;
 
 // One block.  False if a sum came out that is not finite: the block is then done again with
-// kCareful, which stores over it (two functions, so that the registers of one do not weigh
-// on the other).
+// kCareful, which stores over it.  Both are parts of one kernel, and what the second keeps in scratch
+// memory counts for the kernel's; of the first walks' tiles only those at head_dim 128 over int8 read
+// a value back from there.
 template <int kD, int kFormat>
 struct Prompt {
   static constexpr int kM = prompt_tile_cols(kD), kNc = prompt_col_tiles(kD);  // columns of a tile, tiles of a wave
