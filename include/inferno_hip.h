@@ -484,6 +484,82 @@ int32_t ifr_kv8_attention(const void* image_dev, const int64_t* info, const void
                           int64_t head_dim, int64_t kv_stride, float scale,
                           int64_t kv_format, uint64_t stream);
 
+/* ---- behind the attention: 4-bit projections, norms, the next token ---------------
+ * No counterparts in the reference.
+ *
+ * Products with 4-bit weights and group scales, the form of ifr_dispatch_gemm_cols for
+ * weights of 4-bit codes:
+ *   output[m][n] = bf16(sum_g scales[n][g] * sum_{k in group g} x[m][k] * v(codes[n][k]))
+ * x [seq_len][cols] and output [seq_len][rows] bf16; codes [rows][cols / 2], column k in
+ * the lower four bits of byte k / 2 where k is even, in the upper ones where it is odd;
+ * scales [rows][cols / group] bf16, any numbers.  v: IFR_W4_INT4 -8 to 7 in two's
+ * complement; IFR_W4_E2M1 0, 0.5, 1, 1.5, 2, 3, 4, 6 and, from code 8, their negatives.
+ * Sums are f32, and nothing is rounded before the output; their order depends on
+ * seq_len, and where a workspace is used, on its size.  A token's results depend on
+ * its own x alone, so infinities and NaN stay in their token.
+ * group 32, 64 or 128; cols a multiple of 128; any rows.  All pointers 16-byte aligned.
+ * workspace: device memory of ifr_w4_gemm_workspace_bytes (0: null will do), written
+ * before it is read in every call; calls that may overlap each need their own. */
+#define IFR_W4_INT4 1
+#define IFR_W4_E2M1 2
+int64_t ifr_w4_gemm_workspace_bytes(int64_t rows, int64_t cols, int64_t seq_len);
+int32_t ifr_dispatch_w4_gemm_cols(const void* x, const void* codes, const void* scales,
+                                  void* output, int64_t rows, int64_t cols,
+                                  int64_t seq_len, int64_t group, int64_t w_format,
+                                  void* workspace, int64_t workspace_bytes,
+                                  uint64_t stream);
+
+/* The norm behind a block, its gate and residual scale, and the norm ahead of the next
+ * block:
+ *   t  = y / sqrt(mean(y^2) + eps) * post_weight       (post_norm 0: t = y)
+ *   r' = residual_scale * residual + block_scale * gate * t
+ *   x  = r' / sqrt(mean(r'^2) + eps) * pre_weight      (x_out null: left out)
+ * for each of seq_len rows of `hidden` elements, in f32; r' and x are rounded once each, x
+ * from the unrounded r'.  y, x_out and the weights bf16; residual and residual_out of
+ * residual_type.  A null weight is one of ones; a null gate is left out; gate
+ * [gate rows][hidden] bf16 with gate_stride 0 for one row for all tokens, else the
+ * elements between two tokens' rows (a multiple of 8, hidden or more).  residual_out may
+ * be residual, and x_out may be y; otherwise outputs overlap nothing.  hidden: a multiple
+ * of 8, up to 65,536; eps > 0.  The sum of a row's squares has to stay in f32's range.
+ * All pointers 16-byte aligned. */
+#define IFR_RESIDUAL_BF16 0
+#define IFR_RESIDUAL_F32 1
+int32_t ifr_norm_residual(const void* y, const void* residual, void* residual_out,
+                          void* x_out, const void* post_weight, const void* gate,
+                          const void* pre_weight, int64_t hidden, int64_t seq_len,
+                          int64_t residual_type, int64_t post_norm, int64_t gate_stride,
+                          float residual_scale, float block_scale, float eps,
+                          uint64_t stream);
+
+/* A token for each of num_rows rows of logits z, from a given number u in [0, 1):
+ *   w_i = exp((z_i - max z) / temperature)
+ *   K   = the first top_k tokens by (z descending, index ascending)
+ *   P   = the shortest prefix of K with sum w >= top_p * (sum over K of w), one token
+ *         at least
+ *   M   = { i in P : w_i >= min_p }
+ *   token = the first i of M, by index, with
+ *           (sum over j <= i in M of w_j) > u * (sum over M of w)
+ * Sums have 64 bits, and the draw does not depend on how the work is cut.  temperature,
+ * top_k, top_p, min_p and uniform hold a number for each row, in device memory; each of the
+ * first four may be null.  A temperature of 0, below it or NaN takes the first of the
+ * largest logits; top_k <= 0, top_p >= 1 or NaN and min_p <= 0 or NaN are off; top_p <= 0
+ * keeps one token, min_p >= 1 the largest logits.  u outside [0, 1) counts as the nearest
+ * inside, NaN as 0.  Logits of -inf and NaN are never drawn; a row of nothing else gives -1.
+ * Logits of +inf share the draw.
+ * logits [num_rows][row_stride] of logits_type, of which vocab (1 to 2^20) are read;
+ * num_rows up to 2^20.  workspace: device memory of ifr_sample_workspace_bytes, 16-byte
+ * aligned (0: null will do), written before it is read in every call; calls that may
+ * overlap each need their own. */
+#define IFR_LOGITS_BF16 0
+#define IFR_LOGITS_F32 1
+int64_t ifr_sample_workspace_bytes(int64_t num_rows, int64_t vocab);
+int32_t ifr_dispatch_sample_tokens(const void* logits, const float* uniform, int32_t* tokens,
+                                   const float* temperature, const int32_t* top_k,
+                                   const float* top_p, const float* min_p, int64_t num_rows,
+                                   int64_t vocab, int64_t row_stride, int64_t logits_type,
+                                   void* workspace, int64_t workspace_bytes,
+                                   uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,7 @@ WINDOW_INFO_LEN = 32
 PLAN_SPLIT_MERGE, PLAN_TOKEN_DIRECT, PLAN_TOKEN_MERGE = 0, 1, 2
 PLAN_WINDOW = 3
 KV8_FORMATS = {"e4m3": 1, "int8": 2}
+W4_FORMATS = {"int4": 1, "e2m1": 2}
 
 # name -> (restype, argtypes)
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -94,6 +95,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                   I64, I64, I64, I64, I64, I64, U64]),
     "ifr_kv8_attention": (I32, [VP, P_I64, VP, VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, I64,
                                 F32, I64, U64]),
+    "ifr_w4_gemm_workspace_bytes": (I64, [I64, I64, I64]),
+    "ifr_dispatch_w4_gemm_cols": (I32, [VP, VP, VP, VP, I64, I64, I64, I64, I64, VP, I64, U64]),
+    "ifr_norm_residual": (I32, [VP, VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, I64, F32, F32,
+                                F32, U64]),
+    "ifr_sample_workspace_bytes": (I64, [I64, I64]),
+    "ifr_dispatch_sample_tokens": (I32, [VP, VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, VP, I64,
+                                         U64]),
     # ---- host-side page state (include/inferno_host.h) ----
     "ifr_splitmix64": (U64, [U64]),
     "ifr_hash_token_block": (U64, [VP, I64, I64]),

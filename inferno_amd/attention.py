@@ -11,7 +11,7 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import KV8_FORMATS, P_I64, check, lib
+from ._lib import KV8_FORMATS, P_I64, W4_FORMATS, check, lib
 from .kv import (FULL, SLIDING, AttentionPlan, KVRunTable, WindowPlan,
                  flash_partial_stride)
 
@@ -427,6 +427,151 @@ def kv8_attention(plan: WindowPlan, q, k_base, k_scale, v_base, v_scale, output,
         scale, _kv8_format(kv_format), _window_stream(plan)))
 
 
+def _current_device(t):
+    """The device of t, which has to be the current one."""
+    import torch
+
+    if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"a tensor is on {t.device}, the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+    return t.device
+
+
+def _tensor(device, name: str, t, numel: int, itemsize: int) -> int:
+    """The address of a contiguous tensor of at least numel elements on the device."""
+    import torch
+
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.element_size() != itemsize or t.dtype == torch.float16 or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous, of {itemsize}-byte elements (has "
+                         f"{t.dtype}, strides {tuple(t.stride())})")
+    if t.numel() < numel:
+        raise ValueError(f"{name} has {t.numel()} elements, {numel} are needed")
+    return t.data_ptr()
+
+
+def w4_gemm_workspace(rows: int, cols: int, seq_len: int, device="cuda"):
+    """f32 workspace for dispatch_w4_gemm_cols at this shape (None if unneeded)."""
+    import torch
+
+    n = lib().ifr_w4_gemm_workspace_bytes(rows, cols, seq_len)
+    if n < 0:
+        raise ValueError("bad w4_gemm_cols shape")
+    return torch.empty(n // 4, dtype=torch.float32, device=device) if n else None
+
+
+def dispatch_w4_gemm_cols(x, codes, scales, output, *, rows: int, cols: int, seq_len: int,
+                          group: int, w_format: str, workspace=None) -> None:
+    """dispatch_gemm_cols for a weight of 4-bit codes with a scale for each `group` columns
+    of a row: output[m][n] = bf16(sum_k x[m][k] * scales[n][k // group] * codes[n][k]).
+    codes [rows][cols / 2] of one byte, even columns in the lower four bits; w_format "int4"
+    (two's complement) or "e2m1"; scales [rows][cols / group] bf16.  No counterpart in the
+    reference."""
+    if w_format not in W4_FORMATS:
+        raise ValueError(f"w_format must be one of {sorted(W4_FORMATS)}, not {w_format!r}")
+    if group not in (32, 64, 128):
+        raise ValueError("group must be 32, 64 or 128")
+    dev = _current_device(x)
+    ws, ws_bytes = None, 0
+    if workspace is not None:
+        ws, ws_bytes = _tensor(dev, "workspace", workspace, 0, 4), workspace.numel() * 4
+    check(lib().ifr_dispatch_w4_gemm_cols(
+        _tensor(dev, "x", x, seq_len * cols, 2),
+        _tensor(dev, "codes", codes, rows * (cols // 2), 1),
+        _tensor(dev, "scales", scales, rows * (cols // group), 2),
+        _tensor(dev, "output", output, seq_len * rows, 2), rows, cols, seq_len, group,
+        W4_FORMATS[w_format], ws, ws_bytes, _stream()))
+
+
+def dispatch_norm_residual(y, residual, residual_out, x_out=None, *, hidden: int, seq_len: int,
+                           eps: float, post_norm: bool = True, post_weight=None, gate=None,
+                           residual_scale: float = 1.0, block_scale: float = 1.0,
+                           pre_weight=None) -> None:
+    """The norm behind a block, its gate and residual scale, and the norm ahead of the next
+    block (ifr_norm_residual in include/inferno_hip.h):
+    residual_out = residual_scale * residual + block_scale * gate * norm(y) * post_weight and
+    x_out = norm(residual_out) * pre_weight.  residual is bf16 or f32, and residual_out of the
+    same type; gate has hidden elements or seq_len * hidden.  residual_out may be residual,
+    x_out may be y.  No counterpart in the reference."""
+    import torch
+
+    dev = _current_device(y)
+    n = seq_len * hidden
+    f32 = residual.dtype == torch.float32
+    if residual_out.dtype != residual.dtype:
+        raise ValueError(f"residual is {residual.dtype}, residual_out {residual_out.dtype}")
+    if post_weight is not None and not post_norm:
+        raise ValueError("post_weight without post_norm")
+    if pre_weight is not None and x_out is None:
+        raise ValueError("pre_weight without x_out")
+
+    def ptr(name, t, numel):
+        return None if t is None else _tensor(dev, name, t, numel, 2)
+
+    gate_stride = 0
+    if gate is not None and gate.numel() != hidden:
+        gate_stride = hidden
+    check(lib().ifr_norm_residual(
+        ptr("y", y, n), _tensor(dev, "residual", residual, n, 4 if f32 else 2),
+        _tensor(dev, "residual_out", residual_out, n, 4 if f32 else 2), ptr("x_out", x_out, n),
+        ptr("post_weight", post_weight, hidden),
+        ptr("gate", gate, n if gate_stride else hidden), ptr("pre_weight", pre_weight, hidden),
+        hidden, seq_len, int(f32), int(post_norm), gate_stride, residual_scale, block_scale, eps,
+        _stream()))
+
+
+def sample_workspace(num_rows: int, vocab: int, device="cuda"):
+    """Workspace for dispatch_sample_tokens at this shape (None if unneeded)."""
+    import torch
+
+    n = lib().ifr_sample_workspace_bytes(num_rows, vocab)
+    if n < 0:
+        raise ValueError("bad sample_tokens shape")
+    return torch.empty(n // 4, dtype=torch.float32, device=device) if n else None
+
+
+def dispatch_sample_tokens(logits, uniform, tokens, workspace=None, *, num_rows: int, vocab: int,
+                           row_stride: int | None = None, temperature=None, top_k=None,
+                           top_p=None, min_p=None) -> None:
+    """A token for each row of logits from a given random number of [0, 1), with
+    temperature, top-k, top-p and min-p (ifr_dispatch_sample_tokens in
+    include/inferno_hip.h has the rules).  logits: bf16 or f32, either a matrix whose rows
+    may be apart, or with row_stride a flat buffer; uniform, temperature, top_p, min_p:
+    f32, top_k and tokens int32, a number for each row.  No counterpart in the reference."""
+    import torch
+
+    dev = _current_device(logits)
+    f32 = logits.dtype == torch.float32
+    if row_stride is not None:
+        ptr = _tensor(dev, "logits", logits, (num_rows - 1) * row_stride + vocab,
+                      4 if f32 else 2)
+    else:
+        if (logits.dim() != 2 or logits.shape[0] < num_rows or logits.shape[1] < vocab
+                or (vocab > 1 and logits.stride(1) != 1)
+                or (num_rows > 1 and logits.stride(0) < vocab)):
+            raise ValueError(f"logits of shape {tuple(logits.shape)} and strides "
+                             f"{tuple(logits.stride())} have no {num_rows} rows of {vocab}")
+        row_stride = max(logits.stride(0), vocab)
+        ptr = _tensor(dev, "logits", logits[:1, :vocab], 0, 4 if f32 else 2)
+    ws, ws_bytes = None, 0
+    if workspace is not None:
+        ws, ws_bytes = _tensor(dev, "workspace", workspace, 0, 4), workspace.numel() * 4
+
+    def of_rows(name, t, dtype):
+        if t is None:
+            return None
+        if t.dtype != dtype:
+            raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+        return _tensor(dev, name, t, num_rows, 4)
+
+    check(lib().ifr_dispatch_sample_tokens(
+        ptr, of_rows("uniform", uniform, torch.float32), of_rows("tokens", tokens, torch.int32),
+        of_rows("temperature", temperature, torch.float32), of_rows("top_k", top_k, torch.int32),
+        of_rows("top_p", top_p, torch.float32), of_rows("min_p", min_p, torch.float32), num_rows,
+        vocab, row_stride, int(f32), ws, ws_bytes, _stream()))
+
+
 __all__ = [
     "SLIDING", "FULL", "KVRunTable", "AttentionPlan", "WindowPlan", "window_workspace",
     "window_attention_bf16", "dispatch_kv8_cache_write", "kv8_attention", "partials_buffer",
@@ -436,5 +581,6 @@ __all__ = [
     "dispatch_bq_attn_prep", "bq_attention", "dispatch_bq_block_quant",
     "gemm_cols_workspace", "dispatch_gemm_cols", "index_scores_buffer",
     "dispatch_lightning_indexer", "dispatch_block_sparse_attention",
-    "dispatch_bq_block_sparse_attention",
+    "dispatch_bq_block_sparse_attention", "w4_gemm_workspace", "dispatch_w4_gemm_cols",
+    "dispatch_norm_residual", "sample_workspace", "dispatch_sample_tokens",
 ]

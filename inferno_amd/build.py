@@ -33,7 +33,7 @@ SOURCES = ["api.hip", "attention.hip", "attention_wide.hip", "append.hip", "copy
            "prefill.hip", "prefill_narrow.hip", "prefill_pair.hip", "prefill_sliding.hip",
            "prefill_wide.hip",
            "gemm.hip", "sparse.hip", "window_api.hip", "window_rows.hip", "window_prefill.hip",
-           "kv8_write.hip"]
+           "kv8_write.hip", "step_api.hip", "w4_gemm.hip", "norm_residual.hip", "sample.hip"]
 # Host-only C++ (page state, scheduler): built with the host compiler.
 HOST_SOURCES = ["host_state.cpp", "host_api.cpp"]
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wextra", f"-I{INCLUDE}"]

@@ -1,0 +1,168 @@
+// The norm behind a block, its gate and residual scale, and the norm ahead of the next
+// block, in one pass over a token's row:
+//   t  = y / sqrt(mean(y^2) + eps) * post_weight          (or y)
+//   r' = residual_scale * residual + block_scale * (gate * t)
+//   x  = r' / sqrt(mean(r'^2) + eps) * pre_weight
+// in f32; r' and x are each rounded once, x from the unrounded r'.
+#include "common.hpp"
+#include "step.hpp"
+
+namespace ifr {
+namespace {
+
+__device__ __forceinline__ float wave_sum(float v) { return pair_sum32(pair_sum16(tree16_sum(v))); }
+
+__device__ __forceinline__ void unpack8(uint4 p, float* v) {
+  v[0] = bf16_lo(p.x), v[1] = bf16_hi(p.x), v[2] = bf16_lo(p.y), v[3] = bf16_hi(p.y);
+  v[4] = bf16_lo(p.z), v[5] = bf16_hi(p.z), v[6] = bf16_lo(p.w), v[7] = bf16_hi(p.w);
+}
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  bf16x2_t p;
+  p[0] = static_cast<__bf16>(lo);
+  p[1] = static_cast<__bf16>(hi);
+  return __builtin_bit_cast(uint32_t, p);
+}
+__device__ __forceinline__ uint4 pack8(const float* v) {
+  return make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+}
+
+// W waves a row, C chunks of 8 elements a lane: the row stays in registers between
+// its reads and its writes, and each of the two sums is one reduction.
+template <int W, int C, bool kF32>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_residual_kernel(NormResidualArgs a) {
+  constexpr int kRowThreads = 64 * W;
+  __shared__ float part[2][W];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t row = W == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + wave : blockIdx.x;
+  if (row >= a.rows) return;  // W > 1: block-uniform
+  const int t = W == 1 ? lane : threadIdx.x;
+  const int hidden = static_cast<int>(a.hidden), chunks = hidden / 8;
+  const float n = static_cast<float>(hidden);
+
+  auto row_sum = [&](float v, int which) {
+    v = wave_sum(v);
+    if constexpr (W > 1) {
+      if (lane == 0) part[which][wave] = v;
+      __syncthreads();
+      v = part[which][0];
+#pragma unroll
+      for (int w = 1; w < W; ++w) v = v + part[which][w];
+    }
+    return v;
+  };
+
+  uint4 y[C], g[C], pw[C], qw[C];
+  float r[C][8];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int at = c * kRowThreads + t;
+    if (at < chunks) {
+      y[c] = reinterpret_cast<const uint4*>(a.y + row * hidden)[at];
+      if constexpr (kF32) {
+        const float4* p = reinterpret_cast<const float4*>(
+                              static_cast<const float*>(a.residual) + row * hidden) + 2 * at;
+        const float4 lo = p[0], hi = p[1];
+        r[c][0] = lo.x, r[c][1] = lo.y, r[c][2] = lo.z, r[c][3] = lo.w;
+        r[c][4] = hi.x, r[c][5] = hi.y, r[c][6] = hi.z, r[c][7] = hi.w;
+      } else {
+        unpack8(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.residual) +
+                                               row * hidden)[at], r[c]);
+      }
+      if (a.gate) g[c] = reinterpret_cast<const uint4*>(a.gate + row * a.gate_stride)[at];
+      if (a.post_weight) pw[c] = reinterpret_cast<const uint4*>(a.post_weight)[at];
+      if (a.pre_weight) qw[c] = reinterpret_cast<const uint4*>(a.pre_weight)[at];
+    }
+  }
+  float inv = 1.0f;
+  if (a.post_norm) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (c * kRowThreads + t >= chunks) continue;
+      float v[8];
+      unpack8(y[c], v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(v[i], v[i], ss);
+    }
+    inv = 1.0f / sqrtf(row_sum(ss, 0) / n + a.eps);
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int at = c * kRowThreads + t;
+    if (at >= chunks) continue;
+    float v[8], w[8];
+    unpack8(y[c], v);
+    if (a.post_weight) {
+      unpack8(pw[c], w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = v[i] * inv;
+    }
+    if (a.gate) {
+      unpack8(g[c], w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = v[i] * w[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      r[c][i] = __builtin_fmaf(a.block_scale, v[i], a.residual_scale * r[c][i]);
+      ss = __builtin_fmaf(r[c][i], r[c][i], ss);
+    }
+    if constexpr (kF32) {
+      float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.residual_out) + row * hidden) +
+                  2 * at;
+      p[0] = make_float4(r[c][0], r[c][1], r[c][2], r[c][3]);
+      p[1] = make_float4(r[c][4], r[c][5], r[c][6], r[c][7]);
+    } else {
+      reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.residual_out) + row * hidden)[at] =
+          pack8(r[c]);
+    }
+  }
+  if (!a.x_out) return;
+  inv = 1.0f / sqrtf(row_sum(ss, 1) / n + a.eps);
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int at = c * kRowThreads + t;
+    if (at >= chunks) continue;
+    float v[8], w[8];
+    if (a.pre_weight) unpack8(qw[c], w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = a.pre_weight ? r[c][i] * inv * w[i] : r[c][i] * inv;
+    reinterpret_cast<uint4*>(a.x_out + row * hidden)[at] = pack8(v);
+  }
+}
+
+template <int W, int C>
+hipError_t launch_wc(const NormResidualArgs& a, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(W == 1 ? (a.rows + 3) / 4 : a.rows));
+  const dim3 block(W == 1 ? 256 : 64 * W);
+  if (a.f32)
+    hipLaunchKernelGGL((norm_residual_kernel<W, C, true>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((norm_residual_kernel<W, C, false>), grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+
+template <int W>
+hipError_t launch_w(const NormResidualArgs& a, hipStream_t stream) {
+  const int64_t c = (a.hidden / 8 + 64 * W - 1) / (64 * W);
+  if (c <= 1) return launch_wc<W, 1>(a, stream);
+  if (c <= 2) return launch_wc<W, 2>(a, stream);
+  if (c <= 4) return launch_wc<W, 4>(a, stream);
+  return launch_wc<W, 8>(a, stream);
+}
+
+}  // namespace
+
+hipError_t launch_norm_residual(const NormResidualArgs& a, hipStream_t stream) {
+  const int64_t chunks = a.hidden / 8;
+  if (chunks <= 64 * 4) return launch_w<1>(a, stream);
+  if (chunks <= 256 * 4) return launch_w<4>(a, stream);
+  return launch_w<16>(a, stream);
+}
+
+}  // namespace ifr
