@@ -4,6 +4,8 @@
 // [N][K / group].  Codes become bf16 numbers without rounding (int4: -8..7, e2m1:
 // two significant bits), the matrix products sum a group in f32, and the group's scale
 // multiplies that sum in f32: nothing is rounded before the result.
+#include <algorithm>
+
 #include "common.hpp"
 #include "step.hpp"
 
@@ -48,59 +50,428 @@ __device__ __forceinline__ bf16x8_t w4_values(uint32_t w) {
   return __builtin_bit_cast(bf16x8_t, r);
 }
 
+// A step is 128 columns of 16 weight rows: lane l holds 16 bytes, columns 32 q .. + 31 of row
+// r, for r = l % 16 and q = l / 16, and v_mfma_f32_16x16x32_bf16 takes the weight as its B
+// operand (column r of the output, eight k of quarter q), so that a lane holds codes of one
+// row and one scale multiplies its sums.  A matrix product adds over the quarters, so groups
+// of less than 128 have to be moved to one register first: swaps between the quarters
+// (transposing words, four of a lane, with quarters) leave word j of all lanes in group
+// 32 j / kGroup.  x has to come in the same order: x_offset is the k, within the step, of the
+// eight values that lane quarter q multiplies with word j.
+template <int kGroup>
+__device__ __forceinline__ int x_offset(int j, int q) {
+  if constexpr (kGroup == 128) return 32 * q + 8 * j;
+  if constexpr (kGroup == 64) return 64 * (j >> 1) + 8 * (j & 1) + 32 * (q & 1) + 16 * (q >> 1);
+  return 32 * j + 8 * q;
+}
+__device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0], b = r[1];
+}
+__device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0], b = r[1];
+}
+template <int kGroup>
+__device__ __forceinline__ void order_words(uint4& w) {
+  if constexpr (kGroup < 128) {
+    swap32(w.x, w.z);
+    swap32(w.y, w.w);
+  }
+  if constexpr (kGroup < 64) {
+    swap16(w.x, w.y);
+    swap16(w.z, w.w);
+  }
+}
+
+// The scales of a step of one row: 128 / kGroup bf16 numbers.
+template <int kGroup>
+struct StepScales {
+  uint32_t v[kGroup == 32 ? 2 : 1];
+  __device__ __forceinline__ void load(const uint16_t* p) {
+    if constexpr (kGroup == 128) v[0] = *p;
+    if constexpr (kGroup == 64) v[0] = *reinterpret_cast<const uint32_t*>(p);
+    if constexpr (kGroup == 32) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      v[0] = u.x, v[1] = u.y;
+    }
+  }
+  __device__ __forceinline__ float get(int g) const {
+    return g & 1 ? bf16_hi(v[g >> 1]) : bf16_lo(v[g >> 1]);
+  }
+};
+
+// sum += the step's products, TM tiles of 16 tokens.  R: the values of a lane that stand for
+// tokens (token t is row 4 (t / R) + t % R of its tile: with at most four tokens one value a
+// lane has to be scaled, not four).
+template <int kFmt, int kGroup, int TM, int R>
+__device__ __forceinline__ void multiply_step(const bf16x8_t (&xf)[TM][4], uint4 w,
+                                              const StepScales<kGroup>& s, f32x4_t (&sum)[TM]) {
+  order_words<kGroup>(w);
+  const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+  constexpr int kPer = kGroup / 32;  // words of a group
+#pragma unroll
+  for (int g = 0; g < 4 / kPer; ++g) {
+    f32x4_t acc[TM];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const bf16x8_t b = w4_values<kFmt>(word[g * kPer + j]);
+#pragma unroll
+      for (int t = 0; t < TM; ++t)
+        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[t][g * kPer + j], b, acc[t], 0, 0, 0);
+    }
+    const float sc = s.get(g);
+#pragma unroll
+    for (int t = 0; t < TM; ++t)
+#pragma unroll
+      for (int i = 0; i < R; ++i) sum[t][i] = __builtin_fmaf(sc, acc[t][i], sum[t][i]);
+  }
+}
+
+template <int R>
+__device__ __forceinline__ int token_of_row(int row) {
+  return (row >> 2) * R + min(row & 3, R - 1);
+}
+
+// Up to 16 tokens and few columns: a workgroup takes `cols` columns (NT tiles of 16), its waves
+// take ST steps of k in turn, and their sums meet in LDS, added in wave order.  Every load of
+// ST steps is under way before the first product; x comes from L2.
+template <int kFmt, int kGroup, int NT, int ST, int R>
+__global__ __launch_bounds__(1024) void w4_few_kernel(W4Args a, int cols) {
+  __shared__ float part[16][NT * R][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int waves = blockDim.x >> 6;
+  const int r = lane & 15, q = lane >> 4;
+  const int M = static_cast<int>(a.M), N = static_cast<int>(a.N), K = static_cast<int>(a.K);
+  const int n0 = blockIdx.x * cols, steps = K / 128;
+  const uint16_t* xp = a.x + static_cast<int64_t>(min(token_of_row<R>(r), M - 1)) * K;
+  const uint8_t* wp[NT];
+  const uint16_t* sp[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t n = min(n0 + min(16 * t + r, cols - 1), N - 1);
+    wp[t] = a.codes + n * (K / 2) + 16 * q;
+    sp[t] = a.scales + n * (K / kGroup);
+  }
+  f32x4_t sum[NT][1];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) sum[t][0] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = wave * ST; s0 < steps; s0 += waves * ST) {
+    uint4 w[ST][NT];
+    StepScales<kGroup> sc[ST][NT];
+    bf16x8_t xf[ST][1][4];
+#pragma unroll
+    for (int i = 0; i < ST; ++i) {
+      const int s = min(s0 + i, steps - 1);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        w[i][t] = *reinterpret_cast<const uint4*>(wp[t] + 64 * s);
+        sc[i][t].load(sp[t] + s * (128 / kGroup));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < ST; ++i) {
+      const int s = min(s0 + i, steps - 1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        xf[i][0][j] = *reinterpret_cast<const bf16x8_t*>(xp + 128 * s + x_offset<kGroup>(j, q));
+    }
+    __builtin_amdgcn_sched_barrier(0);  // every load ahead of the first product
+#pragma unroll
+    for (int i = 0; i < ST; ++i)
+      if (s0 + i < steps)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          multiply_step<kFmt, kGroup, 1, R>(xf[i], w[i][t], sc[i][t], sum[t]);
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < R; ++i) part[wave][t * R + i][lane] = sum[t][0][i];
+  __syncthreads();
+  for (int e = threadIdx.x; e < NT * R * 64; e += blockDim.x) {
+    const int v = e >> 6, l = e & 63;
+    const int m = (l >> 4) * R + v % R, c = 16 * (v / R) + (l & 15);
+    if (m >= M || c >= cols || n0 + c >= N) continue;
+    float total = part[0][v][l];
+    for (int z = 1; z < waves; ++z) total = total + part[z][v][l];
+    a.out[static_cast<int64_t>(m) * N + n0 + c] =
+        static_cast<uint16_t>(pack_bf16(kUnit<kFmt> * total, 0.0f));
+  }
+}
+
+// Up to 16 TM tokens: a wave takes NT tiles of 16 columns over the workgroup's span of k, with x
+// in LDS, a chunk of k at a time, and the codes straight from memory into registers, two
+// steps ahead.  With several spans the sums go to part [span][M][N].
+constexpr int kStreamWaves = 8;
+constexpr int kStreamLds = 72 * 1024;  // two workgroups a CU
+template <int kFmt, int kGroup, int TM, int NT, int R, bool kSplit>
+__global__ __launch_bounds__(64 * kStreamWaves, TM <= 2 ? 2 : 1) void w4_stream_kernel(
+    W4Args a, int span_steps, int chunk_steps, int64_t part_stride) {
+  extern __shared__ __align__(16) uint8_t xs[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int r = lane & 15, q = lane >> 4;
+  const int M = static_cast<int>(a.M), N = static_cast<int>(a.N), K = static_cast<int>(a.K);
+  const int n0 = (blockIdx.x * kStreamWaves + wave) * 16 * NT;
+  const int first = blockIdx.y * span_steps;
+  const int steps = min(span_steps, K / 128 - first);
+  const int pitch = 256 * chunk_steps + 16;  // rows four banks apart
+
+  const uint8_t* wp[NT];
+  const uint16_t* sp[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t n = min(n0 + 16 * t + r, N - 1);
+    wp[t] = a.codes + n * (K / 2) + 64 * first + 16 * q;
+    sp[t] = a.scales + n * (K / kGroup) + first * (128 / kGroup);
+  }
+  uint4 w[2][NT];
+  StepScales<kGroup> sc[2][NT];
+  auto load = [&](int set, int s) {
+    s = min(s, steps - 1);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      w[set][t] = *reinterpret_cast<const uint4*>(wp[t] + 64 * s);
+      sc[set][t].load(sp[t] + s * (128 / kGroup));
+    }
+  };
+  load(0, 0);
+  load(1, 1);
+
+  f32x4_t sum[NT][TM];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int m = 0; m < TM; ++m) sum[t][m] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const uint8_t* xrow[TM];
+#pragma unroll
+  for (int m = 0; m < TM; ++m)
+    xrow[m] = xs + min(16 * m + token_of_row<R>(r), M - 1) * pitch;
+
+  auto multiply = [&](int set, int s, int in_chunk) {
+    bf16x8_t xf[TM][4];
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        xf[m][j] = *reinterpret_cast<const bf16x8_t*>(xrow[m] + 256 * in_chunk +
+                                                      2 * x_offset<kGroup>(j, q));
+    uint4 now[NT];
+    StepScales<kGroup> now_sc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) now[t] = w[set][t], now_sc[t] = sc[set][t];
+    load(set, s + 2);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      multiply_step<kFmt, kGroup, TM, R>(xf, now[t], now_sc[t], sum[t]);
+  };
+  for (int c0 = 0; c0 < steps; c0 += chunk_steps) {
+    const int here = min(chunk_steps, steps - c0);
+    if (c0) __syncthreads();
+    // Rows of `here` steps of 256 bytes, 16 bytes a thread.
+    const int per = 16 * here;
+    for (int i = threadIdx.x; i < M * per; i += 64 * kStreamWaves) {
+      const int m = i / per, at = i - m * per;
+      *reinterpret_cast<uint4*>(xs + m * pitch + 16 * at) = *reinterpret_cast<const uint4*>(
+          a.x + static_cast<int64_t>(m) * K + 128 * (first + c0) + 8 * at);
+    }
+    __syncthreads();
+    for (int s = 0; s < here; s += 2) {
+      multiply(0, c0 + s, s);
+      if (s + 1 < here) multiply(1, c0 + s + 1, s + 1);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int n = n0 + 16 * t + r;
+    if (n >= N) continue;
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const int token = 16 * m + q * R + i;
+        if (token >= M) continue;
+        const int64_t o = static_cast<int64_t>(token) * N + n;
+        if constexpr (kSplit)
+          a.workspace[blockIdx.y * part_stride + o] = sum[t][m][i];
+        else
+          a.out[o] = static_cast<uint16_t>(pack_bf16(kUnit<kFmt> * sum[t][m][i], 0.0f));
+      }
+  }
+}
+
+// out = bf16(unit * (part[0] + part[1] + ...)), four outputs a thread, added in order.
+__global__ __launch_bounds__(256) void w4_reduce_kernel(const float* __restrict__ part,
+                                                        uint16_t* __restrict__ out, int64_t count,
+                                                        int64_t part_stride, int splits,
+                                                        float unit) {
+  const int64_t i = 4 * (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x);
+  if (i >= count) return;
+  float4 s = *reinterpret_cast<const float4*>(part + i);
+#pragma unroll 4
+  for (int z = 1; z < splits; ++z) {
+    const float4 v = *reinterpret_cast<const float4*>(part + z * part_stride + i);
+    s.x = s.x + v.x, s.y = s.y + v.y, s.z = s.z + v.z, s.w = s.w + v.w;
+  }
+  const uint2 p = make_uint2(pack_bf16(unit * s.x, unit * s.y), pack_bf16(unit * s.z, unit * s.w));
+  if (i + 4 <= count) {
+    *reinterpret_cast<uint2*>(out + i) = p;
+  } else {
+    const uint16_t v[4] = {static_cast<uint16_t>(p.x), static_cast<uint16_t>(p.x >> 16),
+                           static_cast<uint16_t>(p.y), 0};
+    for (int j = 0; i + j < count; ++j) out[i + j] = v[j];
+  }
+}
+
 // One wave: 16 columns of the output for 16 tokens, all of k, straight from memory.
-// v_mfma_f32_16x16x32_bf16 with x as A (lane l: token l % 16) and the weight as B (column
-// l % 16), k 8 * (l / 16) .. + 7.
-template <int kFmt>
-__global__ __launch_bounds__(256) void w4_gemm_wave_kernel(
-    const uint16_t* __restrict__ x, const uint8_t* __restrict__ codes,
-    const uint16_t* __restrict__ scales, uint16_t* __restrict__ out, int M, int N, int K,
-    int group) {
+template <int kFmt, int kGroup>
+__global__ __launch_bounds__(256) void w4_gemm_wave_kernel(W4Args a) {
   const int lane = threadIdx.x & 63;
   const int r = lane & 15, q = lane >> 4;
+  const int M = static_cast<int>(a.M), N = static_cast<int>(a.N), K = static_cast<int>(a.K);
   const int n0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 16;
   if (n0 >= N) return;
   const int m0 = blockIdx.y * 16;
   const int64_t n = min(n0 + r, N - 1);
-  const uint16_t* xp = x + static_cast<int64_t>(min(m0 + r, M - 1)) * K + 8 * q;
-  const uint8_t* wp = codes + n * (K / 2) + 4 * q;
-  const uint16_t* sp = scales + n * (K / group);
-  f32x4_t sum{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int g = 0; g < K / group; ++g) {
-    f32x4_t acc{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k = g * group; k < (g + 1) * group; k += 32) {
-      const uint4 a = *reinterpret_cast<const uint4*>(xp + k);
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(wp + k / 2);
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
-                                                    w4_values<kFmt>(w), acc, 0, 0, 0);
-    }
-    const float s = bf16_to_f32(sp[g]);
+  const uint16_t* xp = a.x + static_cast<int64_t>(min(m0 + r, M - 1)) * K;
+  const uint8_t* wp = a.codes + n * (K / 2) + 16 * q;
+  const uint16_t* sp = a.scales + n * (K / kGroup);
+  f32x4_t sum[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
+  for (int s = 0; s < K / 128; ++s) {
+    bf16x8_t xf[1][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(s, acc[i], sum[i]);
+    for (int j = 0; j < 4; ++j)
+      xf[0][j] = *reinterpret_cast<const bf16x8_t*>(xp + 128 * s + x_offset<kGroup>(j, q));
+    StepScales<kGroup> sc;
+    sc.load(sp + s * (128 / kGroup));
+    multiply_step<kFmt, kGroup, 1, 4>(xf, *reinterpret_cast<const uint4*>(wp + 64 * s), sc, sum);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int m = m0 + 4 * q + i;
     if (m < M && n0 + r < N)
-      out[static_cast<int64_t>(m) * N + n0 + r] =
-          static_cast<uint16_t>(f32_to_bf16_bits(kUnit<kFmt> * sum[i]));
+      a.out[static_cast<int64_t>(m) * N + n0 + r] =
+          static_cast<uint16_t>(pack_bf16(kUnit<kFmt> * sum[0][i], 0.0f));
   }
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+enum Kind : int { kFew, kStream, kTile };
+struct Plan {
+  Kind kind;
+  int nt;      // tiles of 16 columns a wave
+  int splits;  // spans of k with partial sums in the workspace
+  int span;    // steps of 128 k in one
+};
+
+Plan plan_of(int64_t M, int64_t N, int64_t K) {
+  const int steps = static_cast<int>(K / 128);
+  if (M <= 16 && N < 32768) {
+    const int nt = N <= 4096 ? 1 : N <= 8192 ? 2 : 4;
+    return {kFew, nt, 1, steps};
+  }
+  if (M <= 64) {
+    const int64_t wide = 16 * kStreamWaves;  // columns a workgroup at one tile a wave
+    const int nt = M <= 32 && ceil_div(N, 4 * wide) >= 512 ? 4 : ceil_div(N, 2 * wide) >= 512 ? 2 : 1;
+    const int64_t blocks = ceil_div(N, wide * nt);
+    int splits = static_cast<int>(std::min<int64_t>({ceil_div(256, blocks), 16, steps}));
+    const int span = static_cast<int>(ceil_div(steps, splits));
+    splits = static_cast<int>(ceil_div(steps, span));
+    return {kStream, nt, splits, span};
+  }
+  return {kTile, 0, 1, steps};
+}
+int64_t part_stride(int64_t M, int64_t N) { return (M * N + 3) / 4 * 4; }
+
+template <int kFmt, int kGroup, int NT, int ST>
+hipError_t launch_few(const W4Args& a, hipStream_t stream) {
+  const int cols = NT > 1 ? 16 * NT : static_cast<int>(std::min<int64_t>(16, ceil_div(a.N, 256)));
+  const int64_t steps = a.K / 128;
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.N, cols)));
+  const dim3 block(static_cast<unsigned>(64 * std::min<int64_t>(16, ceil_div(steps, ST))));
+  if (a.M <= 4)
+    hipLaunchKernelGGL((w4_few_kernel<kFmt, kGroup, NT, ST, 1>), grid, block, 0, stream, a, cols);
+  else
+    hipLaunchKernelGGL((w4_few_kernel<kFmt, kGroup, NT, ST, 4>), grid, block, 0, stream, a, cols);
+  return hipGetLastError();
+}
+
+template <int kFmt, int kGroup, int TM, int NT, int R>
+hipError_t launch_stream(const W4Args& a, const Plan& p, hipStream_t stream) {
+  // The largest even number of steps of x that fits, all of the span if it does.
+  const int64_t room = (kStreamLds / a.M - 16) / 256 / 2 * 2;
+  const int chunk = static_cast<int>(std::min<int64_t>(room, p.span));
+  const size_t lds = static_cast<size_t>(a.M * (256 * chunk + 16));
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.N, 16 * NT * kStreamWaves)),
+                  static_cast<unsigned>(p.splits));
+  const int64_t stride = part_stride(a.M, a.N);
+  auto go = [&](auto kernel) {
+    if (lds > 65536) {
+      hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, kStreamLds);
+      if (err != hipSuccess) return err;
+    }
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * kStreamWaves), lds, stream, a, p.span, chunk, stride);
+    return hipGetLastError();
+  };
+  if (p.splits == 1) return go(w4_stream_kernel<kFmt, kGroup, TM, NT, R, false>);
+  hipError_t err = go(w4_stream_kernel<kFmt, kGroup, TM, NT, R, true>);
+  if (err != hipSuccess) return err;
+  const int64_t count = a.M * a.N;
+  hipLaunchKernelGGL(w4_reduce_kernel, dim3(static_cast<unsigned>(ceil_div(count, 1024))),
+                     dim3(256), 0, stream, a.workspace, a.out, count, stride, p.splits,
+                     kUnit<kFmt>);
+  return hipGetLastError();
+}
+
+template <int kFmt, int kGroup, int NT>
+hipError_t launch_stream_tokens(const W4Args& a, const Plan& p, hipStream_t stream) {
+  if (a.M <= 4) return launch_stream<kFmt, kGroup, 1, NT, 1>(a, p, stream);
+  if (a.M <= 16) return launch_stream<kFmt, kGroup, 1, NT, 4>(a, p, stream);
+  if (a.M <= 32) return launch_stream<kFmt, kGroup, 2, NT, 4>(a, p, stream);
+  if constexpr (NT <= 2) return launch_stream<kFmt, kGroup, 4, NT, 4>(a, p, stream);
+  return hipErrorInvalidValue;
+}
+
+template <int kFmt, int kGroup>
+hipError_t launch_group(const W4Args& a, hipStream_t stream) {
+  const Plan p = plan_of(a.M, a.N, a.K);
+  if (p.kind == kFew) {
+    if (p.nt == 4) return launch_few<kFmt, kGroup, 4, 2>(a, stream);
+    if (p.nt == 2) return launch_few<kFmt, kGroup, 2, 2>(a, stream);
+    if (a.K > 4096) return launch_few<kFmt, kGroup, 1, 4>(a, stream);
+    return launch_few<kFmt, kGroup, 1, 2>(a, stream);
+  }
+  if (p.kind == kStream) {
+    if (p.nt == 4) return launch_stream_tokens<kFmt, kGroup, 4>(a, p, stream);
+    if (p.nt == 2) return launch_stream_tokens<kFmt, kGroup, 2>(a, p, stream);
+    return launch_stream_tokens<kFmt, kGroup, 1>(a, p, stream);
+  }
+  const dim3 grid(static_cast<unsigned>((a.N + 63) / 64), static_cast<unsigned>((a.M + 15) / 16));
+  hipLaunchKernelGGL((w4_gemm_wave_kernel<kFmt, kGroup>), grid, dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+template <int kFmt>
+hipError_t launch_format(const W4Args& a, hipStream_t stream) {
+  if (a.group == 32) return launch_group<kFmt, 32>(a, stream);
+  if (a.group == 64) return launch_group<kFmt, 64>(a, stream);
+  return launch_group<kFmt, 128>(a, stream);
 }
 
 }  // namespace
 
-int64_t w4_gemm_workspace_bytes(int64_t, int64_t, int64_t) { return 0; }
+int64_t w4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  const Plan p = plan_of(M, N, K);
+  return p.splits > 1 ? p.splits * part_stride(M, N) * 4 : 0;
+}
 
 hipError_t launch_w4_gemm(const W4Args& a, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((a.N + 63) / 64), static_cast<unsigned>((a.M + 15) / 16));
-  const int m = static_cast<int>(a.M), n = static_cast<int>(a.N), k = static_cast<int>(a.K);
-  if (a.format == kW4Int4)
-    hipLaunchKernelGGL((w4_gemm_wave_kernel<kW4Int4>), grid, dim3(256), 0, stream, a.x, a.codes,
-                       a.scales, a.out, m, n, k, a.group);
-  else
-    hipLaunchKernelGGL((w4_gemm_wave_kernel<kW4E2m1>), grid, dim3(256), 0, stream, a.x, a.codes,
-                       a.scales, a.out, m, n, k, a.group);
-  return hipGetLastError();
+  return a.format == kW4Int4 ? launch_format<kW4Int4>(a, stream)
+                             : launch_format<kW4E2m1>(a, stream);
 }
 
 }  // namespace ifr
