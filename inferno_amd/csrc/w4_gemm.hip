@@ -202,70 +202,99 @@ __global__ __launch_bounds__(1024) void w4_few_kernel(W4Args a, int cols) {
   }
 }
 
-// Up to 16 TM tokens: a wave takes NT tiles of 16 columns over the workgroup's span of k, with x
-// in LDS, a chunk of k at a time, and the codes straight from memory into registers, two
-// steps ahead.  With several spans the sums go to part [span][M][N].
+// The scales of a tile's 16 rows, through LDS: a window of 64 bytes a row (kGroup / 4 steps) is one
+// load of 16 bytes a lane, where a load for each step asks for the 16 rows' lines again every
+// time (one token x 262,144 x 2,816, groups of 128: 93 us with a load a step).
+constexpr int kScalePitch = 80;  // bytes of a row's window in LDS: 20 banks apart
+template <int kGroup>
+struct ScaleWindow {
+  static constexpr int kSteps = kGroup / 4;
+  static constexpr int kStepBytes = 256 / kGroup;
+  // Row r's window from byte `at` of its scales (`row_bytes` a row; rows from n0).  Windows may
+  // reach past a row's end, into the next rows, but not past the N rows.
+  static __device__ __forceinline__ uint4 load(const W4Args& a, int64_t n0, int row_bytes, int at,
+                                               int r, int q) {
+    const uint8_t* base = reinterpret_cast<const uint8_t*>(a.scales);
+    const int64_t total = a.N * row_bytes;
+    const int64_t off = (n0 + r) * row_bytes + at + 16 * q;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if ((n0 + 15) * row_bytes + at + 64 <= total) {  // wave-uniform
+      __builtin_memcpy(&v, base + off, 16);
+    } else {
+      uint32_t d[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (off + 2 * i + 2 <= total)
+          d[i / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(base + off + 2 * i))
+                      << (16 * (i % 2));
+      v = make_uint4(d[0], d[1], d[2], d[3]);
+    }
+    return v;
+  }
+};
+
+// Up to four tokens against many columns: a wave takes NT tiles of 16 columns over all of k, with x in
+// LDS, a chunk of k at a time, and the codes straight from memory into registers, two steps
+// ahead.
 constexpr int kStreamWaves = 8;
-constexpr int kStreamLds = 72 * 1024;  // two workgroups a CU
-template <int kFmt, int kGroup, int TM, int NT, int R, bool kSplit>
-__global__ __launch_bounds__(64 * kStreamWaves, TM <= 2 ? 2 : 1) void w4_stream_kernel(
-    W4Args a, int span_steps, int chunk_steps, int64_t part_stride) {
+constexpr int kStreamTiles = 2;  // NT
+constexpr int kStreamLds = 56 * 1024;  // x: two workgroups a CU
+template <int kFmt, int kGroup>
+__global__ __launch_bounds__(64 * kStreamWaves, 4) void w4_stream_kernel(W4Args a, int chunk_steps) {
+  using Window = ScaleWindow<kGroup>;
+  constexpr int NT = kStreamTiles;
   extern __shared__ __align__(16) uint8_t xs[];
+  __shared__ __align__(16) uint8_t scale_lds[kStreamWaves * NT * 16 * kScalePitch];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = lane & 15, q = lane >> 4;
   const int M = static_cast<int>(a.M), N = static_cast<int>(a.N), K = static_cast<int>(a.K);
   const int n0 = (blockIdx.x * kStreamWaves + wave) * 16 * NT;
-  const int first = blockIdx.y * span_steps;
-  const int steps = min(span_steps, K / 128 - first);
+  const int steps = K / 128;
   const int pitch = 256 * chunk_steps + 16;  // rows four banks apart
+  uint8_t* my_scales = scale_lds + wave * NT * 16 * kScalePitch + r * kScalePitch;
 
   const uint8_t* wp[NT];
-  const uint16_t* sp[NT];
+  uint4 w[2][NT], window[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int64_t n = min(n0 + 16 * t + r, N - 1);
-    wp[t] = a.codes + n * (K / 2) + 64 * first + 16 * q;
-    sp[t] = a.scales + n * (K / kGroup) + first * (128 / kGroup);
+    wp[t] = a.codes + n * (K / 2) + 16 * q;
   }
-  uint4 w[2][NT];
-  StepScales<kGroup> sc[2][NT];
-  auto load = [&](int set, int s) {
-    s = min(s, steps - 1);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      w[set][t] = *reinterpret_cast<const uint4*>(wp[t] + 64 * s);
-      sc[set][t].load(sp[t] + s * (128 / kGroup));
-    }
-  };
-  load(0, 0);
-  load(1, 1);
-
-  f32x4_t sum[NT][TM];
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int m = 0; m < TM; ++m) sum[t][m] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  const uint8_t* xrow[TM];
-#pragma unroll
-  for (int m = 0; m < TM; ++m)
-    xrow[m] = xs + min(16 * m + token_of_row<R>(r), M - 1) * pitch;
-
-  auto multiply = [&](int set, int s, int in_chunk) {
-    bf16x8_t xf[TM][4];
-#pragma unroll
-    for (int m = 0; m < TM; ++m)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        xf[m][j] = *reinterpret_cast<const bf16x8_t*>(xrow[m] + 256 * in_chunk +
-                                                      2 * x_offset<kGroup>(j, q));
-    uint4 now[NT];
-    StepScales<kGroup> now_sc[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) now[t] = w[set][t], now_sc[t] = sc[set][t];
-    load(set, s + 2);
+  const int row_bytes = K / kGroup * 2;
+  auto load_window = [&](int s) {
+    if (s >= steps) return;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
-      multiply_step<kFmt, kGroup, TM, R>(xf, now[t], now_sc[t], sum[t]);
+      window[t] = Window::load(a, n0 + 16 * t, row_bytes, s * Window::kStepBytes, r, q);
+  };
+  // Two steps, the halves of a row's 128-byte lines, behind each other: with a step of the first
+  // half between them lines are fetched twice (75 us against 68 at 262,144 x 2,816).
+  auto load = [&](int s) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[h][t] = *reinterpret_cast<const uint4*>(wp[t] + 64 * min(s + h, steps - 1));
+  };
+  load_window(0);
+  load(0);
+
+  f32x4_t sum[NT][1];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) sum[t][0] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const uint8_t* xrow = xs + min(token_of_row<1>(r), M - 1) * pitch;
+  auto multiply = [&](const uint4 (&now)[NT], int s, int in_chunk) {
+    bf16x8_t xf[1][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      xf[0][j] = *reinterpret_cast<const bf16x8_t*>(xrow + 256 * in_chunk + 2 * x_offset<kGroup>(j, q));
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      StepScales<kGroup> sc;
+      sc.load(reinterpret_cast<const uint16_t*>(my_scales + t * 16 * kScalePitch +
+                                                s % Window::kSteps * Window::kStepBytes));
+      multiply_step<kFmt, kGroup, 1, 1>(xf, now[t], sc, sum[t]);
+    }
   };
   for (int c0 = 0; c0 < steps; c0 += chunk_steps) {
     const int here = min(chunk_steps, steps - c0);
@@ -275,14 +304,180 @@ __global__ __launch_bounds__(64 * kStreamWaves, TM <= 2 ? 2 : 1) void w4_stream_
     for (int i = threadIdx.x; i < M * per; i += 64 * kStreamWaves) {
       const int m = i / per, at = i - m * per;
       *reinterpret_cast<uint4*>(xs + m * pitch + 16 * at) = *reinterpret_cast<const uint4*>(
-          a.x + static_cast<int64_t>(m) * K + 128 * (first + c0) + 8 * at);
+          a.x + static_cast<int64_t>(m) * K + 128 * c0 + 8 * at);
     }
     __syncthreads();
-    for (int s = 0; s < here; s += 2) {
-      multiply(0, c0 + s, s);
-      if (s + 1 < here) multiply(1, c0 + s + 1, s + 1);
+    for (int s = c0; s < c0 + here; s += 2) {
+      if (s % Window::kSteps == 0) {  // the wave's own LDS: its accesses are in order
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          *reinterpret_cast<uint4*>(my_scales + t * 16 * kScalePitch + 16 * q) = window[t];
+        load_window(s + Window::kSteps);
+      }
+      uint4 now[2][NT];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) now[h][t] = w[h][t];
+      load(s + 2);
+      multiply(now[0], s, s - c0);
+      if (s + 1 < c0 + here) multiply(now[1], s + 1, s + 1 - c0);
     }
   }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int n = n0 + 16 * t + r;
+    if (n < N && q < M)
+      a.out[static_cast<int64_t>(q) * N + n] =
+          static_cast<uint16_t>(pack_bf16(kUnit<kFmt> * sum[t][0][0], 0.0f));
+  }
+}
+
+// 17 to 64 tokens, and 5 to 16 against many columns: as the stream kernel, with x in units of two steps that go
+// from memory into LDS by themselves (global_load_lds), one unit ahead, so that W waves of NT tiles
+// share it behind one barrier a unit.  The codes of a unit are loaded again as soon as the unit
+// before is multiplied, two units ahead of their use.
+//
+// 16-byte chunk c of x row r lies at c ^ (r % 16), so that the 16 rows of a quarter of a
+// fragment read lie in 16 different bank groups.
+typedef __attribute__((address_space(3))) void lds_void_t;
+template <int kFmt, int kGroup, int TM, int NT, int W, bool kSplit>
+__global__ __launch_bounds__(64 * W, W == 16 ? 4 : 2) void w4_batch_kernel(W4Args a, int span_steps,
+                                                              int64_t part_stride) {
+  using Window = ScaleWindow<kGroup>;
+  constexpr int kUnitBytes = TM * 16 * 512;
+  constexpr int kLoads = (TM * 8 + W - 1) / W;  // 1 KiB loads (two rows) of a wave a unit
+  __shared__ __align__(16) uint8_t x0[kUnitBytes];
+  __shared__ __align__(16) uint8_t x1[kUnitBytes];
+  __shared__ __align__(16) uint8_t scale_lds[W * NT * 16 * kScalePitch];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int r = lane & 15, q = lane >> 4;
+  const int M = static_cast<int>(a.M), N = static_cast<int>(a.N), K = static_cast<int>(a.K);
+  const int n0 = (blockIdx.x * W + wave) * 16 * NT;
+  const int first = blockIdx.y * span_steps;
+  const int steps = min(span_steps, K / 128 - first);
+  const int units = (steps + 1) / 2;
+  uint8_t* my_scales = scale_lds + wave * NT * 16 * kScalePitch + r * kScalePitch;
+
+  const uint8_t* wp[NT];
+  uint4 w[2][2][NT], window[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t n = min(n0 + 16 * t + r, N - 1);
+    wp[t] = a.codes + n * (K / 2) + 64 * first + 16 * q;
+  }
+  const int row_bytes = K / kGroup * 2;
+  auto load_window = [&](int s) {
+    if (s >= steps) return;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      window[t] = Window::load(a, n0 + 16 * t, row_bytes, (first + s) * Window::kStepBytes, r, q);
+  };
+  auto load_half = [&](int set, int u, int t) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      w[set][h][t] = *reinterpret_cast<const uint4*>(wp[t] + 64 * min(2 * u + h, steps - 1));
+  };
+  // x rows 2 i and 2 i + 1 of unit u; rows past M and k past K repeat others (not used).
+  const uint16_t* xsrc[kLoads];
+  int xcol[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int row = 2 * (wave + W * i) + (lane >> 5);
+    xsrc[i] = a.x + static_cast<int64_t>(min(row, M - 1)) * K;
+    xcol[i] = 128 * first + 8 * ((lane & 31) ^ (row & 15));
+  }
+  auto load_x = [&](int u, uint8_t* buf) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      if (TM * 8 % W == 0 || wave + W * i < TM * 8)
+        __builtin_amdgcn_global_load_lds(
+            static_cast<const void*>(xsrc[i] + min(xcol[i] + 256 * u, K - 8)),
+            (lds_void_t*)(buf + 1024 * (wave + W * i)), 16, 0, 0);
+  };
+
+  f32x4_t sum[NT][TM];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int m = 0; m < TM; ++m) sum[t][m] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+  auto multiply = [&](uint4 (&now)[NT], int s, int half, const uint8_t* xb) {
+    StepScales<kGroup> sc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      sc[t].load(reinterpret_cast<const uint16_t*>(my_scales + t * 16 * kScalePitch +
+                                                   s % Window::kSteps * Window::kStepBytes));
+#pragma unroll
+    for (int t = 0; t < NT; ++t) order_words<kGroup>(now[t]);
+    constexpr int kPer = kGroup / 32;  // words of a group
+#pragma unroll
+    for (int g = 0; g < 4 / kPer; ++g) {
+      f32x4_t acc[NT][TM];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int m = 0; m < TM; ++m) acc[t][m] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = g * kPer; j < (g + 1) * kPer; ++j) {
+        bf16x8_t xf[TM];
+#pragma unroll
+        for (int m = 0; m < TM; ++m)
+          xf[m] = *reinterpret_cast<const bf16x8_t*>(
+              xb + 512 * (16 * m + r) + 256 * half + 16 * ((x_offset<kGroup>(j, q) / 8) ^ r));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const uint32_t word = j == 0 ? now[t].x : j == 1 ? now[t].y : j == 2 ? now[t].z : now[t].w;
+          const bf16x8_t b = w4_values<kFmt>(word);
+#pragma unroll
+          for (int m = 0; m < TM; ++m)
+            acc[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[m], b, acc[t][m], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float scale = sc[t].get(g);
+#pragma unroll
+        for (int m = 0; m < TM; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            sum[t][m][i] = __builtin_fmaf(scale, acc[t][m][i], sum[t][m][i]);
+      }
+    }
+  };
+
+  load_window(0);
+  load_x(0, x0);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int set = 0; set < 2; ++set)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) load_half(set, set, t);
+  auto unit = [&](int set, int u, const uint8_t* cur, uint8_t* next) {
+    // x of unit u has landed when only the codes loaded behind it are outstanding (2 NT loads at
+    // least), and nobody reads the buffer of unit u - 1 any more.
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NT) : "memory");
+    load_x(min(u + 1, units - 1), next);
+    __builtin_amdgcn_sched_barrier(0);
+    const int s = 2 * u;
+    if (s % Window::kSteps == 0) {  // the wave's own LDS: its accesses are in order
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        *reinterpret_cast<uint4*>(my_scales + t * 16 * kScalePitch + 16 * q) = window[t];
+      load_window(s + Window::kSteps);
+    }
+    multiply(w[set][0], s, 0, cur);
+    if (s + 1 < steps) multiply(w[set][1], s + 1, 1, cur);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) load_half(set, u + 2, t);
+  };
+  for (int u = 0; u < units; u += 2) {
+    unit(0, u, x0, x1);
+    if (u + 1 < units) unit(1, u + 1, x1, x0);
+  }
+  // No load may still be on its way into LDS when the workgroup ends.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int n = n0 + 16 * t + r;
@@ -290,8 +485,8 @@ __global__ __launch_bounds__(64 * kStreamWaves, TM <= 2 ? 2 : 1) void w4_stream_
 #pragma unroll
     for (int m = 0; m < TM; ++m)
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const int token = 16 * m + q * R + i;
+      for (int i = 0; i < 4; ++i) {
+        const int token = 16 * m + 4 * q + i;
         if (token >= M) continue;
         const int64_t o = static_cast<int64_t>(token) * N + n;
         if constexpr (kSplit)
@@ -359,30 +554,33 @@ __global__ __launch_bounds__(256) void w4_gemm_wave_kernel(W4Args a) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-enum Kind : int { kFew, kStream, kTile };
+enum Kind : int { kFew, kStream, kBatch, kTile };
 struct Plan {
   Kind kind;
-  int nt;      // tiles of 16 columns a wave
-  int splits;  // spans of k with partial sums in the workspace
-  int span;    // steps of 128 k in one
+  int nt, waves;  // tiles of 16 columns a wave, and waves of a workgroup
+  int splits;     // spans of k with partial sums in the workspace
+  int span;       // steps of 128 k in one
 };
+
+// From 32,768 columns there are 128 workgroups of 256 columns or more, and the kernels that
+// stream them.
+constexpr int64_t kManyColumns = 32768;
 
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
   const int steps = static_cast<int>(K / 128);
-  if (M <= 16 && N < 32768) {
-    const int nt = N <= 4096 ? 1 : N <= 8192 ? 2 : 4;
-    return {kFew, nt, 1, steps};
-  }
+  if (M <= 16 && N < kManyColumns) return {kFew, N <= 4096 ? 1 : N <= 8192 ? 2 : 4, 16, 1, steps};
+  if (M <= 4) return {kStream, kStreamTiles, kStreamWaves, 1, steps};
   if (M <= 64) {
-    const int64_t wide = 16 * kStreamWaves;  // columns a workgroup at one tile a wave
-    const int nt = M <= 32 && ceil_div(N, 4 * wide) >= 512 ? 4 : ceil_div(N, 2 * wide) >= 512 ? 2 : 1;
-    const int64_t blocks = ceil_div(N, wide * nt);
-    int splits = static_cast<int>(std::min<int64_t>({ceil_div(256, blocks), 16, steps}));
-    const int span = static_cast<int>(ceil_div(steps, splits));
-    splits = static_cast<int>(ceil_div(steps, span));
-    return {kStream, nt, splits, span};
+    const bool many = N >= kManyColumns;
+    const int nt = M > 16 && M <= 32 && many ? 2 : 1;
+    const int waves = !many ? 4 : M <= 32 ? 16 : 8;
+    const int64_t blocks = ceil_div(N, 16 * nt * waves);
+    // Spans of an even number of steps, four at least.
+    const int64_t want = std::min<int64_t>(ceil_div(256, blocks), std::min(16, (steps + 3) / 4));
+    const int span = static_cast<int>(ceil_div(ceil_div(steps, want), 2) * 2);
+    return {kBatch, nt, waves, static_cast<int>(ceil_div(steps, span)), span};
   }
-  return {kTile, 0, 1, steps};
+  return {kTile, 0, 0, 1, steps};
 }
 int64_t part_stride(int64_t M, int64_t N) { return (M * N + 3) / 4 * 4; }
 
@@ -399,41 +597,36 @@ hipError_t launch_few(const W4Args& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int kFmt, int kGroup, int TM, int NT, int R>
-hipError_t launch_stream(const W4Args& a, const Plan& p, hipStream_t stream) {
-  // The largest even number of steps of x that fits, all of the span if it does.
+template <int kFmt, int kGroup>
+hipError_t launch_stream(const W4Args& a, hipStream_t stream) {
+  // The largest even number of steps of x that fits, all of them if they do.
   const int64_t room = (kStreamLds / a.M - 16) / 256 / 2 * 2;
-  const int chunk = static_cast<int>(std::min<int64_t>(room, p.span));
-  const size_t lds = static_cast<size_t>(a.M * (256 * chunk + 16));
-  const dim3 grid(static_cast<unsigned>(ceil_div(a.N, 16 * NT * kStreamWaves)),
+  const int chunk = static_cast<int>(std::min<int64_t>(room, a.K / 128));
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.N, 16 * kStreamTiles * kStreamWaves)));
+  hipLaunchKernelGGL((w4_stream_kernel<kFmt, kGroup>), grid, dim3(64 * kStreamWaves),
+                     static_cast<size_t>(a.M * (256 * chunk + 16)), stream, a, chunk);
+  return hipGetLastError();
+}
+
+template <int kFmt, int kGroup, int TM, int NT, int W>
+hipError_t launch_batch(const W4Args& a, const Plan& p, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.N, 16 * NT * W)),
                   static_cast<unsigned>(p.splits));
   const int64_t stride = part_stride(a.M, a.N);
-  auto go = [&](auto kernel) {
-    if (lds > 65536) {
-      hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, kStreamLds);
-      if (err != hipSuccess) return err;
-    }
-    hipLaunchKernelGGL(kernel, grid, dim3(64 * kStreamWaves), lds, stream, a, p.span, chunk, stride);
+  if (p.splits == 1) {
+    hipLaunchKernelGGL((w4_batch_kernel<kFmt, kGroup, TM, NT, W, false>), grid, dim3(64 * W), 0,
+                       stream, a, p.span, stride);
     return hipGetLastError();
-  };
-  if (p.splits == 1) return go(w4_stream_kernel<kFmt, kGroup, TM, NT, R, false>);
-  hipError_t err = go(w4_stream_kernel<kFmt, kGroup, TM, NT, R, true>);
+  }
+  hipLaunchKernelGGL((w4_batch_kernel<kFmt, kGroup, TM, NT, W, true>), grid, dim3(64 * W), 0, stream,
+                     a, p.span, stride);
+  const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   const int64_t count = a.M * a.N;
   hipLaunchKernelGGL(w4_reduce_kernel, dim3(static_cast<unsigned>(ceil_div(count, 1024))),
                      dim3(256), 0, stream, a.workspace, a.out, count, stride, p.splits,
                      kUnit<kFmt>);
   return hipGetLastError();
-}
-
-template <int kFmt, int kGroup, int NT>
-hipError_t launch_stream_tokens(const W4Args& a, const Plan& p, hipStream_t stream) {
-  if (a.M <= 4) return launch_stream<kFmt, kGroup, 1, NT, 1>(a, p, stream);
-  if (a.M <= 16) return launch_stream<kFmt, kGroup, 1, NT, 4>(a, p, stream);
-  if (a.M <= 32) return launch_stream<kFmt, kGroup, 2, NT, 4>(a, p, stream);
-  if constexpr (NT <= 2) return launch_stream<kFmt, kGroup, 4, NT, 4>(a, p, stream);
-  return hipErrorInvalidValue;
 }
 
 template <int kFmt, int kGroup>
@@ -445,10 +638,13 @@ hipError_t launch_group(const W4Args& a, hipStream_t stream) {
     if (a.K > 4096) return launch_few<kFmt, kGroup, 1, 4>(a, stream);
     return launch_few<kFmt, kGroup, 1, 2>(a, stream);
   }
-  if (p.kind == kStream) {
-    if (p.nt == 4) return launch_stream_tokens<kFmt, kGroup, 4>(a, p, stream);
-    if (p.nt == 2) return launch_stream_tokens<kFmt, kGroup, 2>(a, p, stream);
-    return launch_stream_tokens<kFmt, kGroup, 1>(a, p, stream);
+  if (p.kind == kStream) return launch_stream<kFmt, kGroup>(a, stream);
+  if (p.kind == kBatch) {
+    if (p.waves == 16 && p.nt == 1) return launch_batch<kFmt, kGroup, 1, 1, 16>(a, p, stream);
+    if (p.waves == 16) return launch_batch<kFmt, kGroup, 2, 2, 16>(a, p, stream);
+    if (p.waves == 8) return launch_batch<kFmt, kGroup, 4, 1, 8>(a, p, stream);
+    if (a.M <= 32) return launch_batch<kFmt, kGroup, 2, 1, 4>(a, p, stream);
+    return launch_batch<kFmt, kGroup, 4, 1, 4>(a, p, stream);
   }
   const dim3 grid(static_cast<unsigned>((a.N + 63) / 64), static_cast<unsigned>((a.M + 15) / 16));
   hipLaunchKernelGGL((w4_gemm_wave_kernel<kFmt, kGroup>), grid, dim3(256), 0, stream, a);

@@ -38,7 +38,10 @@ SHAPES = [(1, 1, 128), (1, 16, 128), (1, 2816, 4096), (2, 17, 256), (3, 65, 384)
           (17, 50, 512), (31, 257, 2816), (32, 80, 4096), (33, 511, 1280), (48, 64, 128),
           (61, 2816, 4096), (64, 1000, 256), (65, 130, 2816), (100, 257, 512), (127, 96, 384),
           (128, 128, 128), (129, 129, 1024), (200, 2816, 640), (255, 63, 2816), (300, 400, 4096),
-          (513, 2816, 512), (1000, 1111, 896), (2050, 300, 256)]
+          (513, 2816, 512), (1000, 1111, 896), (2050, 300, 256),
+          # Many columns: streams of weights, one to 64 tokens, odd steps and x in more than one chunk.
+          (1, 32768, 256), (4, 33001, 384), (3, 40000, 128), (2, 32769, 16512), (5, 32800, 384), (16, 33333, 640), (17, 32768, 256),
+          (32, 32999, 896), (33, 32770, 512), (64, 40001, 384)]
 
 
 @pytest.mark.parametrize("fmt", ["int4", "e2m1"])
