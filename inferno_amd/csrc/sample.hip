@@ -6,19 +6,29 @@
 //   the token is the first i of M, by index, with sum over j <= i in M of w_j > u * sum over M of w
 //
 // A draw lands next to a border between two tokens as often as the sums are wrong there: with
-// 2^18 tokens of equal weight f32 sums would give another token in 2 to 3 % of draws.
-// The weights are f64 exponentials, taken as integers of 2^-shift (44 bits at 2^18 tokens) and
-// added as 64-bit integers: the sums do not depend on their order.
+// 2^18 tokens of equal weight f32 sums would give another token in 2 to 3 % of draws.  So the
+// weights and sums have 64 bits (f64 adds run at the rate of f32 ones on this card), and every sum is
+// taken in an order that does not depend on timing.
 //
-// K and P are prefixes of the order by z, that is all keys above a key and the first few tokens of
-// that key: the key is found 11, 11 and 10 bits at a time from histograms of counts or weights.
+// Three launches.  The first reads every logit once and leaves, for each 64 places, the
+// largest key and, for rows that need it, the sum of weights relative to it.  The second has a
+// workgroup a row, which in most cases reads a few of those 64 again and is done:
+//  - without any limit, the sums give the 64 tokens in which the draw lands;
+//  - a top-k of up to 1,024: the k-th largest of the 64s' largest is at most the k-th largest
+//    logit, so the candidates are the tokens above it, little more than k, which are sorted;
+//  - top-p alone: the same with 128 and then 1,024, if the cut lies above; min-p alone has its
+//    threshold.
+// The third, with a larger workgroup a row, takes the rows that are left: a cut among very many
+// tokens in one pass (sample_wide), a larger top-k or very many equal logits by descending
+// through the keys, 11, 11 and 10 bits at a time, in histograms of counts or weights of the row.
 #include "common.hpp"
 #include "step.hpp"
 
 namespace ifr {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024;  // of a row in the third launch
+constexpr int kPickThreads = 512;
 constexpr int kBins = 2048;
 constexpr int kMaxSubs = 4096;  // sub-chunks of a row
 
@@ -40,13 +50,37 @@ __device__ __forceinline__ float load_logit(const void* row, int64_t i) {
     return bf16_to_f32(static_cast<const uint16_t*>(row)[i]);
 }
 
+// 2^t for t <= 0: 2^n times the Taylor sum of 2^f = e^(f ln 2), |f| <= 1/2, up to the eleventh
+// power (the next term is below 2^-47 of the result); 0 below 2^-1000, and for NaN.
+constexpr double kLn2 = 0.693147180559945309417;
+template <int n>
+constexpr double kTaylor = kTaylor<n - 1> * kLn2 / n;
+template <>
+constexpr double kTaylor<0> = 1.0;
+__device__ __forceinline__ double exp2_neg(double t) {
+  const double n = __builtin_rint(t);
+  const double f = t - n;
+  double p = kTaylor<11>;
+  p = __builtin_fma(p, f, kTaylor<10>);
+  p = __builtin_fma(p, f, kTaylor<9>);
+  p = __builtin_fma(p, f, kTaylor<8>);
+  p = __builtin_fma(p, f, kTaylor<7>);
+  p = __builtin_fma(p, f, kTaylor<6>);
+  p = __builtin_fma(p, f, kTaylor<5>);
+  p = __builtin_fma(p, f, kTaylor<4>);
+  p = __builtin_fma(p, f, kTaylor<3>);
+  p = __builtin_fma(p, f, kTaylor<2>);
+  p = __builtin_fma(p, f, kTaylor<1>);
+  p = __builtin_fma(p, f, 1.0);
+  return t > -1000.0 ? __builtin_ldexp(p, static_cast<int>(n)) : 0.0;
+}
+
 struct Weights {
   uint32_t top;  // the largest key
-  double zmax, inv_t, unit;
+  double zmax, rate, unit;  // rate: log2 e / T; unit: of the integers of the descent
   __device__ __forceinline__ double real(uint32_t key) const {
     if (key == top) return 1.0;
-    const double a = (static_cast<double>(logit_of(key)) - zmax) * inv_t;
-    return a > -745.0 ? exp(a) : 0.0;  // NaN (inf - inf, inf * 0): 0
+    return exp2_neg((static_cast<double>(logit_of(key)) - zmax) * rate);  // inf * 0: NaN, so 0
   }
   __device__ __forceinline__ uint64_t fixed(uint32_t key) const {
     return static_cast<uint64_t>(__builtin_rint(real(key) * unit));
@@ -97,45 +131,166 @@ struct Cut {
   unsigned long long ties;     // that many, the lowest indexes first
 };
 
+constexpr double kLog2E = 1.44269504088896340736;
+
+// What a row asks for; k 0: no limit.
+struct Asked {
+  float t, top_p, min_p;
+  int64_t k;
+  __device__ __forceinline__ Asked(const SampleArgs& a, int64_t row) {
+    t = a.temperature ? a.temperature[row] : 1.0f;
+    k = a.top_k ? a.top_k[row] : 0;
+    if (k < 0 || k >= a.vocab) k = 0;
+    if (!(t > 0.0f)) k = a.vocab > 1 ? 1 : 0;
+    top_p = a.top_p ? a.top_p[row] : 1.0f;
+    if (!(top_p < 1.0f)) top_p = 1.0f;
+    if (!(top_p > 0.0f)) top_p = 0.0f;
+    min_p = a.min_p ? a.min_p[row] : 0.0f;
+    if (!(min_p > 0.0f)) min_p = 0.0f;
+  }
+  __device__ __forceinline__ double rate() const {
+    return t > 0.0f ? kLog2E / static_cast<double>(t) : kLog2E;
+  }
+  // The sums of the first launch are those of the whole row.
+  __device__ __forceinline__ bool needs_sums() const {
+    return k == 0 && (top_p < 1.0f || min_p == 0.0f);
+  }
+};
+
+// A row's logits in vectors of 16 bytes from the last aligned address at or before it: place p
+// holds token p - shift.
 template <bool kF32>
-__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, int shift) {
-  __shared__ unsigned long long bins[kMaxSubs];
-  __shared__ uint32_t tie_counts[kMaxSubs];
-  __shared__ unsigned long long waves[kThreads / 64];
-  __shared__ Found found;
-  __shared__ uint32_t s_top;
-  const int64_t row = blockIdx.x;
+struct RowView {
+  static constexpr int kPer = kF32 ? 4 : 8;  // logits of a vector
+  const void* z;
+  int shift, vocab;
+  __device__ __forceinline__ RowView(const SampleArgs& a, int64_t row) {
+    const char* p = static_cast<const char*>(a.logits) + row * a.row_stride * (kF32 ? 4 : 2);
+    z = p;
+    shift = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15) / (kF32 ? 4 : 2);
+    vocab = static_cast<int>(a.vocab);
+  }
+  __device__ __forceinline__ uint32_t key(int place) const {
+    const int i = place - shift;
+    return i >= 0 && i < vocab ? key_of(load_logit<kF32>(z, i)) : 0;
+  }
+  // A vector's bits; those of -inf behind the row's ends.
+  __device__ __forceinline__ uint4 raw(int place) const {
+    const int i = place - shift;
+    if (i >= 0 && i + kPer <= vocab) {
+      if constexpr (kF32)
+        return *reinterpret_cast<const uint4*>(static_cast<const float*>(z) + i);
+      else
+        return *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(z) + i);
+    }
+    uint32_t b[4];
+    if constexpr (kF32) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        b[j] = i + j >= 0 && i + j < vocab ? static_cast<const uint32_t*>(z)[i + j] : 0xFF800000u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t v = i + j >= 0 && i + j < vocab ? static_cast<const uint16_t*>(z)[i + j] : 0xFF80u;
+        b[j / 2] |= v << (16 * (j % 2));
+      }
+    }
+    return make_uint4(b[0], b[1], b[2], b[3]);
+  }
+  // Its logits; -inf in the place of NaN.
+  static __device__ __forceinline__ void unpack(uint4 u, float (&v)[kPer]) {
+    if constexpr (kF32) {
+      v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y);
+      v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
+    } else {
+      v[0] = bf16_lo(u.x), v[1] = bf16_hi(u.x), v[2] = bf16_lo(u.y), v[3] = bf16_hi(u.y);
+      v[4] = bf16_lo(u.z), v[5] = bf16_hi(u.z), v[6] = bf16_lo(u.w), v[7] = bf16_hi(u.w);
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = __builtin_fmaxf(v[j], -__builtin_inff());
+  }
+  __device__ __forceinline__ void logits(int place, float (&v)[kPer]) const { unpack(raw(place), v); }
+};
+
+constexpr int kSub = 64;             // places of a sub-chunk
+constexpr int kScanThreads = 256;
+constexpr int kScanVectors = 4;      // of a thread
+
+// subs[row][s]: the largest key of sub-chunk s; sums[row][s]: its weights relative to that key.
+template <bool kF32>
+__global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleArgs a, uint32_t* subs,
+                                                                   double* sums, int num_subs,
+                                                                   int chunks) {
+  constexpr int kPer = RowView<kF32>::kPer;
+  constexpr int kLanes = kSub / kPer;  // of a sub-chunk
+  const int64_t row = blockIdx.x / static_cast<unsigned>(chunks);
+  const int chunk = static_cast<int>(blockIdx.x - row * chunks);
+  const RowView<kF32> view(a, row);
+  float z[kScanVectors][kPer];
+#pragma unroll
+  for (int v = 0; v < kScanVectors; ++v)
+    view.logits(((chunk * kScanVectors + v) * kScanThreads + static_cast<int>(threadIdx.x)) * kPer, z[v]);
+  const Asked asked(a, row);
+  const bool with_sums = asked.needs_sums();
+  const double rate = asked.rate();
+#pragma unroll
+  for (int v = 0; v < kScanVectors; ++v) {
+    float top = z[v][0];
+#pragma unroll
+    for (int j = 1; j < kPer; ++j) top = __builtin_fmaxf(top, z[v][j]);
+#pragma unroll
+    for (int d = 1; d < kLanes; d *= 2) top = __builtin_fmaxf(top, __shfl_xor(top, d));
+    const int s = ((chunk * kScanVectors + v) * kScanThreads + static_cast<int>(threadIdx.x)) / kLanes;
+    const bool writes = threadIdx.x % kLanes == 0 && s < num_subs;
+    if (writes) subs[row * num_subs + s] = key_of(top);
+    if (!with_sums) continue;
+    const double zmax = static_cast<double>(top);
+    double sum = 0.0;
+    if (__any(top == __builtin_inff())) {  // equal infinities weigh 1, though their difference is NaN
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        sum += z[v][j] == top && top > -__builtin_inff()
+                   ? 1.0
+                   : exp2_neg((static_cast<double>(z[v][j]) - zmax) * rate);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        sum += exp2_neg((static_cast<double>(z[v][j]) - zmax) * rate);
+    }
+#pragma unroll
+    for (int d = 1; d < kLanes; d *= 2) sum += __shfl_xor(sum, d);
+    if (writes) sums[row * num_subs + s] = sum;
+  }
+}
+
+__device__ __forceinline__ double uniform_of(const SampleArgs& a, int64_t row) {
+  const float u = a.uniform[row];
+  return u > 0.0f ? (u < 1.0f ? static_cast<double>(u) : 1.0 - 0x1p-24) : 0.0;
+}
+
+// The row by its keys' bits.
+template <bool kF32>
+__device__ __noinline__ void sample_descent(const SampleArgs& a, int shift, int64_t row,
+                                            uint32_t top, unsigned long long* bins,
+                                            uint32_t* tie_counts, unsigned long long* waves,
+                                            Found* found_at) {
+  Found& found = *found_at;
+  const Asked asked(a, row);
   const int vocab = static_cast<int>(a.vocab);
   const void* z = static_cast<const char*>(a.logits) + row * a.row_stride * (kF32 ? 4 : 2);
   const int tid = threadIdx.x, lane = tid & 63;
-
-  if (tid == 0) s_top = 0;
-  __syncthreads();
-  uint32_t top = 0;
+  const int64_t k = asked.k;
+  const float top_p = asked.top_p, min_p = asked.min_p;
   int valid = 0;
-  for (int i = tid; i < vocab; i += kThreads) {
-    const uint32_t k = key_of(load_logit<kF32>(z, i));
-    top = max(top, k);
-    valid += k != 0;
-  }
-  atomicMax(&s_top, top);
+  for (int i = tid; i < vocab; i += kThreads) valid += key_of(load_logit<kF32>(z, i)) != 0;
   unsigned long long count = block_inclusive<unsigned long long>(valid, waves);
   if (tid == kThreads - 1) found.above = count;
   __syncthreads();
-  top = s_top;
   count = found.above;
   __syncthreads();
-  if (count == 0) {  // block-uniform
-    if (tid == 0) a.tokens[row] = -1;
-    return;
-  }
-
-  const float t = a.temperature ? a.temperature[row] : 1.0f;
-  int64_t k = a.top_k ? a.top_k[row] : 0;
-  if (!(t > 0.0f)) k = 1;
-  const float top_p = a.top_p ? a.top_p[row] : 1.0f;
-  const float min_p = a.min_p ? a.min_p[row] : 0.0f;
-  const Weights w{top, static_cast<double>(logit_of(top)), t > 0.0f ? 1.0 / static_cast<double>(t) : 1.0,
+  const Weights w{top, static_cast<double>(logit_of(top)), asked.rate(),
                   static_cast<double>(1ull << shift)};
 
   // Keys of `digit` bits at a time: the histogram of value(key) over the keys that
@@ -156,7 +311,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, int 
         if (v) atomicAdd(&bins[(key >> lo) & ((1u << width) - 1)], v);
       }
       __syncthreads();
-      const Found f = find_from_top(bins, target - above, waves, &found);
+      const Found f = find_from_top(bins, target - above, waves, found_at);
       above += f.above;
       prefix = (prefix << width) | f.bin;
       __syncthreads();
@@ -185,8 +340,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, int 
     const unsigned long long strict = found.above;
     __syncthreads();
     const unsigned long long total = strict + cut.ties * tie;
-    const double p = top_p > 0.0f ? static_cast<double>(top_p) : 0.0;  // NaN: off, by the test above
-    const double want = __builtin_ceil(p * static_cast<double>(total));
+    const double want = __builtin_ceil(static_cast<double>(top_p) * static_cast<double>(total));
     unsigned long long target = want < 1.0 ? 1 : static_cast<unsigned long long>(want);
     target = target < total ? target : total;
     if (target > strict) {  // within the ties of the top-k cut
@@ -202,7 +356,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, int 
   int sub = 8;
   while (((vocab - 1) >> sub) + 1 > kMaxSubs) ++sub;
   const int subs = ((vocab - 1) >> sub) + 1;
-  const double floor_w = min_p > 0.0f ? static_cast<double>(min_p) : 0.0;
+  const double floor_w = static_cast<double>(min_p);
   auto kept = [&](uint32_t key) -> unsigned long long {
     if (key == 0) return 0;
     const double v = w.real(key);
@@ -253,9 +407,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, int 
   __syncthreads();
   const unsigned long long total = found.above;
   __syncthreads();
-  const float u = a.uniform[row];
-  const double ud = u > 0.0f ? (u < 1.0f ? static_cast<double>(u) : 1.0 - 0x1p-24) : 0.0;
-  unsigned long long goal = static_cast<unsigned long long>(ud * static_cast<double>(total));
+  unsigned long long goal = static_cast<unsigned long long>(uniform_of(a, row) * static_cast<double>(total));
   if (goal >= total) goal = total - 1;  // total >= 1: the largest logit is kept
   __shared__ int s_sub;
   __shared__ unsigned long long s_before, s_ties;
@@ -301,6 +453,668 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, int 
   }
 }
 
+constexpr int kMaxK = 1024;     // candidates that are sought
+constexpr int kMaxSorted = 2048;  // and at most taken
+
+// Descending, in place; slots from n on hold 0 afterwards up to the next power of two.
+template <int kT>
+__device__ __forceinline__ void sort_descending(unsigned long long* v, unsigned long long* tmp, int n) {
+  const int tid = threadIdx.x;
+  if (n <= 256) {  // each entry counts those above it
+    if (tid < n) {
+      const unsigned long long mine = v[tid];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += v[j] > mine;
+      tmp[rank] = mine;
+    }
+    __syncthreads();
+    if (tid < n) v[tid] = tmp[tid];
+    __syncthreads();
+    return;
+  }
+  int size = 512;
+  while (size < n) size *= 2;
+  for (int i = n + tid; i < size; i += kT) v[i] = 0;
+  __syncthreads();
+  for (int width = 2; width <= size; width *= 2) {
+    for (int d = width / 2; d > 0; d /= 2) {
+      for (int i = tid; i < size / 2; i += kT) {
+        const int lo = 2 * i - (i & (d - 1)), hi = lo + d;
+        const unsigned long long x = v[lo], y = v[hi];
+        const bool up = (lo & width) != 0;  // ascending runs
+        if ((x < y) != up) v[lo] = y, v[hi] = x;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+constexpr int kMaxBand = 12288;
+constexpr uint32_t kInfKey = 0xFF800000u;  // of +inf
+
+// A row without a top-k that keeps very many tokens: one pass over its logits.
+//
+// min-p alone: the pass adds the weights of the kept ones by sub-chunk.  top-p: first a sample (about
+// 32,000 of the logits, evenly spread) says where the weights below add up to about 1 - top_p of all;
+// those are many small ones, so a sample of them is good to a few percent.  Tokens above that
+// band go to the sums, those within it to a list, in which the cut is then found from its keys' bits.
+// False if it is not there (or the list is full, or very many are equal): the caller descends.
+//
+// A CU takes 2 us for each instruction on all of 2^18 logits, so the pass does little for each:
+// those at or above the band are moved together, 64 at a time, before their weights are taken.
+template <bool kF32>
+__device__ __noinline__ bool sample_wide(const SampleArgs& a, int64_t row, const RowView<kF32>& view,
+                                         const Asked& asked, const Weights& w, double total,
+                                         int num_subs, unsigned long long* sub_sums,
+                                         unsigned long long* digits, unsigned long long* band,
+                                         unsigned long long* waves, Found* found) {
+  unsigned long long* queues = digits;  // between the two uses of the digits
+  __shared__ unsigned long long order[256];
+  constexpr int kPer = RowView<kF32>::kPer;
+  constexpr int kBand = 1024;  // bins of the sample
+  __shared__ int s_n, s_a, s_b, s_place;
+  __shared__ unsigned long long s_u64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int vectors = num_subs * kSub / kPer;
+  const float zmax = logit_of(w.top);
+  const bool nucleus = asked.top_p < 1.0f;
+  const double floor_w = static_cast<double>(asked.min_p);
+  // Bins of (zmax - z) * per: `lim` is the first that is not looked at, `above` the first of the band.
+  float per, lim;
+  int above;
+  double goal = 0.0;  // in units
+  if (nucleus) {
+    goal = static_cast<double>(asked.top_p) * total * w.unit;
+    const double rest = (1.0 - static_cast<double>(asked.top_p)) * total;
+    // Tokens of less than rest / vocab add up to less than rest: the cut is above.
+    const double depth = -log2(rest / static_cast<double>(view.vocab)) / w.rate;
+    if (!(depth > 0.0 && depth < 1e30)) return false;
+    per = static_cast<float>((kBand - 1) / depth);
+    if (!(per > 0.0f && per < 1e30f)) return false;
+    for (int i = tid; i < kBins; i += kThreads) digits[i] = 0;
+    __syncthreads();
+    const int stride = max(1, vectors / (32768 / kPer));
+    for (int v = tid * stride; v < vectors; v += kThreads * stride) {
+      float z[kPer];
+      view.logits(v * kPer, z);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const double wz = exp2_neg((static_cast<double>(z[j]) - w.zmax) * w.rate);
+        const unsigned long long f = static_cast<unsigned long long>(__builtin_rint(wz * w.unit));
+        const float x = (zmax - z[j]) * per;
+        // Behind the looked-at bins lies the last one, counted from the bottom for find_from_top.
+        if (f) atomicAdd(&digits[x < kBand - 1 ? static_cast<int>(x) : kBand - 1], f);
+      }
+    }
+    if (tid == 0) s_a = 0, s_b = kBand - 1;
+    __syncthreads();
+    const double mine = tid < kBand ? static_cast<double>(digits[tid]) : 0.0;
+    const double incl = block_inclusive<double>(mine, reinterpret_cast<double*>(waves));
+    if (tid == kThreads - 1) s_u64 = static_cast<unsigned long long>(incl);
+    __syncthreads();
+    // Below bin tid, over the row; its error: each of the small tokens there is seen or not, and
+    // weighs at most what its bin does.
+    const double seen = static_cast<double>(s_u64);
+    const double below = (seen - (incl - mine)) * stride, after = (seen - incl) * stride;
+    const double rest_u = rest * w.unit;
+    const double weight = exp2_neg(-static_cast<double>(tid) / per * w.rate) * w.unit;
+    const double slack = stride == 1 ? 0.0 : 2.5 * sqrt(stride * weight * rest_u) + rest_u / 128.0;
+    // The band: from the last bin above which too little can be cut off, to the first below which
+    // too much would be.
+    if (below > rest_u + slack) atomicMax(&s_a, tid);
+    if (after < rest_u - slack) atomicMin(&s_b, tid);
+    __syncthreads();
+    above = s_a;
+    lim = static_cast<float>(max(s_a, s_b) + 1);
+    if (lim >= kBand) return false;
+  } else {
+    const double depth = -log2(floor_w) / w.rate;
+    if (!(depth < 1e30)) return false;
+    per = depth > 0.0 ? static_cast<float>((kBand - 2) / depth) : static_cast<float>(kBand);
+    above = kBand;
+    lim = static_cast<float>(kBand - 1);  // a bin past the exact border
+  }
+
+  if (!(per > 0.0f && per < 1e30f)) return false;
+
+  int group = 0;
+  while (((num_subs - 1) >> group) + 1 > kMaxSubs) ++group;
+  for (int i = tid; i < kMaxSubs; i += kThreads) sub_sums[i] = 0;
+  if (tid == 0) s_n = 0;
+  __syncthreads();
+  unsigned long long* queue = queues + 128 * wave;
+  int head = 0, tail = 0;  // wave-uniform
+  unsigned long long my_above = 0;
+  auto take = [&](int n) {  // the next n of the queue, one a lane
+    if (lane < n) {
+      const unsigned long long e = queue[(head + lane) & 127];
+      const uint32_t key = static_cast<uint32_t>(e >> 32);
+      const int place = static_cast<int>(static_cast<uint32_t>(e));
+      const double v = w.real(key);
+      const unsigned long long f = static_cast<unsigned long long>(__builtin_rint(v * w.unit));
+      const float x = (zmax - logit_of(key)) * per;
+      if (x < static_cast<float>(above)) {
+        my_above += f;
+        if (v >= floor_w || key == w.top) atomicAdd(&sub_sums[place / kSub >> group], f);
+      } else {
+        const int slot = atomicAdd(&s_n, 1);
+        if (slot < kMaxBand)
+          band[slot] = (e & 0xFFFFFFFF00000000ull) |
+                       (0xFFFFFFFFu - static_cast<uint32_t>(place - view.shift));
+      }
+    }
+    head += n;
+  };
+  constexpr int kAhead = 4;
+  uint4 next[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) next[i] = view.raw((tid + i * kThreads) * kPer);
+  for (int v0 = tid; v0 - tid < vectors; v0 += kAhead * kThreads) {
+    float z[kAhead][kPer];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      RowView<kF32>::unpack(next[i], z[i]);
+      next[i] = view.raw((v0 + (i + kAhead) * kThreads) * kPer);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const bool in = (zmax - z[i][j]) * per < lim;
+        const unsigned long long m = __ballot(in);
+        if (!m) continue;
+        if (in)
+          queue[(tail + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(m >> 32),
+                                                  __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(m), 0))) & 127] =
+              (static_cast<unsigned long long>(key_of(z[i][j])) << 32) |
+              static_cast<uint32_t>((v0 + i * kThreads) * kPer + j);
+        tail += __popcll(m);
+        __builtin_amdgcn_wave_barrier();
+        if (tail - head >= 64) take(64);
+      }
+  }
+  take(tail - head);
+  const unsigned long long above_incl = block_inclusive<unsigned long long>(my_above, waves);
+  if (tid == kThreads - 1) s_u64 = above_incl;
+  __syncthreads();
+  const int listed = s_n;
+  uint32_t cut_key = 0, cut_index = 0xFFFFFFFFu;  // kept: above the key, or it up to that index
+  if (nucleus) {
+    if (listed > kMaxBand) return false;
+    const double left = __builtin_ceil(goal - static_cast<double>(s_u64));
+    if (!(left >= 1.0)) return false;  // the cut lies above the band
+    const unsigned long long target = static_cast<unsigned long long>(left);
+    uint32_t prefix = 0;
+    unsigned long long ahead = 0;
+    for (int level = 0; level < 3; ++level) {
+      const int lo = level == 0 ? 21 : level == 1 ? 10 : 0;
+      const int width = level == 2 ? 10 : 11;
+      for (int b = tid; b < kBins; b += kThreads) digits[b] = 0;
+      __syncthreads();
+      for (int i = tid; i < listed; i += kThreads) {
+        const uint32_t key = static_cast<uint32_t>(band[i] >> 32);
+        if (level > 0 && (key >> (lo + width)) != prefix) continue;
+        atomicAdd(&digits[(key >> lo) & ((1u << width) - 1)], w.fixed(key));
+      }
+      if (tid == 0) found->bin = kBins;
+      __syncthreads();
+      const Found f = find_from_top(digits, target - ahead, waves, found);
+      if (f.bin == kBins) return false;  // the cut lies below the band
+      ahead += f.above;
+      prefix = (prefix << width) | f.bin;
+    }
+    // Of the tokens of that key the lowest indexes, as many as it takes.
+    const unsigned long long each = w.fixed(prefix);
+    const unsigned long long ties = (target - ahead + each - 1) / each;
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    for (int i = tid; i < listed; i += kThreads)
+      if (static_cast<uint32_t>(band[i] >> 32) == prefix) {
+        const int slot = atomicAdd(&s_n, 1);
+        if (slot < kMaxSorted) digits[slot] = band[i];
+      }
+    __syncthreads();
+    const int equal = s_n;
+    __syncthreads();
+    if (equal > kMaxSorted) return false;
+    sort_descending<kThreads>(digits, order, equal);
+    cut_key = prefix;
+    cut_index = 0xFFFFFFFFu - static_cast<uint32_t>(
+        digits[min(static_cast<int>(ties), equal) - 1]);
+    __syncthreads();
+  }
+  for (int i = tid; i < min(listed, kMaxBand); i += kThreads) {
+    const uint32_t key = static_cast<uint32_t>(band[i] >> 32);
+    const uint32_t index = 0xFFFFFFFFu - static_cast<uint32_t>(band[i]);
+    if (key < cut_key || (key == cut_key && index > cut_index)) continue;
+    if (w.real(key) >= floor_w || key == w.top)
+      atomicAdd(&sub_sums[(static_cast<int>(index) + view.shift) / kSub >> group], w.fixed(key));
+  }
+  __syncthreads();
+  // The sub-chunks (of `group` doublings) in which the draw lands; thread t has 4t .. 4t + 3.
+  constexpr int kEach = kMaxSubs / kThreads;
+  unsigned long long sum = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) sum += sub_sums[kEach * tid + j];
+  const unsigned long long incl = block_inclusive<unsigned long long>(sum, waves);
+  if (tid == kThreads - 1) s_u64 = incl;
+  __syncthreads();
+  const unsigned long long all = s_u64;
+  unsigned long long want = static_cast<unsigned long long>(uniform_of(a, row) * static_cast<double>(all));
+  if (want >= all) want = all - 1;
+  __syncthreads();
+  if (incl - sum <= want && want < incl) {
+    unsigned long long before = incl - sum;
+    int at = kEach * tid;
+    while (want >= before + sub_sums[at]) before += sub_sums[at++];
+    s_place = at;
+    s_u64 = want - before;
+  }
+  __syncthreads();
+  if (wave != 0) return true;
+  unsigned long long left = s_u64;
+  for (int place = (s_place << group) * kSub + lane; ; place += 64) {
+    const uint32_t key = view.key(place);
+    const uint32_t index = static_cast<uint32_t>(place - view.shift);
+    unsigned long long v = 0;
+    if (key > cut_key || (key != 0 && key == cut_key && index <= cut_index))
+      if (w.real(key) >= floor_w || key == w.top) v = w.fixed(key);
+    unsigned long long run = v;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const unsigned long long o = __shfl_up(run, d);
+      if (lane >= d) run += o;
+    }
+    const unsigned long long hit = __ballot(run > left);
+    if (hit) {
+      const int l = __ffsll(hit) - 1;
+      if (lane == l) a.tokens[row] = static_cast<int32_t>(index);
+      return true;
+    }
+    left -= __shfl(run, 63);
+    if (place - lane >= view.vocab + view.shift) return true;  // not reached: the sums are the same
+  }
+}
+
+// What the second launch leaves for the third.
+struct RowRest {
+  double total;     // the sum of the row's weights, if it has one
+  uint32_t top;     // its largest key
+  uint32_t is_left;
+};
+
+template <bool kF32>
+__global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a, int shift,
+                                                               const RowRest* __restrict__ rest,
+                                                               int num_subs) {
+  __shared__ unsigned long long bins[kMaxSubs];
+  __shared__ unsigned long long digits[kBins];
+  __shared__ unsigned long long band[kMaxBand];
+  __shared__ unsigned long long waves[kThreads / 64];
+  __shared__ Found found;
+  const int64_t row = blockIdx.x;
+  const RowRest mine = rest[row];
+  if (!mine.is_left) return;  // block-uniform
+  const Asked asked(a, row);
+  const RowView<kF32> view(a, row);
+  const Weights w{mine.top, static_cast<double>(logit_of(mine.top)), asked.rate(),
+                  static_cast<double>(1ull << shift)};
+  if (asked.k == 0 && mine.top != kInfKey &&
+      sample_wide<kF32>(a, row, view, asked, w, mine.total, num_subs, bins, digits, band, waves, &found))
+    return;
+  sample_descent<kF32>(a, shift, row, mine.top, bins, reinterpret_cast<uint32_t*>(digits), waves, &found);
+}
+
+// The first thread by number whose condition holds, or else the last whose `or_else` does.
+__device__ __forceinline__ int first_thread(bool holds, bool or_else, int* first, int* last) {
+  if (threadIdx.x == 0) *first = 0x7FFFFFFF, *last = -1;
+  __syncthreads();
+  if (holds) atomicMin(first, static_cast<int>(threadIdx.x));
+  if (or_else) atomicMax(last, static_cast<int>(threadIdx.x));
+  __syncthreads();
+  const int f = *first, l = *last;
+  __syncthreads();
+  return f != 0x7FFFFFFF ? f : l;
+}
+
+// One workgroup a row.  PER: sub-chunks a thread looks at.
+template <bool kF32, int PER>
+__global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
+    SampleArgs a, const uint32_t* __restrict__ subs, const double* __restrict__ sums,
+    RowRest* __restrict__ rest, int num_subs) {
+  constexpr int kWaves = kPickThreads / 64;
+  constexpr int kPickBins = 2 * kPickThreads;
+  constexpr int kEach = kMaxSorted / kPickThreads;  // entries of a thread
+  __shared__ unsigned long long cand[kMaxSorted];
+  __shared__ unsigned long long other[kMaxSorted];
+  __shared__ uint32_t list[kMaxSorted];
+  __shared__ uint32_t bins[kPickBins];
+  __shared__ unsigned long long waves[kWaves];
+  __shared__ unsigned long long s_counts[2][kWaves];
+  __shared__ int s_num, s_at, s_last;
+  __shared__ uint32_t s_key;
+  __shared__ double s_sum;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x;
+  const Asked asked(a, row);
+  const double u = uniform_of(a, row);
+  const RowView<kF32> view(a, row);
+
+  // Thread t has sub-chunks PER t .. PER t + PER - 1.
+  uint32_t sub[PER];
+  uint32_t top = 0, low = 0xFFFFFFFFu;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int s = PER * tid + j;
+    sub[j] = s < num_subs ? subs[row * num_subs + s] : 0;
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    top = max(top, sub[j]);
+    low = min(low, sub[j] - 1);  // key 0, no logit, passes for the largest
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    top = max(top, static_cast<uint32_t>(__shfl_xor(top, d)));
+    low = min(low, static_cast<uint32_t>(__shfl_xor(low, d)));
+  }
+  if (lane == 0) s_counts[0][wave] = (static_cast<unsigned long long>(low) << 32) | top;
+  for (int i = tid; i < kPickBins; i += kPickThreads) bins[i] = 0;
+  if (tid == 0) s_at = 0x7FFFFFFF;
+  __syncthreads();
+  const unsigned long long both = s_counts[0][lane % kWaves];
+  top = static_cast<uint32_t>(both), low = static_cast<uint32_t>(both >> 32);
+#pragma unroll
+  for (int d = 1; d < kWaves; d *= 2) {
+    top = max(top, static_cast<uint32_t>(__shfl_xor(top, d)));
+    low = min(low, static_cast<uint32_t>(__shfl_xor(low, d)));
+  }
+  low += 1;
+  if (top == 0 || asked.k == 1) {  // block-uniform
+    // The first of the largest logits: the first sub-chunk that has it.
+    int at = 0x7FFFFFFF;
+#pragma unroll
+    for (int j = PER - 1; j >= 0; --j)
+      if (sub[j] == top) at = PER * tid + j;
+    if (top != 0 && at != 0x7FFFFFFF) atomicMin(&s_at, at);
+    __syncthreads();
+    if (wave == 0) {
+      const unsigned long long m = top ? __ballot(view.key(s_at * kSub + lane) == top) : 0;
+      if (lane == 0) {
+        a.tokens[row] = top ? s_at * kSub + __ffsll(m) - 1 - view.shift : -1;
+        rest[row].is_left = 0;
+      }
+    }
+    return;
+  }
+  const Weights w{top, static_cast<double>(logit_of(top)), asked.rate(), 1.0};
+  double mass[PER];
+  double my_mass = 0.0, mass_incl = 0.0, total = 0.0;
+  if (asked.needs_sums()) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int s = PER * tid + j;
+      mass[j] = sub[j] ? sums[row * num_subs + s] : 0.0;
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      mass[j] = sub[j] ? mass[j] * w.real(sub[j]) : 0.0;
+      my_mass += mass[j];
+    }
+    mass_incl = block_inclusive<double>(my_mass, reinterpret_cast<double*>(waves));
+    if (tid == kPickThreads - 1) s_sum = mass_incl;
+    __syncthreads();
+    total = s_sum;
+    __syncthreads();
+  }
+
+  if (asked.k == 0 && asked.top_p == 1.0f && asked.min_p == 0.0f) {
+    // Sums of different threads are added in different orders, so that by rounding none may pass
+    // the goal: then the last with any weight has it.
+    const double goal = u * total;
+    if (tid == first_thread(my_mass > 0.0 && mass_incl > goal, my_mass > 0.0, &s_at, &s_last)) {
+      int at = -1;
+      double before = mass_incl - my_mass, at_before = 0.0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        if (mass[j] > 0.0 && (at < 0 || goal >= before)) at = PER * tid + j, at_before = before;
+        before += mass[j];
+      }
+      s_num = at;
+      s_sum = goal - at_before;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    const int place = s_num * kSub + lane;
+    const uint32_t key = view.key(place);
+    const double v = key ? w.real(key) : 0.0;
+    double sum = v;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const double o = __shfl_up(sum, d);
+      if (lane >= d) sum += o;
+    }
+    const unsigned long long hit = __ballot(v > 0.0 && sum > s_sum);
+    const unsigned long long any = __ballot(v > 0.0);
+    const int l = hit ? __ffsll(hit) - 1 : 63 - __clzll(any);
+    if (lane == 0) {
+      a.tokens[row] = s_num * kSub + l - view.shift;
+      rest[row].is_left = 0;
+    }
+    return;
+  }
+
+  auto leave = [&]() {
+    if (tid == 0) rest[row] = {total, top, 1};
+  };
+  if (asked.k > kMaxK) return leave();
+  const float zmax = logit_of(top), zlow = logit_of(low);
+  const double floor_w = static_cast<double>(asked.min_p);
+  const bool by_floor = asked.k == 0 && asked.top_p == 1.0f;
+
+  // The sub-chunks' largest in bins of equal width, from the top.
+  const float per = static_cast<float>(kPickBins - 1) / (zmax - zlow);
+  const bool binned = per > 0.0f && per < 1e30f;
+  auto bin_of = [&](uint32_t key) {
+    return binned ? min(static_cast<int>((zmax - logit_of(key)) * per), kPickBins - 1) : 0;
+  };
+  if (!by_floor) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (sub[j]) atomicAdd(&bins[bin_of(sub[j])], 1u);
+    __syncthreads();
+  }
+
+  int want = asked.k > 0 ? static_cast<int>(asked.k) : 128;
+  int n = 0, kept = 0;
+  for (;;) {
+    // A key t0 with `want` sub-chunks or more at or above it, and not many more; 1 (every token that
+    // can be drawn) if there are not as many.
+    uint32_t t0 = 1;
+    if (by_floor) {
+      // Weights below min_p are below this by more than rounding.
+      const double depth = -log2(floor_w) / w.rate;
+      const float z = static_cast<float>(w.zmax - depth - 1e-5 * (__builtin_fabs(w.zmax) + depth));
+      t0 = min(max(key_of(z), 1u), top);
+    } else if (num_subs * kSub > kMaxSorted) {
+      const int b0 = static_cast<int>(bins[2 * tid]), b1 = static_cast<int>(bins[2 * tid + 1]);
+      const int incl = block_inclusive<int>(b0 + b1, reinterpret_cast<int*>(waves));
+      if (tid == 0) s_at = -1, s_key = 0xFFFFFFFFu;
+      __syncthreads();
+      if (incl - b0 - b1 < want && want <= incl) {
+        const bool first = incl - b1 >= want;
+        s_at = 2 * tid + !first;
+        s_num = first ? incl - b1 : incl;
+      }
+      __syncthreads();
+      const int bin = s_at, count = s_num;
+      if (bin >= 0) {
+        if (count <= 2 * want + 64) {
+          uint32_t least = 0xFFFFFFFFu;
+#pragma unroll
+          for (int j = 0; j < PER; ++j)
+            if (sub[j] && bin_of(sub[j]) <= bin) least = min(least, sub[j]);
+#pragma unroll
+          for (int d = 1; d < 64; d *= 2) least = min(least, static_cast<uint32_t>(__shfl_xor(least, d)));
+          if (lane == 0) atomicMin(&s_key, least);
+          __syncthreads();
+          t0 = s_key;
+        } else {
+          // Too many of one bin (a few logits far below or above the rest, or equal ones): bisection.
+          uint32_t lo = 1, hi = top;  // at least want at lo
+          int round = 0;
+          const int enough = want + want / 4 + 16;
+          while (lo < hi) {
+            const uint32_t span = hi - lo;  // thresholds in (lo, hi]
+            const uint32_t t[3] = {lo + max(span / 4, 1u), lo + max(span / 2, 1u), lo + span - span / 4};
+            unsigned long long c = 0;  // three counts of 21 bits
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+#pragma unroll
+              for (int j = 0; j < PER; ++j)
+                c += static_cast<unsigned long long>(__popcll(__ballot(sub[j] >= t[i]))) << (21 * i);
+            if (lane == 0) s_counts[round & 1][wave] = c;
+            __syncthreads();
+            c = s_counts[round & 1][lane % kWaves];
+#pragma unroll
+            for (int d = 1; d < kWaves; d *= 2) c += __shfl_xor(c, d);
+            ++round;
+            int at = -1, n_at = 0;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+              const int ci = static_cast<int>(c >> (21 * i)) & 0x1FFFFF;
+              if (ci >= want) at = i, n_at = ci;
+            }
+            if (at < 2) hi = t[at + 1] - 1;
+            if (at >= 0) lo = t[at];
+            if (at >= 0 && n_at <= enough) break;
+          }
+          t0 = lo;
+        }
+      }
+    }
+    // Sub-chunks with candidates, then the candidates: (key, lowest index first) as one number.
+    __syncthreads();
+    if (tid == 0) s_num = 0, s_last = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const bool in = sub[j] >= t0;
+      const unsigned long long m = __ballot(in);
+      if (!m) continue;
+      int base = 0;
+      if (lane == 0) base = atomicAdd(&s_num, __popcll(m));
+      base = __shfl(base, 0);
+      const int at = base + __popcll(m & ((1ull << lane) - 1));
+      if (in && at < kMaxSorted) list[at] = PER * tid + j;
+    }
+    __syncthreads();
+    const int lists = s_num;
+    bool fits = lists <= kMaxSorted;
+    if (fits) {
+      constexpr int kAhead = 8;
+      for (int i0 = wave; i0 < lists; i0 += kAhead * kWaves) {
+        uint32_t key[kAhead];
+        int at[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int l = i0 + i * kWaves;
+          at[i] = l < lists ? static_cast<int>(list[l]) * kSub + lane : -1;
+          key[i] = at[i] >= 0 ? view.key(at[i]) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const bool in = key[i] >= t0;
+          const unsigned long long m = __ballot(in);
+          if (!m) continue;
+          int base = 0;
+          if (lane == 0) base = atomicAdd(&s_last, __popcll(m));
+          base = __shfl(base, 0);
+          const int slot = base + __popcll(m & ((1ull << lane) - 1));
+          if (in && slot < kMaxSorted)
+            cand[slot] = (static_cast<unsigned long long>(key[i]) << 32) |
+                         (0xFFFFFFFFu - static_cast<uint32_t>(at[i] - view.shift));
+        }
+      }
+      __syncthreads();
+      n = s_last;
+      fits = n <= kMaxSorted;
+    }
+    if (!fits) return leave();  // block-uniform
+    sort_descending<kPickThreads>(cand, other, n);
+    const int first = asked.k > 0 ? min(n, static_cast<int>(asked.k)) : n;
+    // Thread t has entries kEach t .. kEach t + kEach - 1.
+    double v[kEach], mine = 0.0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int i = kEach * tid + j;
+      v[j] = i < first ? w.real(static_cast<uint32_t>(cand[i] >> 32)) : 0.0;
+      mine += v[j];
+    }
+    const double incl = block_inclusive<double>(mine, reinterpret_cast<double*>(waves));
+    if (tid == kPickThreads - 1) s_sum = incl;
+    __syncthreads();
+    const double listed = s_sum;
+    const double goal = static_cast<double>(asked.top_p) * (asked.k > 0 ? listed : total);
+    if (asked.k == 0 && asked.top_p < 1.0f && t0 > 1 && listed < goal) {
+      // The cut lies below t0.
+      if (want == kMaxK) return leave();
+      want = kMaxK;
+      __syncthreads();
+      continue;
+    }
+    double before = incl - mine;
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int i = kEach * tid + j;
+      const bool in_p = asked.top_p == 1.0f || i == 0 || before < goal;
+      c += i < first && in_p && (v[j] >= floor_w || static_cast<uint32_t>(cand[i] >> 32) == top);
+      before += v[j];
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) c += __shfl_xor(c, d);
+    if (lane == 0) s_counts[0][wave] = static_cast<unsigned long long>(c);
+    __syncthreads();
+    kept = static_cast<int>(s_counts[0][lane % kWaves]);
+#pragma unroll
+    for (int d = 1; d < kWaves; d *= 2) kept += __shfl_xor(kept, d);
+    break;
+  }
+  __syncthreads();
+  // The kept ones, a prefix, in order of their indexes: (index from the end, place) descending.
+  // The keys move to list[], which the sub-chunks no longer need.
+  for (int i = tid; i < kept; i += kPickThreads) {
+    const unsigned long long e = cand[i];
+    list[i] = static_cast<uint32_t>(e >> 32);
+    other[i] = (e << 32) | static_cast<uint32_t>(i);
+  }
+  __syncthreads();
+  sort_descending<kPickThreads>(other, cand, kept);
+  double v[kEach], mine = 0.0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = kEach * tid + j;
+    v[j] = i < kept ? w.real(list[static_cast<uint32_t>(other[i])]) : 0.0;
+    mine += v[j];
+  }
+  const double incl = block_inclusive<double>(mine, reinterpret_cast<double*>(waves));
+  if (tid == kPickThreads - 1) s_sum = incl;
+  __syncthreads();
+  const double goal = u * s_sum;
+  if (tid == first_thread(mine > 0.0 && incl > goal, mine > 0.0, &s_at, &s_last)) {
+    int at = -1;
+    double before = incl - mine;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      if (v[j] > 0.0 && (at < 0 || goal >= before)) at = kEach * tid + j;
+      before += v[j];
+    }
+    a.tokens[row] = static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(other[at] >> 32));
+    rest[row].is_left = 0;
+  }
+}
+
 // Bits of the integers that stand for weights of at most 1: sums of a row stay below 2^63.
 int weight_shift(int64_t vocab) {
   int bits = 0;
@@ -308,19 +1122,45 @@ int weight_shift(int64_t vocab) {
   return bits < 10 ? 52 : 62 - bits;
 }
 
+int64_t sub_chunks(int64_t vocab) { return (vocab + 7 + kSub - 1) / kSub; }
+
+template <bool kF32>
+hipError_t launch(const SampleArgs& a, hipStream_t stream) {
+  const int subs = static_cast<int>(sub_chunks(a.vocab));
+  double* sums = static_cast<double*>(a.workspace);
+  RowRest* rest = reinterpret_cast<RowRest*>(sums + a.rows * subs);
+  uint32_t* tops = reinterpret_cast<uint32_t*>(rest + a.rows);
+  constexpr int kChunk = kScanThreads * kScanVectors * RowView<kF32>::kPer;
+  const int chunks = (subs * kSub + kChunk - 1) / kChunk;
+  hipLaunchKernelGGL(sample_scan_kernel<kF32>, dim3(static_cast<unsigned>(a.rows * chunks)),
+                     dim3(kScanThreads), 0, stream, a, tops, sums, subs, chunks);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  const dim3 grid(static_cast<unsigned>(a.rows));
+  if (subs <= kPickThreads)
+    hipLaunchKernelGGL((sample_pick_kernel<kF32, 1>), grid, dim3(kPickThreads), 0, stream, a, tops,
+                       sums, rest, subs);
+  else if (subs <= 9 * kPickThreads)
+    hipLaunchKernelGGL((sample_pick_kernel<kF32, 9>), grid, dim3(kPickThreads), 0, stream, a, tops,
+                       sums, rest, subs);
+  else
+    hipLaunchKernelGGL((sample_pick_kernel<kF32, 33>), grid, dim3(kPickThreads), 0, stream, a, tops,
+                       sums, rest, subs);
+  err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  hipLaunchKernelGGL(sample_rest_kernel<kF32>, grid, dim3(kThreads), 0, stream, a,
+                     weight_shift(a.vocab), rest, subs);
+  return hipGetLastError();
+}
+
 }  // namespace
 
-int64_t sample_workspace_bytes(int64_t, int64_t) { return 0; }
+int64_t sample_workspace_bytes(int64_t rows, int64_t vocab) {
+  return (rows * (sub_chunks(vocab) * 12 + static_cast<int64_t>(sizeof(RowRest))) + 15) / 16 * 16;
+}
 
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
-  const int shift = weight_shift(a.vocab);
-  if (a.f32)
-    hipLaunchKernelGGL(sample_row_kernel<true>, dim3(static_cast<unsigned>(a.rows)),
-                       dim3(kThreads), 0, stream, a, shift);
-  else
-    hipLaunchKernelGGL(sample_row_kernel<false>, dim3(static_cast<unsigned>(a.rows)),
-                       dim3(kThreads), 0, stream, a, shift);
-  return hipGetLastError();
+  return a.f32 ? launch<true>(a, stream) : launch<false>(a, stream);
 }
 
 }  // namespace ifr
