@@ -174,6 +174,13 @@ struct RowView {
     const int i = place - shift;
     return i >= 0 && i < vocab ? key_of(load_logit<kF32>(z, i)) : 0;
   }
+  // Vectors [first_full, end_full) lie within the row.
+  __device__ __forceinline__ int first_full() const { return shift ? 1 : 0; }
+  __device__ __forceinline__ int end_full() const { return (shift + vocab) / kPer; }
+  __device__ __forceinline__ uint4 full(int vector) const {
+    return *reinterpret_cast<const uint4*>(static_cast<const char*>(z) +
+                                           (static_cast<int64_t>(vector) * kPer - shift) * (kF32 ? 4 : 2));
+  }
   // A vector's bits; those of -inf behind the row's ends.
   __device__ __forceinline__ uint4 raw(int place) const {
     const int i = place - shift;
@@ -229,9 +236,16 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleArgs a,
   const int chunk = static_cast<int>(blockIdx.x - row * chunks);
   const RowView<kF32> view(a, row);
   float z[kScanVectors][kPer];
+  const int v0 = chunk * kScanVectors * kScanThreads;
+  if (v0 >= view.first_full() && v0 + kScanVectors * kScanThreads <= view.end_full()) {
 #pragma unroll
-  for (int v = 0; v < kScanVectors; ++v)
-    view.logits(((chunk * kScanVectors + v) * kScanThreads + static_cast<int>(threadIdx.x)) * kPer, z[v]);
+    for (int v = 0; v < kScanVectors; ++v)
+      RowView<kF32>::unpack(view.full(v0 + v * kScanThreads + static_cast<int>(threadIdx.x)), z[v]);
+  } else {
+#pragma unroll
+    for (int v = 0; v < kScanVectors; ++v)
+      view.logits((v0 + v * kScanThreads + static_cast<int>(threadIdx.x)) * kPer, z[v]);
+  }
   const Asked asked(a, row);
   const bool with_sums = asked.needs_sums();
   const double rate = asked.rate();
@@ -272,7 +286,7 @@ __device__ __forceinline__ double uniform_of(const SampleArgs& a, int64_t row) {
 
 // The row by its keys' bits.
 template <bool kF32>
-__device__ __noinline__ void sample_descent(const SampleArgs& a, int shift, int64_t row,
+__device__ __forceinline__ void sample_descent(const SampleArgs& a, int shift, int64_t row,
                                             uint32_t top, unsigned long long* bins,
                                             uint32_t* tie_counts, unsigned long long* waves,
                                             Found* found_at) {
@@ -456,7 +470,58 @@ __device__ __noinline__ void sample_descent(const SampleArgs& a, int shift, int6
 constexpr int kMaxK = 1024;     // candidates that are sought
 constexpr int kMaxSorted = 2048;  // and at most taken
 
-// Descending, in place; slots from n on hold 0 afterwards up to the next power of two.
+// Bitonic sort, descending, of kT * E entries: entry 64 E wave + 64 e + lane is in register e of its
+// lane, so that only distances of 64 E and more pass through LDS.
+template <int kT, int E>
+__device__ __forceinline__ void sort_registers(unsigned long long* v, int n) {
+  const int tid = threadIdx.x, lane = tid & 63, base = (tid >> 6) * 64 * E;
+  unsigned long long x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = base + 64 * e + lane;
+    x[e] = i < n ? v[i] : 0;
+  }
+  auto order = [](unsigned long long mine, unsigned long long theirs, bool larger) {
+    return (mine < theirs) == larger ? theirs : mine;
+  };
+  for (int width = 2; width <= kT * E; width *= 2) {
+    for (int d = width / 2; d >= 64 * E; d /= 2) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[base + 64 * e + lane] = x[e];
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int i = base + 64 * e + lane;
+        x[e] = order(x[e], v[i ^ d], ((i & d) == 0) == ((i & width) == 0));
+      }
+    }
+#pragma unroll
+    for (int r = E / 2; r > 0; r /= 2) {
+      if (width < 128 * r) continue;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (e & r) continue;
+        const bool down = ((base + 64 * e + lane) & width) == 0;
+        const unsigned long long lo = x[e], hi = x[e + r];
+        if ((lo < hi) == down) x[e] = hi, x[e + r] = lo;
+      }
+    }
+    for (int d = min(width / 2, 32); d > 0; d /= 2) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int i = base + 64 * e + lane;
+        x[e] = order(x[e], __shfl_xor(x[e], d), ((i & d) == 0) == ((i & width) == 0));
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[base + 64 * e + lane] = x[e];
+  __syncthreads();
+}
+
+// Descending, in place (n up to kMaxSorted, of which v has room for all).
 template <int kT>
 __device__ __forceinline__ void sort_descending(unsigned long long* v, unsigned long long* tmp, int n) {
   const int tid = threadIdx.x;
@@ -470,22 +535,12 @@ __device__ __forceinline__ void sort_descending(unsigned long long* v, unsigned 
     __syncthreads();
     if (tid < n) v[tid] = tmp[tid];
     __syncthreads();
-    return;
-  }
-  int size = 512;
-  while (size < n) size *= 2;
-  for (int i = n + tid; i < size; i += kT) v[i] = 0;
-  __syncthreads();
-  for (int width = 2; width <= size; width *= 2) {
-    for (int d = width / 2; d > 0; d /= 2) {
-      for (int i = tid; i < size / 2; i += kT) {
-        const int lo = 2 * i - (i & (d - 1)), hi = lo + d;
-        const unsigned long long x = v[lo], y = v[hi];
-        const bool up = (lo & width) != 0;  // ascending runs
-        if ((x < y) != up) v[lo] = y, v[hi] = x;
-      }
-      __syncthreads();
-    }
+  } else if (n <= kT) {
+    sort_registers<kT, 1>(v, n);
+  } else if (n <= 2 * kT) {
+    sort_registers<kT, 2>(v, n);
+  } else {
+    sort_registers<kT, kMaxSorted / kT>(v, n);
   }
 }
 
@@ -503,7 +558,7 @@ constexpr uint32_t kInfKey = 0xFF800000u;  // of +inf
 // A CU takes 2 us for each instruction on all of 2^18 logits, so the pass does little for each:
 // those at or above the band are moved together, 64 at a time, before their weights are taken.
 template <bool kF32>
-__device__ __noinline__ bool sample_wide(const SampleArgs& a, int64_t row, const RowView<kF32>& view,
+__device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, const RowView<kF32>& view,
                                          const Asked& asked, const Weights& w, double total,
                                          int num_subs, unsigned long long* sub_sums,
                                          unsigned long long* digits, unsigned long long* band,
@@ -605,33 +660,42 @@ __device__ __noinline__ bool sample_wide(const SampleArgs& a, int64_t row, const
     }
     head += n;
   };
-  constexpr int kAhead = 4;
-  uint4 next[kAhead];
+  auto push = [&](float z, int place) {
+    const bool in = (zmax - z) * per < lim;
+    const unsigned long long m = __ballot(in);
+    if (!m) return;
+    if (in)
+      queue[(tail + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(m >> 32),
+                                              __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(m), 0))) & 127] =
+          (static_cast<unsigned long long>(key_of(z)) << 32) | static_cast<uint32_t>(place);
+    tail += __popcll(m);
+    __builtin_amdgcn_wave_barrier();
+    if (tail - head >= 64) take(64);
+  };
+  constexpr int kAhead = kF32 ? 8 : 4;
+  const int v_first = view.first_full(), v_end = view.end_full();
+  if (v_first < v_end) {
+    uint4 next[kAhead];
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) next[i] = view.raw((tid + i * kThreads) * kPer);
-  for (int v0 = tid; v0 - tid < vectors; v0 += kAhead * kThreads) {
-    float z[kAhead][kPer];
+    for (int i = 0; i < kAhead; ++i) next[i] = view.full(min(v_first + tid + i * kThreads, v_end - 1));
+    for (int v0 = v_first + tid; v0 - tid < v_end; v0 += kAhead * kThreads) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      RowView<kF32>::unpack(next[i], z[i]);
-      next[i] = view.raw((v0 + (i + kAhead) * kThreads) * kPer);
-    }
+      for (int i = 0; i < kAhead; ++i) {
+        const int v = v0 + i * kThreads;
+        if (v - tid >= v_end) break;
+        float z[kPer];
+        RowView<kF32>::unpack(next[i], z);
+        next[i] = view.full(min(v + kAhead * kThreads, v_end - 1));
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const bool in = (zmax - z[i][j]) * per < lim;
-        const unsigned long long m = __ballot(in);
-        if (!m) continue;
-        if (in)
-          queue[(tail + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(m >> 32),
-                                                  __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(m), 0))) & 127] =
-              (static_cast<unsigned long long>(key_of(z[i][j])) << 32) |
-              static_cast<uint32_t>((v0 + i * kThreads) * kPer + j);
-        tail += __popcll(m);
-        __builtin_amdgcn_wave_barrier();
-        if (tail - head >= 64) take(64);
+        for (int j = 0; j < kPer; ++j) push(v < v_end ? z[j] : -__builtin_inff(), v * kPer + j);
       }
+    }
+  }
+  if (wave == 0) {  // the ends: less than two vectors
+    const int place = lane < kPer ? lane : max(v_end, v_first) * kPer + lane - kPer;
+    const bool end = lane < kPer ? v_first > 0 : lane < 2 * kPer;
+    const uint32_t key = end ? view.key(place) : 0;
+    push(key ? logit_of(key) : -__builtin_inff(), place);
   }
   take(tail - head);
   const unsigned long long above_incl = block_inclusive<unsigned long long>(my_above, waves);
@@ -1012,28 +1076,37 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
     const int lists = s_num;
     bool fits = lists <= kMaxSorted;
     if (fits) {
+      // A load of 16 bytes a lane takes kGroup sub-chunks.
+      constexpr int kPer = RowView<kF32>::kPer, kLanes = kSub / kPer, kGroup = 64 / kLanes;
       constexpr int kAhead = 8;
-      for (int i0 = wave; i0 < lists; i0 += kAhead * kWaves) {
-        uint32_t key[kAhead];
+      for (int i0 = wave * kGroup; i0 < lists; i0 += kAhead * kWaves * kGroup) {
+        uint4 raw[kAhead];
         int at[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-          const int l = i0 + i * kWaves;
-          at[i] = l < lists ? static_cast<int>(list[l]) * kSub + lane : -1;
-          key[i] = at[i] >= 0 ? view.key(at[i]) : 0;
+          const int l = i0 + i * kWaves * kGroup + lane / kLanes;
+          at[i] = l < lists ? static_cast<int>(list[l]) * kSub + lane % kLanes * kPer : -kPer - 16;
+          raw[i] = view.raw(at[i]);
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-          const bool in = key[i] >= t0;
-          const unsigned long long m = __ballot(in);
-          if (!m) continue;
-          int base = 0;
-          if (lane == 0) base = atomicAdd(&s_last, __popcll(m));
-          base = __shfl(base, 0);
-          const int slot = base + __popcll(m & ((1ull << lane) - 1));
-          if (in && slot < kMaxSorted)
-            cand[slot] = (static_cast<unsigned long long>(key[i]) << 32) |
-                         (0xFFFFFFFFu - static_cast<uint32_t>(at[i] - view.shift));
+          if (i0 + i * kWaves * kGroup >= lists) break;
+          float z[kPer];
+          RowView<kF32>::unpack(raw[i], z);
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            const uint32_t key = key_of(z[j]);
+            const bool in = key >= t0;
+            const unsigned long long m = __ballot(in);
+            if (!m) continue;
+            int base = 0;
+            if (lane == 0) base = atomicAdd(&s_last, __popcll(m));
+            base = __shfl(base, 0);
+            const int slot = base + __popcll(m & ((1ull << lane) - 1));
+            if (in && slot < kMaxSorted)
+              cand[slot] = (static_cast<unsigned long long>(key) << 32) |
+                           (0xFFFFFFFFu - static_cast<uint32_t>(at[i] + j - view.shift));
+          }
         }
       }
       __syncthreads();
