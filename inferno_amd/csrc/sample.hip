@@ -21,6 +21,8 @@
 // The third, with a larger workgroup a row, takes the rows that are left: a cut among very many
 // tokens in one pass (sample_wide), a larger top-k or very many equal logits by descending
 // through the keys, 11, 11 and 10 bits at a time, in histograms of counts or weights of the row.
+#include <type_traits>
+
 #include "common.hpp"
 #include "step.hpp"
 
@@ -82,19 +84,42 @@ struct Weights {
     if (key == top) return 1.0;
     return exp2_neg((static_cast<double>(logit_of(key)) - zmax) * rate);  // inf * 0: NaN, so 0
   }
-  __device__ __forceinline__ uint64_t fixed(uint32_t key) const {
-    return static_cast<uint64_t>(__builtin_rint(real(key) * unit));
+  __device__ __forceinline__ unsigned long long fixed(uint32_t key) const { return units(real(key)); }
+  // weight * unit, at most 2^51, to the nearest integer: the low bits of its sum with 2^52.
+  __device__ __forceinline__ unsigned long long units(double weight) const {
+    return __builtin_bit_cast(unsigned long long, weight * unit + 0x1p52) & 0xFFFFFFFFFFFFFull;
   }
 };
 
+// A value of the lane that a DPP control names, 0 (or the lane's own nothing) where there is none.
+template <int kCtrl, int kRows, typename T>
+__device__ __forceinline__ T dpp_or_zero(T v) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl,
+                                                             kRows, 0xF, true));
+  } else {
+    const uint2 u = __builtin_bit_cast(uint2, v);
+    uint2 r;
+    r.x = __builtin_amdgcn_update_dpp(0, static_cast<int>(u.x), kCtrl, kRows, 0xF, true);
+    r.y = __builtin_amdgcn_update_dpp(0, static_cast<int>(u.y), kCtrl, kRows, 0xF, true);
+    return __builtin_bit_cast(T, r);
+  }
+}
+// Sums over the lanes up to each: within rows of 16, then the rows before.
+template <typename T>
+__device__ __forceinline__ T wave_inclusive(T v) {
+  v += dpp_or_zero<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+  v += dpp_or_zero<0x112, 0xF>(v);
+  v += dpp_or_zero<0x114, 0xF>(v);
+  v += dpp_or_zero<0x118, 0xF>(v);
+  v += dpp_or_zero<0x142, 0xA>(v);  // lane 15 of a row to the next, rows 1 and 3
+  v += dpp_or_zero<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
+  return v;
+}
 template <typename T>
 __device__ __forceinline__ T block_inclusive(T v, T* waves) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const T o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
+  v = wave_inclusive(v);
   if (lane == 63) waves[wave] = v;
   __syncthreads();
   T before = 0;
@@ -206,8 +231,7 @@ struct RowView {
     }
     return make_uint4(b[0], b[1], b[2], b[3]);
   }
-  // Its logits; -inf in the place of NaN.
-  static __device__ __forceinline__ void unpack(uint4 u, float (&v)[kPer]) {
+  static __device__ __forceinline__ void split(uint4 u, float (&v)[kPer]) {
     if constexpr (kF32) {
       v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y);
       v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
@@ -215,6 +239,10 @@ struct RowView {
       v[0] = bf16_lo(u.x), v[1] = bf16_hi(u.x), v[2] = bf16_lo(u.y), v[3] = bf16_hi(u.y);
       v[4] = bf16_lo(u.z), v[5] = bf16_hi(u.z), v[6] = bf16_lo(u.w), v[7] = bf16_hi(u.w);
     }
+  }
+  // Its logits; -inf in the place of NaN.
+  static __device__ __forceinline__ void unpack(uint4 u, float (&v)[kPer]) {
+    split(u, v);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) v[j] = __builtin_fmaxf(v[j], -__builtin_inff());
   }
@@ -374,7 +402,7 @@ __device__ __forceinline__ void sample_descent(const SampleArgs& a, int shift, i
   auto kept = [&](uint32_t key) -> unsigned long long {
     if (key == 0) return 0;
     const double v = w.real(key);
-    return v >= floor_w || key == top ? static_cast<unsigned long long>(__builtin_rint(v * w.unit)) : 0;
+    return v >= floor_w || key == top ? w.units(v) : 0;
   };
   const unsigned long long tie = kept(cut.key);
   for (int s = tid; s < kMaxSubs; s += kThreads)
@@ -470,6 +498,28 @@ __device__ __forceinline__ void sample_descent(const SampleArgs& a, int shift, i
 constexpr int kMaxK = 1024;     // candidates that are sought
 constexpr int kMaxSorted = 2048;  // and at most taken
 
+// The value of lane ^ D.
+template <int D>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  if constexpr (D == 1) return dpp_i32<kDppXor1>(v);
+  if constexpr (D == 2) return dpp_i32<kDppXor2>(v);
+  if constexpr (D == 4) return dpp_i32<kDppQuadReverse>(dpp_i32<kDppHalfMirror>(v));
+  if constexpr (D == 8) return dpp_i32<kDppRowRor8>(v);
+  if constexpr (D == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  }
+  if constexpr (D == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+  }
+}
+template <int D>
+__device__ __forceinline__ unsigned long long lane_xor64(unsigned long long v) {
+  return (static_cast<unsigned long long>(lane_xor<D>(static_cast<uint32_t>(v >> 32))) << 32) |
+         lane_xor<D>(static_cast<uint32_t>(v));
+}
+
 // Bitonic sort, descending, of kT * E entries: entry 64 E wave + 64 e + lane is in register e of its
 // lane, so that only distances of 64 E and more pass through LDS.
 template <int kT, int E>
@@ -507,13 +557,21 @@ __device__ __forceinline__ void sort_registers(unsigned long long* v, int n) {
         if ((lo < hi) == down) x[e] = hi, x[e + r] = lo;
       }
     }
-    for (int d = min(width / 2, 32); d > 0; d /= 2) {
+    auto step = [&](auto distance) {
+      constexpr int kD = decltype(distance)::value;
+      if (width < 2 * kD) return;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int i = base + 64 * e + lane;
-        x[e] = order(x[e], __shfl_xor(x[e], d), ((i & d) == 0) == ((i & width) == 0));
+        x[e] = order(x[e], lane_xor64<kD>(x[e]), ((i & kD) == 0) == ((i & width) == 0));
       }
-    }
+    };
+    step(std::integral_constant<int, 32>{});
+    step(std::integral_constant<int, 16>{});
+    step(std::integral_constant<int, 8>{});
+    step(std::integral_constant<int, 4>{});
+    step(std::integral_constant<int, 2>{});
+    step(std::integral_constant<int, 1>{});
   }
   __syncthreads();
 #pragma unroll
@@ -574,8 +632,8 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
   const float zmax = logit_of(w.top);
   const bool nucleus = asked.top_p < 1.0f;
   const double floor_w = static_cast<double>(asked.min_p);
-  // Bins of (zmax - z) * per: `lim` is the first that is not looked at, `above` the first of the band.
-  float per, lim;
+  // Bins of (zmax - z) * per, of which `above` is the first of the band; logits from z_from on are looked at.
+  float per, z_from;
   int above;
   double goal = 0.0;  // in units
   if (nucleus) {
@@ -589,18 +647,23 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
     for (int i = tid; i < kBins; i += kThreads) digits[i] = 0;
     __syncthreads();
     const int stride = max(1, vectors / (32768 / kPer));
+    unsigned long long tail_sum = 0;  // of the last bin
     for (int v = tid * stride; v < vectors; v += kThreads * stride) {
       float z[kPer];
       view.logits(v * kPer, z);
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         const double wz = exp2_neg((static_cast<double>(z[j]) - w.zmax) * w.rate);
-        const unsigned long long f = static_cast<unsigned long long>(__builtin_rint(wz * w.unit));
+        const unsigned long long f = w.units(wz);
         const float x = (zmax - z[j]) * per;
-        // Behind the looked-at bins lies the last one, counted from the bottom for find_from_top.
-        if (f) atomicAdd(&digits[x < kBand - 1 ? static_cast<int>(x) : kBand - 1], f);
+        if (x < kBand - 1)
+          atomicAdd(&digits[static_cast<int>(x)], f);
+        else
+          tail_sum += f;  // what lies below the looked-at bins
       }
     }
+    tail_sum = wave_inclusive(tail_sum);
+    if (lane == 63) atomicAdd(&digits[kBand - 1], tail_sum);
     if (tid == 0) s_a = 0, s_b = kBand - 1;
     __syncthreads();
     const double mine = tid < kBand ? static_cast<double>(digits[tid]) : 0.0;
@@ -620,14 +683,15 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
     if (after < rest_u - slack) atomicMin(&s_b, tid);
     __syncthreads();
     above = s_a;
-    lim = static_cast<float>(max(s_a, s_b) + 1);
-    if (lim >= kBand) return false;
+    const int end = max(s_a, s_b) + 1;
+    if (end >= kBand) return false;
+    z_from = zmax - static_cast<float>(end) / per;
   } else {
     const double depth = -log2(floor_w) / w.rate;
     if (!(depth < 1e30)) return false;
     per = depth > 0.0 ? static_cast<float>((kBand - 2) / depth) : static_cast<float>(kBand);
     above = kBand;
-    lim = static_cast<float>(kBand - 1);  // a bin past the exact border
+    z_from = zmax - static_cast<float>(kBand - 1) / per;  // a bin past the exact border
   }
 
   if (!(per > 0.0f && per < 1e30f)) return false;
@@ -643,10 +707,10 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
   auto take = [&](int n) {  // the next n of the queue, one a lane
     if (lane < n) {
       const unsigned long long e = queue[(head + lane) & 127];
-      const uint32_t key = static_cast<uint32_t>(e >> 32);
+      const uint32_t key = key_of(__uint_as_float(static_cast<uint32_t>(e >> 32)));
       const int place = static_cast<int>(static_cast<uint32_t>(e));
       const double v = w.real(key);
-      const unsigned long long f = static_cast<unsigned long long>(__builtin_rint(v * w.unit));
+      const unsigned long long f = w.units(v);
       const float x = (zmax - logit_of(key)) * per;
       if (x < static_cast<float>(above)) {
         my_above += f;
@@ -654,43 +718,49 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
       } else {
         const int slot = atomicAdd(&s_n, 1);
         if (slot < kMaxBand)
-          band[slot] = (e & 0xFFFFFFFF00000000ull) |
+          band[slot] = (static_cast<unsigned long long>(key) << 32) |
                        (0xFFFFFFFFu - static_cast<uint32_t>(place - view.shift));
       }
     }
     head += n;
   };
   auto push = [&](float z, int place) {
-    const bool in = (zmax - z) * per < lim;
+    const bool in = z >= z_from;
     const unsigned long long m = __ballot(in);
     if (!m) return;
     if (in)
-      queue[(tail + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(m >> 32),
-                                              __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(m), 0))) & 127] =
-          (static_cast<unsigned long long>(key_of(z)) << 32) | static_cast<uint32_t>(place);
+      queue[__builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(m >> 32),
+                                      __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(m), tail)) & 127] =
+          (static_cast<unsigned long long>(__float_as_uint(z)) << 32) | static_cast<uint32_t>(place);
     tail += __popcll(m);
     __builtin_amdgcn_wave_barrier();
     if (tail - head >= 64) take(64);
   };
-  constexpr int kAhead = kF32 ? 8 : 4;
+  // (Few loads ahead: each place where the queue is emptied is a copy of that code, and 32 and more
+  // of them no longer fit the instruction cache.)
+  constexpr int kAhead = kF32 ? 4 : 2;
   const int v_first = view.first_full(), v_end = view.end_full();
-  if (v_first < v_end) {
+  const int rounds = max(v_end - v_first, 0) / (kAhead * kThreads);  // of vectors that all threads have
+  const int v_rest = v_first + rounds * kAhead * kThreads;
+  if (rounds > 0) {
     uint4 next[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) next[i] = view.full(min(v_first + tid + i * kThreads, v_end - 1));
-    for (int v0 = v_first + tid; v0 - tid < v_end; v0 += kAhead * kThreads) {
+    for (int i = 0; i < kAhead; ++i) next[i] = view.full(v_first + tid + i * kThreads);
+    for (int v = v_first + tid; v < v_rest; v += kAhead * kThreads) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int v = v0 + i * kThreads;
-        if (v - tid >= v_end) break;
         float z[kPer];
-        RowView<kF32>::unpack(next[i], z);
-        next[i] = view.full(min(v + kAhead * kThreads, v_end - 1));
+        RowView<kF32>::split(next[i], z);
+        next[i] = view.full(min(v + (i + kAhead) * kThreads, v_end - 1));
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) push(v < v_end ? z[j] : -__builtin_inff(), v * kPer + j);
+        for (int j = 0; j < kPer; ++j) push(z[j], (v + i * kThreads) * kPer + j);
       }
     }
   }
+#pragma unroll 1
+  for (int p = v_rest * kPer; p < v_end * kPer; p += kThreads)
+    push(p + tid < v_end * kPer ? load_logit<kF32>(view.z, p + tid - view.shift) : -__builtin_inff(),
+         p + tid);
   if (wave == 0) {  // the ends: less than two vectors
     const int place = lane < kPer ? lane : max(v_end, v_first) * kPer + lane - kPer;
     const bool end = lane < kPer ? v_first > 0 : lane < 2 * kPer;
@@ -1061,16 +1131,20 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
     __syncthreads();
     if (tid == 0) s_num = 0, s_last = 0;
     __syncthreads();
+    int my_subs = 0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const bool in = sub[j] >= t0;
-      const unsigned long long m = __ballot(in);
-      if (!m) continue;
+    for (int j = 0; j < PER; ++j) my_subs += sub[j] >= t0;
+    if (__any(my_subs != 0)) {
+      const int incl = wave_inclusive(my_subs);
       int base = 0;
-      if (lane == 0) base = atomicAdd(&s_num, __popcll(m));
-      base = __shfl(base, 0);
-      const int at = base + __popcll(m & ((1ull << lane) - 1));
-      if (in && at < kMaxSorted) list[at] = PER * tid + j;
+      if (lane == 63) base = atomicAdd(&s_num, incl);
+      int at = __shfl(base, 63) + incl - my_subs;
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (sub[j] >= t0) {
+          if (at < kMaxSorted) list[at] = PER * tid + j;
+          ++at;
+        }
     }
     __syncthreads();
     const int lists = s_num;
@@ -1078,7 +1152,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
     if (fits) {
       // A load of 16 bytes a lane takes kGroup sub-chunks.
       constexpr int kPer = RowView<kF32>::kPer, kLanes = kSub / kPer, kGroup = 64 / kLanes;
-      constexpr int kAhead = 8;
+      constexpr int kAhead = kF32 ? 8 : 4;
       for (int i0 = wave * kGroup; i0 < lists; i0 += kAhead * kWaves * kGroup) {
         uint4 raw[kAhead];
         int at[kAhead];
@@ -1088,26 +1162,32 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
           at[i] = l < lists ? static_cast<int>(list[l]) * kSub + lane % kLanes * kPer : -kPer - 16;
           raw[i] = view.raw(at[i]);
         }
+        uint32_t key[kAhead][kPer];
+        int found = 0;
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-          if (i0 + i * kWaves * kGroup >= lists) break;
           float z[kPer];
           RowView<kF32>::unpack(raw[i], z);
 #pragma unroll
           for (int j = 0; j < kPer; ++j) {
-            const uint32_t key = key_of(z[j]);
-            const bool in = key >= t0;
-            const unsigned long long m = __ballot(in);
-            if (!m) continue;
-            int base = 0;
-            if (lane == 0) base = atomicAdd(&s_last, __popcll(m));
-            base = __shfl(base, 0);
-            const int slot = base + __popcll(m & ((1ull << lane) - 1));
-            if (in && slot < kMaxSorted)
-              cand[slot] = (static_cast<unsigned long long>(key) << 32) |
-                           (0xFFFFFFFFu - static_cast<uint32_t>(at[i] + j - view.shift));
+            key[i][j] = key_of(z[j]);
+            found += key[i][j] >= t0;
           }
         }
+        const int incl = wave_inclusive(found);
+        int base = 0;
+        if (lane == 63) base = atomicAdd(&s_last, incl);
+        int slot = __shfl(base, 63) + incl - found;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+          for (int j = 0; j < kPer; ++j)
+            if (key[i][j] >= t0) {
+              if (slot < kMaxSorted)
+                cand[slot] = (static_cast<unsigned long long>(key[i][j]) << 32) |
+                             (0xFFFFFFFFu - static_cast<uint32_t>(at[i] + j - view.shift));
+              ++slot;
+            }
       }
       __syncthreads();
       n = s_last;
@@ -1131,7 +1211,9 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
     const double goal = static_cast<double>(asked.top_p) * (asked.k > 0 ? listed : total);
     if (asked.k == 0 && asked.top_p < 1.0f && t0 > 1 && listed < goal) {
       // The cut lies below t0.
-      if (want == kMaxK) return leave();
+      // The next ones' weights, if they fell as 1 / rank up to ten times as many, would not do either:
+      // only a guess at what is faster.
+      if (want == kMaxK || listed + 2.3 * n * w.real(t0) < goal) return leave();
       want = kMaxK;
       __syncthreads();
       continue;
@@ -1192,7 +1274,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
 int weight_shift(int64_t vocab) {
   int bits = 0;
   while ((int64_t{1} << bits) < vocab) ++bits;
-  return bits < 10 ? 52 : 62 - bits;
+  return bits < 11 ? 51 : 62 - bits;
 }
 
 int64_t sub_chunks(int64_t vocab) { return (vocab + 7 + kSub - 1) / kSub; }
