@@ -5,6 +5,7 @@
 // two significant bits), the matrix products sum a group in f32, and the group's scale
 // multiplies that sum in f32: nothing is rounded before the result.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 #include "step.hpp"
@@ -520,36 +521,187 @@ __global__ __launch_bounds__(256) void w4_reduce_kernel(const float* __restrict_
   }
 }
 
-// One wave: 16 columns of the output for 16 tokens, all of k, straight from memory.
-template <int kFmt, int kGroup>
-__global__ __launch_bounds__(256) void w4_gemm_wave_kernel(W4Args a) {
-  const int lane = threadIdx.x & 63;
-  const int r = lane & 15, q = lane >> 4;
+// More than 64 tokens: a workgroup of 4 waves (2 x 2) computes 64 MB tokens x 128 columns, each wave MB x 2
+// blocks of v_mfma_f32_32x32x16_bf16.  x is A (lane l: token l % 32, eight k of half l / 32) and
+// travels, 64 k a chunk, from memory into one of three LDS buffers (global_load_lds): while chunk c is
+// multiplied c + 1 lands and c + 2 is issued, so one barrier a chunk publishes c and frees the buffer of
+// c + 2.  The weight is B (column l % 32): its codes go from memory into registers, 16 bytes
+// a lane and chunk, two chunks ahead, and become bf16 there, so that LDS carries x alone.
+//
+// A group's products are summed by themselves and then scaled into the total: exact products, at
+// the price of as many registers again and of an fma for each sum and group.  Rounding scale times
+// code to bf16 instead would need neither, and put 2^-9 of every weight into the result.
+//
+// k within a chunk comes in the order in which a lane holds its words: word j of half h is k
+// 32 h + 8 j; with groups of 32 two swaps between the halves move each group into two words, k
+// 32 (j / 2) + 16 h + 8 (j % 2).
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+constexpr int kTileThreads = 256;
+constexpr int kTileN = 128;
+constexpr int kRowBytes = 128;  // of x in LDS: 64 k; 16-byte chunk q of row r lies at q ^ ((r / 2) % 8)
+template <int kFmt, int kGroup, int MB, bool kSplit>
+__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void w4_tile_kernel(W4Args a, int span_steps, int64_t part_stride, int m_tiles, int n_tiles) {
+  constexpr int BM = 64 * MB;
+  constexpr int kLoads = BM / 32;                    // 1 KiB loads (8 rows) of a wave a chunk
+  constexpr int kScales = kGroup == 32 ? 2 : 1;      // of a column and chunk
+  __shared__ __align__(16) uint8_t buf0[BM * kRowBytes];
+  __shared__ __align__(16) uint8_t buf1[BM * kRowBytes];
+  __shared__ __align__(16) uint8_t buf2[BM * kRowBytes];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int half = lane >> 5, r32 = lane & 31;
   const int M = static_cast<int>(a.M), N = static_cast<int>(a.N), K = static_cast<int>(a.K);
-  const int n0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 16;
-  if (n0 >= N) return;
-  const int m0 = blockIdx.y * 16;
-  const int64_t n = min(n0 + r, N - 1);
-  const uint16_t* xp = a.x + static_cast<int64_t>(min(m0 + r, M - 1)) * K;
-  const uint8_t* wp = a.codes + n * (K / 2) + 16 * q;
-  const uint16_t* sp = a.scales + n * (K / kGroup);
-  f32x4_t sum[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
-  for (int s = 0; s < K / 128; ++s) {
-    bf16x8_t xf[1][4];
+
+  // Workgroups go to the 8 XCDs round robin: XCD b % 8 takes a contiguous run of tiles, ordered in
+  // bands of 8 token tiles (token tile fastest inside a band).
+  const int tiles = m_tiles * n_tiles, per = (tiles + 7) / 8;
+  const int t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= per || t >= tiles) return;  // block-uniform
+  constexpr int kBand = 8;
+  const int band = t / (kBand * n_tiles), in_band = t - band * kBand * n_tiles;
+  const int height = min(kBand, m_tiles - band * kBand);
+  const int m0 = (band * kBand + in_band % height) * BM;
+  const int n0 = (in_band / height) * kTileN;
+  const int k0 = blockIdx.y * span_steps * 128;
+  const int nk = min(span_steps * 128, K - k0) / 64;  // chunks, an even number
+  const int wm = (wave & 1) * (BM / 2), wn = (wave >> 1) * 64;
+
+  const uint16_t* src[kLoads];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      xf[0][j] = *reinterpret_cast<const bf16x8_t*>(xp + 128 * s + x_offset<kGroup>(j, q));
-    StepScales<kGroup> sc;
-    sc.load(sp + s * (128 / kGroup));
-    multiply_step<kFmt, kGroup, 1, 4>(xf, *reinterpret_cast<const uint4*>(wp + 64 * s), sc, sum);
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = 8 * (wave + 4 * i) + (lane >> 3);
+    src[i] = a.x + static_cast<int64_t>(min(m0 + r, M - 1)) * K + k0 + 8 * ((lane & 7) ^ ((r >> 1) & 7));
   }
+  const uint8_t* wp[2];
+  const uint16_t* sp[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + 4 * q + i;
-    if (m < M && n0 + r < N)
-      a.out[static_cast<int64_t>(m) * N + n0 + r] =
-          static_cast<uint16_t>(pack_bf16(kUnit<kFmt> * sum[0][i], 0.0f));
+  for (int b = 0; b < 2; ++b) {
+    const int64_t n = min(n0 + wn + 32 * b + r32, N - 1);
+    wp[b] = a.codes + n * (K / 2) + k0 / 2 + 16 * half;
+    sp[b] = a.scales + n * (K / kGroup) + k0 / kGroup;
   }
+  uint4 w[3][2];
+  uint32_t sc[3][2];
+  auto load_w = [&](int set, int c) {
+    c = min(c, nk - 1);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      w[set][b] = *reinterpret_cast<const uint4*>(wp[b] + 32 * c);
+      if constexpr (kGroup == 32)
+        sc[set][b] = *reinterpret_cast<const uint32_t*>(sp[b] + 2 * c);
+      else
+        sc[set][b] = sp[b][c * 64 / kGroup];
+    }
+  };
+  auto load_x = [&](int c, uint8_t* buf) {
+    c = min(c, nk - 1);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      __builtin_amdgcn_global_load_lds(static_cast<const void*>(src[i] + 64 * c),
+                                       (lds_void_t*)(buf + 8 * (wave + 4 * i) * kRowBytes), 16, 0, 0);
+  };
+
+  f32x16_t sum[MB][2], acc[MB][2];
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) sum[m][b][v] = 0.0f;
+
+  const int lane_sw = (r32 >> 1) & 7;
+  auto chunk = [&](int c, const uint8_t* cur, uint8_t* next, int set, auto starts_group) {
+    constexpr bool kStarts = decltype(starts_group)::value;
+    // Chunk c and its codes have landed when only what was loaded during chunk c - 1 is outstanding.
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads + 4) : "memory");
+    uint4 now[2] = {w[set][0], w[set][1]};
+    const uint32_t now_sc[2] = {sc[set][0], sc[set][1]};
+    load_w((set + 2) % 3, c + 2);
+    load_x(c + 2, next);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kGroup == 32)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        swap32(now[b].x, now[b].z);
+        swap32(now[b].y, now[b].w);
+      }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int q = kGroup == 32 ? 4 * (j >> 1) + (j & 1) + 2 * half : 4 * half + j;
+      bf16x8_t xf[MB], wf[2];
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+        xf[m] = *reinterpret_cast<const bf16x8_t*>(cur + (wm + 32 * m + r32) * kRowBytes +
+                                                   16 * (q ^ lane_sw));
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        wf[b] = w4_values<kFmt>(j == 0 ? now[b].x : j == 1 ? now[b].y : j == 2 ? now[b].z : now[b].w);
+      const bool first = kGroup == 32 ? j % 2 == 0 : j == 0 && kStarts;
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          acc[m][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xf[m], wf[b], first ? f32x16_t{} : acc[m][b],
+                                                              0, 0, 0);
+      const bool last = kGroup == 32 ? j % 2 == 1 : j == 3 && (kGroup == 64 || !kStarts);
+      if (last) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const float scale = kGroup == 32 && j == 3 ? bf16_hi(now_sc[b]) : bf16_lo(now_sc[b]);
+#pragma unroll
+          for (int m = 0; m < MB; ++m)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) sum[m][b][v] = __builtin_fmaf(scale, acc[m][b][v], sum[m][b][v]);
+        }
+      }
+    }
+  };
+  load_w(0, 0);
+  load_x(0, buf0);
+  __builtin_amdgcn_sched_barrier(0);
+  load_w(1, 1);
+  load_x(1, buf1);
+  const std::true_type starts;
+  const std::integral_constant<bool, kGroup != 128> goes_on;  // smaller groups start in every chunk
+  int c = 0;
+  for (; c + 6 <= nk; c += 6) {
+    chunk(c, buf0, buf2, 0, starts);
+    chunk(c + 1, buf1, buf0, 1, goes_on);
+    chunk(c + 2, buf2, buf1, 2, starts);
+    chunk(c + 3, buf0, buf2, 0, goes_on);
+    chunk(c + 4, buf1, buf0, 1, starts);
+    chunk(c + 5, buf2, buf1, 2, goes_on);
+  }
+  if (c < nk) {
+    chunk(c, buf0, buf2, 0, starts);
+    chunk(c + 1, buf1, buf0, 1, goes_on);
+  }
+  if (c + 2 < nk) {
+    chunk(c + 2, buf2, buf1, 2, starts);
+    chunk(c + 3, buf0, buf2, 0, goes_on);
+  }
+  // No load may still be on its way into LDS when the workgroup ends.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+  // C layout: value 4 j + i of a block is token 8 j + 4 half + i, column r32.
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int n = n0 + wn + 32 * b + r32;
+      if (n >= N) continue;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int token = m0 + wm + 32 * m + 8 * (v >> 2) + 4 * half + (v & 3);
+        if (token >= M) continue;
+        const int64_t o = static_cast<int64_t>(token) * N + n;
+        if constexpr (kSplit)
+          a.workspace[blockIdx.y * part_stride + o] = sum[m][b][v];
+        else
+          a.out[o] = static_cast<uint16_t>(pack_bf16(kUnit<kFmt> * sum[m][b][v], 0.0f));
+      }
+    }
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -557,7 +709,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 enum Kind : int { kFew, kStream, kBatch, kTile };
 struct Plan {
   Kind kind;
-  int nt, waves;  // tiles of 16 columns a wave, and waves of a workgroup
+  int nt, waves;  // tiles of 16 columns a wave, and waves of a workgroup; of kTile nt 64s of tokens
   int splits;     // spans of k with partial sums in the workspace
   int span;       // steps of 128 k in one
 };
@@ -580,7 +732,11 @@ Plan plan_of(int64_t M, int64_t N, int64_t K) {
     const int span = static_cast<int>(ceil_div(ceil_div(steps, want), 2) * 2);
     return {kBatch, nt, waves, static_cast<int>(ceil_div(steps, span)), span};
   }
-  return {kTile, 0, 0, 1, steps};
+  const int mb = M <= 64 ? 1 : 2;
+  const int64_t tiles = ceil_div(M, 64 * mb) * ceil_div(N, kTileN);
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({512 / tiles, 16, steps / 4}));
+  const int span = static_cast<int>(ceil_div(steps, want));
+  return {kTile, mb, 4, static_cast<int>(ceil_div(steps, span)), span};
 }
 int64_t part_stride(int64_t M, int64_t N) { return (M * N + 3) / 4 * 4; }
 
@@ -608,6 +764,15 @@ hipError_t launch_stream(const W4Args& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <int kFmt>
+hipError_t launch_reduce(const W4Args& a, const Plan& p, hipStream_t stream) {
+  const int64_t count = a.M * a.N;
+  hipLaunchKernelGGL(w4_reduce_kernel, dim3(static_cast<unsigned>(ceil_div(count, 1024))),
+                     dim3(256), 0, stream, a.workspace, a.out, count, part_stride(a.M, a.N), p.splits,
+                     kUnit<kFmt>);
+  return hipGetLastError();
+}
+
 template <int kFmt, int kGroup, int TM, int NT, int W>
 hipError_t launch_batch(const W4Args& a, const Plan& p, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(ceil_div(a.N, 16 * NT * W)),
@@ -622,11 +787,24 @@ hipError_t launch_batch(const W4Args& a, const Plan& p, hipStream_t stream) {
                      a, p.span, stride);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  const int64_t count = a.M * a.N;
-  hipLaunchKernelGGL(w4_reduce_kernel, dim3(static_cast<unsigned>(ceil_div(count, 1024))),
-                     dim3(256), 0, stream, a.workspace, a.out, count, stride, p.splits,
-                     kUnit<kFmt>);
-  return hipGetLastError();
+  return launch_reduce<kFmt>(a, p, stream);
+}
+
+template <int kFmt, int kGroup, int MB>
+hipError_t launch_tile(const W4Args& a, const Plan& p, hipStream_t stream) {
+  const int mt = static_cast<int>(ceil_div(a.M, 64 * MB)), nt = static_cast<int>(ceil_div(a.N, kTileN));
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(mt) * nt + 7) / 8 * 8),
+                  static_cast<unsigned>(p.splits));
+  const int64_t stride = part_stride(a.M, a.N);
+  if (p.splits == 1) {
+    hipLaunchKernelGGL((w4_tile_kernel<kFmt, kGroup, MB, false>), grid, dim3(kTileThreads), 0, stream, a,
+                       p.span, stride, mt, nt);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL((w4_tile_kernel<kFmt, kGroup, MB, true>), grid, dim3(kTileThreads), 0, stream, a,
+                     p.span, stride, mt, nt);
+  const hipError_t err = hipGetLastError();
+  return err != hipSuccess ? err : launch_reduce<kFmt>(a, p, stream);
 }
 
 template <int kFmt, int kGroup>
@@ -646,9 +824,7 @@ hipError_t launch_group(const W4Args& a, hipStream_t stream) {
     if (a.M <= 32) return launch_batch<kFmt, kGroup, 2, 1, 4>(a, p, stream);
     return launch_batch<kFmt, kGroup, 4, 1, 4>(a, p, stream);
   }
-  const dim3 grid(static_cast<unsigned>((a.N + 63) / 64), static_cast<unsigned>((a.M + 15) / 16));
-  hipLaunchKernelGGL((w4_gemm_wave_kernel<kFmt, kGroup>), grid, dim3(256), 0, stream, a);
-  return hipGetLastError();
+  return launch_tile<kFmt, kGroup, 2>(a, p, stream);
 }
 
 template <int kFmt>
