@@ -29,19 +29,24 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, p);
 }
 
+// The low four bits of byte B as a number of two's complement over 16.  (The whole byte is asked
+// for, though the conversion takes its low half, because that is one operand selection.)
+template <int B>
+__device__ __forceinline__ float code_byte(uint32_t w) {
+  return __builtin_amdgcn_cvt_off_f32_i4((w >> (8 * B)) & 0xFFu);
+}
+
 // The eight values of a word of codes, in order, over kUnit.
 template <int kFmt>
 __device__ __forceinline__ bf16x8_t w4_values(uint32_t w) {
   uint4 r;
   if constexpr (kFmt == kW4Int4) {
-    const uint32_t h = w >> 4;
-    r.x = pack_bf16(__builtin_amdgcn_cvt_off_f32_i4(w), __builtin_amdgcn_cvt_off_f32_i4(h));
-    r.y = pack_bf16(__builtin_amdgcn_cvt_off_f32_i4(w >> 8),
-                    __builtin_amdgcn_cvt_off_f32_i4(h >> 8));
-    r.z = pack_bf16(__builtin_amdgcn_cvt_off_f32_i4(w >> 16),
-                    __builtin_amdgcn_cvt_off_f32_i4(h >> 16));
-    r.w = pack_bf16(__builtin_amdgcn_cvt_off_f32_i4(w >> 24),
-                    __builtin_amdgcn_cvt_off_f32_i4(h >> 24));
+    uint32_t h = w >> 4;
+    asm("" : "+v"(h));  // no instruction: keeps the shift from being taken apart, byte by byte
+    r.x = pack_bf16(code_byte<0>(w), code_byte<0>(h));
+    r.y = pack_bf16(code_byte<1>(w), code_byte<1>(h));
+    r.z = pack_bf16(code_byte<2>(w), code_byte<2>(h));
+    r.w = pack_bf16(code_byte<3>(w), code_byte<3>(h));
   } else {
     r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 0));
     r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 1));
@@ -525,8 +530,10 @@ __global__ __launch_bounds__(256) void w4_reduce_kernel(const float* __restrict_
 // blocks of v_mfma_f32_32x32x16_bf16.  x is A (lane l: token l % 32, eight k of half l / 32) and
 // travels, 64 k a chunk, from memory into one of three LDS buffers (global_load_lds): while chunk c is
 // multiplied c + 1 lands and c + 2 is issued, so one barrier a chunk publishes c and frees the buffer of
-// c + 2.  The weight is B (column l % 32): its codes go from memory into registers, 16 bytes
-// a lane and chunk, two chunks ahead, and become bf16 there, so that LDS carries x alone.
+// c + 2.  The weight is B (column l % 32).  Its codes come the same way, 128 k (two chunks) a
+// stage, two stages ahead, and become bf16 in registers; scales 16 bytes a row at a time.  Straight
+// into registers a load would touch 32 lines for 1 KiB of codes, and again for the scales, which
+// costs more of the CU's address unit than the products take (142 against 124 us at 4,099 x 2,816 x 4,096).
 //
 // A group's products are summed by themselves and then scaled into the total: exact products, at
 // the price of as many registers again and of an fma for each sum and group.  Rounding scale times
@@ -543,11 +550,13 @@ template <int kFmt, int kGroup, int MB, bool kSplit>
 __global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void w4_tile_kernel(W4Args a, int span_steps, int64_t part_stride, int m_tiles, int n_tiles) {
   constexpr int BM = 64 * MB;
-  constexpr int kLoads = BM / 32;                    // 1 KiB loads (8 rows) of a wave a chunk
-  constexpr int kScales = kGroup == 32 ? 2 : 1;      // of a column and chunk
+  constexpr int kLoads = BM / 32;             // 1 KiB loads (8 rows) of x by a wave a chunk
   __shared__ __align__(16) uint8_t buf0[BM * kRowBytes];
   __shared__ __align__(16) uint8_t buf1[BM * kRowBytes];
   __shared__ __align__(16) uint8_t buf2[BM * kRowBytes];
+  __shared__ __align__(16) uint8_t codes0[kTileN * 64];
+  __shared__ __align__(16) uint8_t codes1[kTileN * 64];
+  __shared__ __align__(16) uint8_t codes2[kTileN * 64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int half = lane >> 5, r32 = lane & 31;
   const int M = static_cast<int>(a.M), N = static_cast<int>(a.N), K = static_cast<int>(a.K);
@@ -572,27 +581,23 @@ void w4_tile_kernel(W4Args a, int span_steps, int64_t part_stride, int m_tiles, 
     const int r = 8 * (wave + 4 * i) + (lane >> 3);
     src[i] = a.x + static_cast<int64_t>(min(m0 + r, M - 1)) * K + k0 + 8 * ((lane & 7) ^ ((r >> 1) & 7));
   }
-  const uint8_t* wp[2];
-  const uint16_t* sp[2];
+  // Load i of this wave moves 16 weight rows, 64 bytes each: lane p row p / 4, 16-byte chunk p % 4,
+  // which lies at (p % 4) ^ ((row / 4) % 4), so that 16 rows' chunks are in 16 bank groups.
+  const uint8_t* csrc[2];
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const int64_t n = min(n0 + wn + 32 * b + r32, N - 1);
-    wp[b] = a.codes + n * (K / 2) + k0 / 2 + 16 * half;
-    sp[b] = a.scales + n * (K / kGroup) + k0 / kGroup;
+  for (int i = 0; i < 2; ++i) {
+    const int row = 16 * (wave + 4 * i) + (lane >> 2);
+    csrc[i] = a.codes + static_cast<int64_t>(min(n0 + row, N - 1)) * (K / 2) + k0 / 2 +
+              16 * ((lane & 3) ^ ((row >> 2) & 3));
   }
-  uint4 w[3][2];
-  uint32_t sc[3][2];
-  auto load_w = [&](int set, int c) {
-    c = min(c, nk - 1);
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      w[set][b] = *reinterpret_cast<const uint4*>(wp[b] + 32 * c);
-      if constexpr (kGroup == 32)
-        sc[set][b] = *reinterpret_cast<const uint32_t*>(sp[b] + 2 * c);
-      else
-        sc[set][b] = sp[b][c * 64 / kGroup];
-    }
+  auto load_codes = [&](int i, int stage, uint8_t* buf) {
+    __builtin_amdgcn_global_load_lds(static_cast<const void*>(csrc[i] + 64 * min(stage, nk / 2 - 1)),
+                                     (lds_void_t*)(buf + 1024 * (wave + 4 * i)), 16, 0, 0);
   };
+  // Lane l loads the scales of column wn + l, a stage at a time.
+  const uint16_t* sp = a.scales + static_cast<int64_t>(min(n0 + wn + lane, N - 1)) * (K / kGroup) + k0 / kGroup;
+  StepScales<kGroup> sc[3];
+  auto load_scales = [&](int set, int stage) { sc[set].load(sp + min(stage, nk / 2 - 1) * (128 / kGroup)); };
   auto load_x = [&](int c, uint8_t* buf) {
     c = min(c, nk - 1);
 #pragma unroll
@@ -610,45 +615,63 @@ void w4_tile_kernel(W4Args a, int span_steps, int64_t part_stride, int m_tiles, 
       for (int v = 0; v < 16; ++v) sum[m][b][v] = 0.0f;
 
   const int lane_sw = (r32 >> 1) & 7;
-  auto chunk = [&](int c, const uint8_t* cur, uint8_t* next, int set, auto starts_group) {
-    constexpr bool kStarts = decltype(starts_group)::value;
+  auto chunk = [&](int c, const uint8_t* cur, uint8_t* next, const uint8_t* codes, uint8_t* next_codes,
+                   int set, auto even) {
+    constexpr bool kEven = decltype(even)::value;
+    constexpr bool kStarts = kEven || kGroup != 128;  // a group
     // Chunk c and its codes have landed when only what was loaded during chunk c - 1 is outstanding.
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads + 4) : "memory");
-    uint4 now[2] = {w[set][0], w[set][1]};
-    const uint32_t now_sc[2] = {sc[set][0], sc[set][1]};
-    load_w((set + 2) % 3, c + 2);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kEven ? kLoads + 1 : kLoads + 2)
+                 : "memory");
+    if constexpr (kEven) load_scales((set + 2) % 3, c / 2 + 2);
+    load_codes(kEven ? 0 : 1, c / 2 + 2, next_codes);
     load_x(c + 2, next);
     __builtin_amdgcn_sched_barrier(0);
+    uint4 now[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int row = wn + 32 * b + r32;
+      now[b] = *reinterpret_cast<const uint4*>(codes + 64 * row +
+                                               16 * (((kEven ? 0 : 2) + half) ^ ((row >> 2) & 3)));
+    }
+    // The chunk's scales: those of the lower lanes are block 0's, those of the upper block 1's.
+    const auto both = __builtin_amdgcn_permlane32_swap(sc[set].v[kGroup == 32 && !kEven ? 1 : 0],
+                                                       sc[set].v[kGroup == 32 && !kEven ? 1 : 0], false, false);
     if constexpr (kGroup == 32)
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         swap32(now[b].x, now[b].z);
         swap32(now[b].y, now[b].w);
       }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    bf16x8_t xf[2][MB], wf[2][2];
+    auto fragments = [&](int j) {
       const int q = kGroup == 32 ? 4 * (j >> 1) + (j & 1) + 2 * half : 4 * half + j;
-      bf16x8_t xf[MB], wf[2];
 #pragma unroll
       for (int m = 0; m < MB; ++m)
-        xf[m] = *reinterpret_cast<const bf16x8_t*>(cur + (wm + 32 * m + r32) * kRowBytes +
-                                                   16 * (q ^ lane_sw));
+        xf[j & 1][m] = *reinterpret_cast<const bf16x8_t*>(cur + (wm + 32 * m + r32) * kRowBytes +
+                                                          16 * (q ^ lane_sw));
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-        wf[b] = w4_values<kFmt>(j == 0 ? now[b].x : j == 1 ? now[b].y : j == 2 ? now[b].z : now[b].w);
+        wf[j & 1][b] = w4_values<kFmt>(j == 0 ? now[b].x : j == 1 ? now[b].y : j == 2 ? now[b].z : now[b].w);
+    };
+    fragments(0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (j < 3) fragments(j + 1);
       const bool first = kGroup == 32 ? j % 2 == 0 : j == 0 && kStarts;
 #pragma unroll
       for (int m = 0; m < MB; ++m)
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-          acc[m][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xf[m], wf[b], first ? f32x16_t{} : acc[m][b],
-                                                              0, 0, 0);
-      const bool last = kGroup == 32 ? j % 2 == 1 : j == 3 && (kGroup == 64 || !kStarts);
+          acc[m][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xf[j & 1][m], wf[j & 1][b],
+                                                              first ? f32x16_t{} : acc[m][b], 0, 0, 0);
+      const bool last = kGroup == 32 ? j % 2 == 1 : j == 3 && (kGroup == 64 || !kEven);
       if (last) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const float scale = kGroup == 32 && j == 3 ? bf16_hi(now_sc[b]) : bf16_lo(now_sc[b]);
+          const bool upper = kGroup == 32 ? j == 3 : kGroup == 64 ? !kEven : false;
+          const float scale = upper ? bf16_hi(both[b]) : bf16_lo(both[b]);
 #pragma unroll
           for (int m = 0; m < MB; ++m)
 #pragma unroll
@@ -657,29 +680,33 @@ void w4_tile_kernel(W4Args a, int span_steps, int64_t part_stride, int m_tiles, 
       }
     }
   };
-  load_w(0, 0);
+  load_scales(0, 0);
+  load_codes(0, 0, codes0);
+  load_codes(1, 0, codes0);
   load_x(0, buf0);
   __builtin_amdgcn_sched_barrier(0);
-  load_w(1, 1);
+  load_scales(1, 1);
+  load_codes(0, 1, codes1);
+  load_codes(1, 1, codes1);
   load_x(1, buf1);
-  const std::true_type starts;
-  const std::integral_constant<bool, kGroup != 128> goes_on;  // smaller groups start in every chunk
+  const std::true_type even;
+  const std::false_type odd;
   int c = 0;
   for (; c + 6 <= nk; c += 6) {
-    chunk(c, buf0, buf2, 0, starts);
-    chunk(c + 1, buf1, buf0, 1, goes_on);
-    chunk(c + 2, buf2, buf1, 2, starts);
-    chunk(c + 3, buf0, buf2, 0, goes_on);
-    chunk(c + 4, buf1, buf0, 1, starts);
-    chunk(c + 5, buf2, buf1, 2, goes_on);
+    chunk(c, buf0, buf2, codes0, codes2, 0, even);
+    chunk(c + 1, buf1, buf0, codes0, codes2, 0, odd);
+    chunk(c + 2, buf2, buf1, codes1, codes0, 1, even);
+    chunk(c + 3, buf0, buf2, codes1, codes0, 1, odd);
+    chunk(c + 4, buf1, buf0, codes2, codes1, 2, even);
+    chunk(c + 5, buf2, buf1, codes2, codes1, 2, odd);
   }
   if (c < nk) {
-    chunk(c, buf0, buf2, 0, starts);
-    chunk(c + 1, buf1, buf0, 1, goes_on);
+    chunk(c, buf0, buf2, codes0, codes2, 0, even);
+    chunk(c + 1, buf1, buf0, codes0, codes2, 0, odd);
   }
   if (c + 2 < nk) {
-    chunk(c + 2, buf2, buf1, 2, starts);
-    chunk(c + 3, buf0, buf2, 0, goes_on);
+    chunk(c + 2, buf2, buf1, codes1, codes0, 1, even);
+    chunk(c + 3, buf0, buf2, codes1, codes0, 1, odd);
   }
   // No load may still be on its way into LDS when the workgroup ends.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
