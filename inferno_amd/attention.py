@@ -427,27 +427,37 @@ def kv8_attention(plan: WindowPlan, q, k_base, k_scale, v_base, v_scale, output,
         scale, _kv8_format(kv_format), _window_stream(plan)))
 
 
-def _current_device(t):
-    """The device of t, which has to be the current one."""
+# The types that a buffer of the kernels' types may have: their own, or integers of the size that
+# hold their bits.  Set with the first call, as torch is imported there.
+_KINDS: dict[str, frozenset] = {}
+
+
+def _kinds() -> dict[str, frozenset]:
+    if not _KINDS:
+        import torch
+
+        _KINDS.update(bf16=frozenset((torch.bfloat16, torch.int16, torch.uint16)),
+                      byte=frozenset((torch.uint8, torch.int8)),
+                      f32=frozenset((torch.float32,)), i32=frozenset((torch.int32,)))
+    return _KINDS
+
+
+def _device_stream() -> tuple[int, int]:
+    """The current device and its current stream."""
     import torch
 
-    if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
-        raise ValueError(f"a tensor is on {t.device}, the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
-    return t.device
+    device = torch.cuda.current_device()
+    return device, int(torch._C._cuda_getCurrentRawStream(device))
 
 
-def _tensor(device, name: str, t, numel: int, itemsize: int) -> int:
-    """The address of a contiguous tensor of at least numel elements on the device."""
-    import torch
-
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if t.element_size() != itemsize or t.dtype == torch.float16 or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous, of {itemsize}-byte elements (has "
-                         f"{t.dtype}, strides {tuple(t.stride())})")
-    if t.numel() < numel:
-        raise ValueError(f"{name} has {t.numel()} elements, {numel} are needed")
+def _tensor(device: int, name: str, t, numel: int, kind: frozenset) -> int:
+    """The address of a contiguous tensor of at least numel elements on the current device."""
+    if (t.get_device() != device or t.dtype not in kind or t.numel() < numel
+            or not t.is_contiguous()):
+        types = ", ".join(sorted(str(k) for k in kind))
+        raise ValueError(f"{name} must be contiguous, on cuda:{device} (the current device), of "
+                         f"{types}, with {numel} elements at least (is {tuple(t.shape)} of {t.dtype}, "
+                         f"strides {tuple(t.stride())}, on {t.device})")
     return t.data_ptr()
 
 
@@ -472,16 +482,17 @@ def dispatch_w4_gemm_cols(x, codes, scales, output, *, rows: int, cols: int, seq
         raise ValueError(f"w_format must be one of {sorted(W4_FORMATS)}, not {w_format!r}")
     if group not in (32, 64, 128):
         raise ValueError("group must be 32, 64 or 128")
-    dev = _current_device(x)
+    k = _kinds()
+    dev, stream = _device_stream()
     ws, ws_bytes = None, 0
     if workspace is not None:
-        ws, ws_bytes = _tensor(dev, "workspace", workspace, 0, 4), workspace.numel() * 4
+        ws, ws_bytes = _tensor(dev, "workspace", workspace, 0, k["f32"]), workspace.numel() * 4
     check(lib().ifr_dispatch_w4_gemm_cols(
-        _tensor(dev, "x", x, seq_len * cols, 2),
-        _tensor(dev, "codes", codes, rows * (cols // 2), 1),
-        _tensor(dev, "scales", scales, rows * (cols // group), 2),
-        _tensor(dev, "output", output, seq_len * rows, 2), rows, cols, seq_len, group,
-        W4_FORMATS[w_format], ws, ws_bytes, _stream()))
+        _tensor(dev, "x", x, seq_len * cols, k["bf16"]),
+        _tensor(dev, "codes", codes, rows * (cols // 2), k["byte"]),
+        _tensor(dev, "scales", scales, rows * (cols // group), k["bf16"]),
+        _tensor(dev, "output", output, seq_len * rows, k["bf16"]), rows, cols, seq_len, group,
+        W4_FORMATS[w_format], ws, ws_bytes, stream))
 
 
 def dispatch_norm_residual(y, residual, residual_out, x_out=None, *, hidden: int, seq_len: int,
@@ -494,31 +505,27 @@ def dispatch_norm_residual(y, residual, residual_out, x_out=None, *, hidden: int
     x_out = norm(residual_out) * pre_weight.  residual is bf16 or f32, and residual_out of the
     same type; gate has hidden elements or seq_len * hidden.  residual_out may be residual,
     x_out may be y.  No counterpart in the reference."""
-    import torch
-
-    dev = _current_device(y)
+    k = _kinds()
+    bf16 = k["bf16"]
+    dev, stream = _device_stream()
     n = seq_len * hidden
-    f32 = residual.dtype == torch.float32
-    if residual_out.dtype != residual.dtype:
-        raise ValueError(f"residual is {residual.dtype}, residual_out {residual_out.dtype}")
+    f32 = residual.dtype in k["f32"]
+    res = k["f32"] if f32 else bf16
     if post_weight is not None and not post_norm:
         raise ValueError("post_weight without post_norm")
     if pre_weight is not None and x_out is None:
         raise ValueError("pre_weight without x_out")
-
-    def ptr(name, t, numel):
-        return None if t is None else _tensor(dev, name, t, numel, 2)
-
     gate_stride = 0
     if gate is not None and gate.numel() != hidden:
         gate_stride = hidden
     check(lib().ifr_norm_residual(
-        ptr("y", y, n), _tensor(dev, "residual", residual, n, 4 if f32 else 2),
-        _tensor(dev, "residual_out", residual_out, n, 4 if f32 else 2), ptr("x_out", x_out, n),
-        ptr("post_weight", post_weight, hidden),
-        ptr("gate", gate, n if gate_stride else hidden), ptr("pre_weight", pre_weight, hidden),
-        hidden, seq_len, int(f32), int(post_norm), gate_stride, residual_scale, block_scale, eps,
-        _stream()))
+        _tensor(dev, "y", y, n, bf16), _tensor(dev, "residual", residual, n, res),
+        _tensor(dev, "residual_out", residual_out, n, res),
+        None if x_out is None else _tensor(dev, "x_out", x_out, n, bf16),
+        None if post_weight is None else _tensor(dev, "post_weight", post_weight, hidden, bf16),
+        None if gate is None else _tensor(dev, "gate", gate, n if gate_stride else hidden, bf16),
+        None if pre_weight is None else _tensor(dev, "pre_weight", pre_weight, hidden, bf16),
+        hidden, seq_len, f32, post_norm, gate_stride, residual_scale, block_scale, eps, stream))
 
 
 def sample_workspace(num_rows: int, vocab: int, device="cuda"):
@@ -539,13 +546,13 @@ def dispatch_sample_tokens(logits, uniform, tokens, workspace=None, *, num_rows:
     include/inferno_hip.h has the rules).  logits: bf16 or f32, either a matrix whose rows
     may be apart, or with row_stride a flat buffer; uniform, temperature, top_p, min_p:
     f32, top_k and tokens int32, a number for each row.  No counterpart in the reference."""
-    import torch
-
-    dev = _current_device(logits)
-    f32 = logits.dtype == torch.float32
+    k = _kinds()
+    f, i = k["f32"], k["i32"]
+    dev, stream = _device_stream()
+    f32 = logits.dtype in f
+    kind = f if f32 else k["bf16"]
     if row_stride is not None:
-        ptr = _tensor(dev, "logits", logits, (num_rows - 1) * row_stride + vocab,
-                      4 if f32 else 2)
+        ptr = _tensor(dev, "logits", logits, (num_rows - 1) * row_stride + vocab, kind)
     else:
         if (logits.dim() != 2 or logits.shape[0] < num_rows or logits.shape[1] < vocab
                 or (vocab > 1 and logits.stride(1) != 1)
@@ -553,23 +560,18 @@ def dispatch_sample_tokens(logits, uniform, tokens, workspace=None, *, num_rows:
             raise ValueError(f"logits of shape {tuple(logits.shape)} and strides "
                              f"{tuple(logits.stride())} have no {num_rows} rows of {vocab}")
         row_stride = max(logits.stride(0), vocab)
-        ptr = _tensor(dev, "logits", logits[:1, :vocab], 0, 4 if f32 else 2)
+        ptr = _tensor(dev, "logits", logits[:1, :vocab], 0, kind)
     ws, ws_bytes = None, 0
     if workspace is not None:
-        ws, ws_bytes = _tensor(dev, "workspace", workspace, 0, 4), workspace.numel() * 4
-
-    def of_rows(name, t, dtype):
-        if t is None:
-            return None
-        if t.dtype != dtype:
-            raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
-        return _tensor(dev, name, t, num_rows, 4)
-
+        ws, ws_bytes = _tensor(dev, "workspace", workspace, 0, f), workspace.numel() * 4
     check(lib().ifr_dispatch_sample_tokens(
-        ptr, of_rows("uniform", uniform, torch.float32), of_rows("tokens", tokens, torch.int32),
-        of_rows("temperature", temperature, torch.float32), of_rows("top_k", top_k, torch.int32),
-        of_rows("top_p", top_p, torch.float32), of_rows("min_p", min_p, torch.float32), num_rows,
-        vocab, row_stride, int(f32), ws, ws_bytes, _stream()))
+        ptr, _tensor(dev, "uniform", uniform, num_rows, f),
+        _tensor(dev, "tokens", tokens, num_rows, i),
+        None if temperature is None else _tensor(dev, "temperature", temperature, num_rows, f),
+        None if top_k is None else _tensor(dev, "top_k", top_k, num_rows, i),
+        None if top_p is None else _tensor(dev, "top_p", top_p, num_rows, f),
+        None if min_p is None else _tensor(dev, "min_p", min_p, num_rows, f), num_rows, vocab,
+        row_stride, f32, ws, ws_bytes, stream))
 
 
 __all__ = [

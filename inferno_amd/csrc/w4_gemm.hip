@@ -547,7 +547,7 @@ constexpr int kTileThreads = 256;
 constexpr int kTileN = 128;
 constexpr int kRowBytes = 128;  // of x in LDS: 64 k; 16-byte chunk q of row r lies at q ^ ((r / 2) % 8)
 template <int kFmt, int kGroup, int MB, bool kSplit>
-__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(MB == 1 ? 3 : 2)))
 void w4_tile_kernel(W4Args a, int span_steps, int64_t part_stride, int m_tiles, int n_tiles) {
   constexpr int BM = 64 * MB;
   constexpr int kLoads = BM / 32;             // 1 KiB loads (8 rows) of x by a wave a chunk
@@ -745,6 +745,34 @@ struct Plan {
 // stream them.
 constexpr int64_t kManyColumns = 32768;
 
+// Tokens of a tile and spans of k past 64 tokens: the cheapest by a model of the launch, fitted to 65
+// to 1,024 tokens, both tiles and 1 to 16 spans at N = 2,816, K = 4,096, int4 in groups of 128: 32
+// steps of up to 256 tiles take 33 us (64 tokens) or 45 (128), of each 256 of more tiles, of which a CU
+// has several at once, 23 or 43; spans add a launch and the partial sums' way out and back.
+// It picks the best measured or one within 12 % of it: 65 tokens 15.1 us (best 13.4), 256 20.4
+// (19.6), 512 28.0 (28.0; one span of 128 tokens 48.3), 1,024 43.4 (43.4).
+Plan tile_plan(int64_t M, int64_t N, int steps) {
+  Plan best{kTile, 2, 4, 1, steps};
+  double best_us = 1e30;
+  for (int mb = 1; mb <= 2; ++mb) {
+    const int64_t tiles = ceil_div(M, 64 * mb) * ceil_div(N, kTileN);
+    for (int want = 1; want <= 16 && (want == 1 || steps >= 4 * want); ++want) {
+      const int span = static_cast<int>(ceil_div(steps, want));
+      const int splits = static_cast<int>(ceil_div(steps, span));
+      const int64_t blocks = tiles * splits;
+      const double tile = blocks <= 256 ? (mb == 1 ? 33.0 : 45.0)
+                                        : (mb == 1 ? 23.0 : 43.0) * static_cast<double>(ceil_div(blocks, 256));
+      double us = 2.5 + tile * span / 32.0;
+      if (splits > 1) us += 3.0 + 0.9e-6 * static_cast<double>(splits) * static_cast<double>(M * N);
+      if (us < best_us) {
+        best_us = us;
+        best = {kTile, mb, 4, splits, span};
+      }
+    }
+  }
+  return best;
+}
+
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
   const int steps = static_cast<int>(K / 128);
   if (M <= 16 && N < kManyColumns) return {kFew, N <= 4096 ? 1 : N <= 8192 ? 2 : 4, 16, 1, steps};
@@ -759,11 +787,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K) {
     const int span = static_cast<int>(ceil_div(ceil_div(steps, want), 2) * 2);
     return {kBatch, nt, waves, static_cast<int>(ceil_div(steps, span)), span};
   }
-  const int mb = M <= 64 ? 1 : 2;
-  const int64_t tiles = ceil_div(M, 64 * mb) * ceil_div(N, kTileN);
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({512 / tiles, 16, steps / 4}));
-  const int span = static_cast<int>(ceil_div(steps, want));
-  return {kTile, mb, 4, static_cast<int>(ceil_div(steps, span)), span};
+  return tile_plan(M, N, steps);
 }
 int64_t part_stride(int64_t M, int64_t N) { return (M * N + 3) / 4 * 4; }
 
@@ -851,7 +875,7 @@ hipError_t launch_group(const W4Args& a, hipStream_t stream) {
     if (a.M <= 32) return launch_batch<kFmt, kGroup, 2, 1, 4>(a, p, stream);
     return launch_batch<kFmt, kGroup, 4, 1, 4>(a, p, stream);
   }
-  return launch_tile<kFmt, kGroup, 2>(a, p, stream);
+  return p.nt == 1 ? launch_tile<kFmt, kGroup, 1>(a, p, stream) : launch_tile<kFmt, kGroup, 2>(a, p, stream);
 }
 
 template <int kFmt>
