@@ -496,119 +496,88 @@ __device__ __forceinline__ void sample_descent(const SampleArgs& a, int shift, i
 }
 
 constexpr int kMaxK = 1024;     // candidates that are sought
-constexpr int kMaxSorted = 2048;  // and at most taken
+constexpr int kMaxTaken = 2048;  // and at most taken
 
-// The value of lane ^ D.
-template <int D>
-__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
-  if constexpr (D == 1) return dpp_i32<kDppXor1>(v);
-  if constexpr (D == 2) return dpp_i32<kDppXor2>(v);
-  if constexpr (D == 4) return dpp_i32<kDppQuadReverse>(dpp_i32<kDppHalfMirror>(v));
-  if constexpr (D == 8) return dpp_i32<kDppRowRor8>(v);
-  if constexpr (D == 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return threadIdx.x & 16 ? r[0] : r[1];
-  }
-  if constexpr (D == 32) {
-    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return threadIdx.x & 32 ? r[0] : r[1];
-  }
-}
-template <int D>
-__device__ __forceinline__ unsigned long long lane_xor64(unsigned long long v) {
-  return (static_cast<unsigned long long>(lane_xor<D>(static_cast<uint32_t>(v >> 32))) << 32) |
-         lane_xor<D>(static_cast<uint32_t>(v));
-}
-
-// Bitonic sort, descending, of kT * E entries: entry 64 E wave + 64 e + lane is in register e of its
-// lane, so that only distances of 64 E and more pass through LDS.
+// The entry in which a sum over the workgroup's entries, the largest `order` first, reaches target_of(the
+// sum of all): its order, 0 if the target is 0.  Entry j of a thread has order[j] and weight[j], 0
+// for none; bin_of(j) < 2 kT falls as the order rises, and the sums of the bins say in which one it lies.
 template <int kT, int E>
-__device__ __forceinline__ void sort_registers(unsigned long long* v, int n) {
-  const int tid = threadIdx.x, lane = tid & 63, base = (tid >> 6) * 64 * E;
-  unsigned long long x[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = base + 64 * e + lane;
-    x[e] = i < n ? v[i] : 0;
-  }
-  auto order = [](unsigned long long mine, unsigned long long theirs, bool larger) {
-    return (mine < theirs) == larger ? theirs : mine;
-  };
-  for (int width = 2; width <= kT * E; width *= 2) {
-    for (int d = width / 2; d >= 64 * E; d /= 2) {
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[base + 64 * e + lane] = x[e];
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int i = base + 64 * e + lane;
-        x[e] = order(x[e], v[i ^ d], ((i & d) == 0) == ((i & width) == 0));
-      }
-    }
-#pragma unroll
-    for (int r = E / 2; r > 0; r /= 2) {
-      if (width < 128 * r) continue;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (e & r) continue;
-        const bool down = ((base + 64 * e + lane) & width) == 0;
-        const unsigned long long lo = x[e], hi = x[e + r];
-        if ((lo < hi) == down) x[e] = hi, x[e + r] = lo;
-      }
-    }
-    auto step = [&](auto distance) {
-      constexpr int kD = decltype(distance)::value;
-      if (width < 2 * kD) return;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int i = base + 64 * e + lane;
-        x[e] = order(x[e], lane_xor64<kD>(x[e]), ((i & kD) == 0) == ((i & width) == 0));
-      }
-    };
-    step(std::integral_constant<int, 32>{});
-    step(std::integral_constant<int, 16>{});
-    step(std::integral_constant<int, 8>{});
-    step(std::integral_constant<int, 4>{});
-    step(std::integral_constant<int, 2>{});
-    step(std::integral_constant<int, 1>{});
-  }
-  __syncthreads();
-#pragma unroll
-  for (int e = 0; e < E; ++e) v[base + 64 * e + lane] = x[e];
-  __syncthreads();
-}
+struct Crossing {
+  unsigned long long sums[2 * kT];
+  unsigned long long orders[kT * E], weights[kT * E];  // of that bin's entries
+  unsigned long long waves[kT / 64];
+  unsigned long long total, above, result;
+  int bin, count;
 
-// Descending, in place (n up to kMaxSorted, of which v has room for all).
+  template <typename Bin, typename Target>
+  __device__ __forceinline__ unsigned long long find(const unsigned long long (&order)[E],
+                                                     const unsigned long long (&weight)[E],
+                                                     Bin bin_of, Target target_of) {
+    const int tid = threadIdx.x;
+    sums[2 * tid] = 0, sums[2 * tid + 1] = 0;
+    if (tid == 0) count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (weight[j]) atomicAdd(&sums[bin_of(j)], weight[j]);
+    __syncthreads();
+    const unsigned long long a = sums[2 * tid], b = sums[2 * tid + 1];
+    const unsigned long long incl = block_inclusive<unsigned long long>(a + b, waves);
+    if (tid == kT - 1) total = incl;
+    __syncthreads();
+    const unsigned long long target = target_of(total);
+    if (target == 0) return 0;  // block-uniform
+    const unsigned long long before = incl - a - b;
+    if (before < target && target <= incl) {
+      const bool first = target <= before + a;
+      bin = 2 * tid + !first;
+      above = first ? before : before + a;
+    }
+    __syncthreads();
+    const int at = bin;
+    const unsigned long long ahead = above;
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (weight[j] && bin_of(j) == at) {
+        const int slot = atomicAdd(&count, 1);
+        orders[slot] = order[j];
+        weights[slot] = weight[j];
+      }
+    __syncthreads();
+    const int n = count;
+    for (int i = tid; i < n; i += kT) {
+      const unsigned long long mine = orders[i];
+      unsigned long long sum = ahead;
+      for (int q = 0; q < n; ++q) sum += orders[q] > mine ? weights[q] : 0;
+      if (sum < target && target <= sum + weights[i]) result = mine;
+    }
+    __syncthreads();
+    return result;
+  }
+};
+
+// Descending, in place.  Each entry counts those above it.
 template <int kT>
 __device__ __forceinline__ void sort_descending(unsigned long long* v, unsigned long long* tmp, int n) {
-  const int tid = threadIdx.x;
-  if (n <= 256) {  // each entry counts those above it
-    if (tid < n) {
-      const unsigned long long mine = v[tid];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += v[j] > mine;
-      tmp[rank] = mine;
-    }
-    __syncthreads();
-    if (tid < n) v[tid] = tmp[tid];
-    __syncthreads();
-  } else if (n <= kT) {
-    sort_registers<kT, 1>(v, n);
-  } else if (n <= 2 * kT) {
-    sort_registers<kT, 2>(v, n);
-  } else {
-    sort_registers<kT, kMaxSorted / kT>(v, n);
+  for (int i = threadIdx.x; i < n; i += kT) {
+    const unsigned long long mine = v[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += v[j] > mine;
+    tmp[rank] = mine;
   }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kT) v[i] = tmp[i];
+  __syncthreads();
 }
 
-constexpr int kMaxBand = 12288;
+constexpr int kMaxBand = 11264;
+constexpr int kMaxEqual = 1024;  // equal logits at the cut of a wide row
 constexpr uint32_t kInfKey = 0xFF800000u;  // of +inf
 
 // A row without a top-k that keeps very many tokens: one pass over its logits.
 //
 // min-p alone: the pass adds the weights of the kept ones by sub-chunk.  top-p: first a sample (about
-// 32,000 of the logits, evenly spread) says where the weights below add up to about 1 - top_p of all;
+// 16,000 of the logits, evenly spread) says where the weights below add up to about 1 - top_p of all;
 // those are many small ones, so a sample of them is good to a few percent.  Tokens above that
 // band go to the sums, those within it to a list, in which the cut is then found from its keys' bits.
 // False if it is not there (or the list is full, or very many are equal): the caller descends.
@@ -622,7 +591,7 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
                                          unsigned long long* digits, unsigned long long* band,
                                          unsigned long long* waves, Found* found) {
   unsigned long long* queues = digits;  // between the two uses of the digits
-  __shared__ unsigned long long order[256];
+  __shared__ unsigned long long order[kMaxEqual];
   constexpr int kPer = RowView<kF32>::kPer;
   constexpr int kBand = 1024;  // bins of the sample
   __shared__ int s_n, s_a, s_b, s_place;
@@ -646,7 +615,7 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
     if (!(per > 0.0f && per < 1e30f)) return false;
     for (int i = tid; i < kBins; i += kThreads) digits[i] = 0;
     __syncthreads();
-    const int stride = max(1, vectors / (32768 / kPer));
+    const int stride = max(1, vectors / (16384 / kPer));
     unsigned long long tail_sum = 0;  // of the last bin
     for (int v = tid * stride; v < vectors; v += kThreads * stride) {
       float z[kPer];
@@ -805,12 +774,12 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
     for (int i = tid; i < listed; i += kThreads)
       if (static_cast<uint32_t>(band[i] >> 32) == prefix) {
         const int slot = atomicAdd(&s_n, 1);
-        if (slot < kMaxSorted) digits[slot] = band[i];
+        if (slot < kMaxEqual) digits[slot] = band[i];
       }
     __syncthreads();
     const int equal = s_n;
     __syncthreads();
-    if (equal > kMaxSorted) return false;
+    if (equal > kMaxEqual) return false;
     sort_descending<kThreads>(digits, order, equal);
     cut_key = prefix;
     cut_index = 0xFFFFFFFFu - static_cast<uint32_t>(
@@ -918,10 +887,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
     RowRest* __restrict__ rest, int num_subs) {
   constexpr int kWaves = kPickThreads / 64;
   constexpr int kPickBins = 2 * kPickThreads;
-  constexpr int kEach = kMaxSorted / kPickThreads;  // entries of a thread
-  __shared__ unsigned long long cand[kMaxSorted];
-  __shared__ unsigned long long other[kMaxSorted];
-  __shared__ uint32_t list[kMaxSorted];
+  constexpr int kEach = kMaxTaken / kPickThreads;  // entries of a thread
+  __shared__ unsigned long long cand[kMaxTaken];
+  __shared__ uint32_t list[kMaxTaken];
+  __shared__ Crossing<kPickThreads, kEach> crossing;
   __shared__ uint32_t bins[kPickBins];
   __shared__ unsigned long long waves[kWaves];
   __shared__ unsigned long long s_counts[2][kWaves];
@@ -981,7 +950,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
     }
     return;
   }
-  const Weights w{top, static_cast<double>(logit_of(top)), asked.rate(), 1.0};
+  const Weights w{top, static_cast<double>(logit_of(top)), asked.rate(), 0x1p51};
   double mass[PER];
   double my_mass = 0.0, mass_incl = 0.0, total = 0.0;
   if (asked.needs_sums()) {
@@ -1060,7 +1029,8 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
   }
 
   int want = asked.k > 0 ? static_cast<int>(asked.k) : 128;
-  int n = 0, kept = 0;
+  // Thread t has the candidates t, t + kPickThreads, ..: (key, lowest index first), weight.
+  unsigned long long entry[kEach], weight[kEach];
   for (;;) {
     // A key t0 with `want` sub-chunks or more at or above it, and not many more; 1 (every token that
     // can be drawn) if there are not as many.
@@ -1070,7 +1040,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
       const double depth = -log2(floor_w) / w.rate;
       const float z = static_cast<float>(w.zmax - depth - 1e-5 * (__builtin_fabs(w.zmax) + depth));
       t0 = min(max(key_of(z), 1u), top);
-    } else if (num_subs * kSub > kMaxSorted) {
+    } else if (num_subs * kSub > kMaxTaken) {
       const int b0 = static_cast<int>(bins[2 * tid]), b1 = static_cast<int>(bins[2 * tid + 1]);
       const int incl = block_inclusive<int>(b0 + b1, reinterpret_cast<int*>(waves));
       if (tid == 0) s_at = -1, s_key = 0xFFFFFFFFu;
@@ -1142,13 +1112,13 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
 #pragma unroll
       for (int j = 0; j < PER; ++j)
         if (sub[j] >= t0) {
-          if (at < kMaxSorted) list[at] = PER * tid + j;
+          if (at < kMaxTaken) list[at] = PER * tid + j;
           ++at;
         }
     }
     __syncthreads();
     const int lists = s_num;
-    bool fits = lists <= kMaxSorted;
+    bool fits = lists <= kMaxTaken;
     if (fits) {
       // A load of 16 bytes a lane takes kGroup sub-chunks.
       constexpr int kPer = RowView<kF32>::kPer, kLanes = kSub / kPer, kGroup = 64 / kLanes;
@@ -1183,89 +1153,89 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
 #pragma unroll
           for (int j = 0; j < kPer; ++j)
             if (key[i][j] >= t0) {
-              if (slot < kMaxSorted)
+              if (slot < kMaxTaken)
                 cand[slot] = (static_cast<unsigned long long>(key[i][j]) << 32) |
                              (0xFFFFFFFFu - static_cast<uint32_t>(at[i] + j - view.shift));
               ++slot;
             }
       }
       __syncthreads();
-      n = s_last;
-      fits = n <= kMaxSorted;
+      fits = s_last <= kMaxTaken;
     }
     if (!fits) return leave();  // block-uniform
-    sort_descending<kPickThreads>(cand, other, n);
-    const int first = asked.k > 0 ? min(n, static_cast<int>(asked.k)) : n;
-    // Thread t has entries kEach t .. kEach t + kEach - 1.
-    double v[kEach], mine = 0.0;
+    const int n = s_last;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      const int i = kEach * tid + j;
-      v[j] = i < first ? w.real(static_cast<uint32_t>(cand[i] >> 32)) : 0.0;
-      mine += v[j];
+      const int i = tid + kPickThreads * j;
+      entry[j] = i < n ? cand[i] : 0;
     }
-    const double incl = block_inclusive<double>(mine, reinterpret_cast<double*>(waves));
-    if (tid == kPickThreads - 1) s_sum = incl;
-    __syncthreads();
-    const double listed = s_sum;
-    const double goal = static_cast<double>(asked.top_p) * (asked.k > 0 ? listed : total);
-    if (asked.k == 0 && asked.top_p < 1.0f && t0 > 1 && listed < goal) {
-      // The cut lies below t0.
-      // The next ones' weights, if they fell as 1 / rank up to ten times as many, would not do either:
-      // only a guess at what is faster.
-      if (want == kMaxK || listed + 2.3 * n * w.real(t0) < goal) return leave();
+    // Bins of the logits from the largest down to t0.
+    const float t0_per = static_cast<float>(kPickBins - 1) / (zmax - logit_of(t0));
+    const bool t0_binned = t0 > 1 && t0_per > 0.0f && t0_per < 1e30f;
+    auto entry_bin = [&](int j) {
+      const float z = logit_of(static_cast<uint32_t>(entry[j] >> 32));
+      return t0_binned ? min(static_cast<int>((zmax - z) * t0_per), kPickBins - 1) : 0;
+    };
+    auto keep_from = [&](unsigned long long cut) {
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (entry[j] < cut) entry[j] = 0, weight[j] = 0;
+    };
+    if (asked.k > 0 && n > asked.k) {
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) weight[j] = entry[j] != 0;
+      keep_from(crossing.find(entry, weight, entry_bin, [&](unsigned long long) {
+        return static_cast<unsigned long long>(asked.k);
+      }));
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) weight[j] = entry[j] ? w.fixed(static_cast<uint32_t>(entry[j] >> 32)) : 0;
+    if (by_floor || asked.top_p == 1.0f) break;
+    bool below = false, guess = false;
+    const unsigned long long cut = crossing.find(entry, weight, entry_bin, [&](unsigned long long listed) {
+      const double all = asked.k > 0 ? static_cast<double>(listed) : total * w.unit;
+      const double goal = __builtin_ceil(static_cast<double>(asked.top_p) * all);
+      const double have = static_cast<double>(listed);
+      if (asked.k == 0 && t0 > 1 && have < goal) {  // the cut lies below t0
+        below = true;
+        // The next ones' weights, if they fell as 1 / rank up to ten times as many, would not do
+        // either: only a guess at what is faster.
+        guess = have + 2.3 * n * w.real(t0) * w.unit < goal;
+        return 0ull;
+      }
+      if (goal >= have) return 0ull;  // all of them
+      return goal < 1.0 ? 1ull : static_cast<unsigned long long>(goal);
+    });
+    if (below) {
+      if (want == kMaxK || guess) return leave();
       want = kMaxK;
       __syncthreads();
       continue;
     }
-    double before = incl - mine;
-    int c = 0;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const int i = kEach * tid + j;
-      const bool in_p = asked.top_p == 1.0f || i == 0 || before < goal;
-      c += i < first && in_p && (v[j] >= floor_w || static_cast<uint32_t>(cand[i] >> 32) == top);
-      before += v[j];
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) c += __shfl_xor(c, d);
-    if (lane == 0) s_counts[0][wave] = static_cast<unsigned long long>(c);
-    __syncthreads();
-    kept = static_cast<int>(s_counts[0][lane % kWaves]);
-#pragma unroll
-    for (int d = 1; d < kWaves; d *= 2) kept += __shfl_xor(kept, d);
+    keep_from(cut);
     break;
   }
-  __syncthreads();
-  // The kept ones, a prefix, in order of their indexes: (index from the end, place) descending.
-  // The keys move to list[], which the sub-chunks no longer need.
-  for (int i = tid; i < kept; i += kPickThreads) {
-    const unsigned long long e = cand[i];
-    list[i] = static_cast<uint32_t>(e >> 32);
-    other[i] = (e << 32) | static_cast<uint32_t>(i);
-  }
-  __syncthreads();
-  sort_descending<kPickThreads>(other, cand, kept);
-  double v[kEach], mine = 0.0;
-#pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    const int i = kEach * tid + j;
-    v[j] = i < kept ? w.real(list[static_cast<uint32_t>(other[i])]) : 0.0;
-    mine += v[j];
-  }
-  const double incl = block_inclusive<double>(mine, reinterpret_cast<double*>(waves));
-  if (tid == kPickThreads - 1) s_sum = incl;
-  __syncthreads();
-  const double goal = u * s_sum;
-  if (tid == first_thread(mine > 0.0 && incl > goal, mine > 0.0, &s_at, &s_last)) {
-    int at = -1;
-    double before = incl - mine;
+  if (asked.min_p > 0.0f) {
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      if (v[j] > 0.0 && (at < 0 || goal >= before)) at = kEach * tid + j;
-      before += v[j];
+      const uint32_t key = static_cast<uint32_t>(entry[j] >> 32);
+      if (entry[j] && !(w.real(key) >= floor_w || key == top)) weight[j] = 0;
     }
-    a.tokens[row] = static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(other[at] >> 32));
+  }
+  // The draw, by index.
+  int by = 0;
+  while ((view.vocab - 1) >> by >= kPickBins) ++by;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) entry[j] &= 0xFFFFFFFFull;  // 2^32 - 1 - index
+  __syncthreads();
+  const unsigned long long drawn = crossing.find(
+      entry, weight, [&](int j) { return static_cast<int>((0xFFFFFFFFu - static_cast<uint32_t>(entry[j])) >> by); },
+      [&](unsigned long long listed) {  // the first whose sum passes u of all
+        const unsigned long long goal = static_cast<unsigned long long>(u * static_cast<double>(listed));
+        return min(goal, listed - 1) + 1;
+      });
+  if (tid == 0) {
+    a.tokens[row] = static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(drawn));
     rest[row].is_left = 0;
   }
 }
