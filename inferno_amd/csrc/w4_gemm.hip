@@ -708,6 +708,11 @@ void w4_tile_kernel(W4Args a, int span_steps, int64_t part_stride, int m_tiles, 
     chunk(c + 2, buf2, buf1, codes1, codes0, 1, even);
     chunk(c + 3, buf0, buf2, codes1, codes0, 1, odd);
   }
+  // The scales that the last chunks load are of no use, but the waits count those loads.
+#pragma unroll
+  for (int set = 0; set < 3; ++set)
+#pragma unroll
+    for (uint32_t v : sc[set].v) asm volatile("" ::"v"(v));
   // No load may still be on its way into LDS when the workgroup ends.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
