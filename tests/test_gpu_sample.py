@@ -262,3 +262,79 @@ def test_refusals():
     for bad in (dict(vocab=0), dict(row_stride=99), dict(num_rows=-1), dict(vocab=(1 << 20) + 1, num_rows=1, row_stride=1 << 21, z=empty_dev((1 << 20) + 1, np.float32))):
         with pytest.raises(InfernoHipError):
             call(**bad)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_rows_with_very_many_kept_tokens(f32):
+    """Cuts among tens of thousands of tokens, equal ones among them, and thresholds that keep that many: the rows of the
+    third launch, of odd lengths at odd addresses."""
+    announce(f"sample wide rows f32={f32}")
+    rng = np.random.default_rng(21)
+    vocab = 150001
+    z = rng.standard_normal((14, vocab)) * 2.5
+    z[4:8] = rng.exponential(1.25, (4, vocab)) - 4
+    z[8] = np.round(z[8] * 2) / 2          # some forty values
+    z[9] = 1.0                             # one
+    z[10] = np.where(rng.random(vocab) < 0.3, 2.0, 1.0)
+    z[11, ::2] = -np.inf
+    z[12] = np.linspace(5, -5, vocab)      # in order, which a sample of every n-th token sees well
+    z[13] = np.where(np.arange(vocab) % 16 == 0, -20.0, z[13])  # and one that it sees badly
+    asked = [(1.0, 0, p, floor) for p, floor in ((0.9, 0.0), (0.5, 0.0), (0.99, 1e-4), (0.05, 0.0))] * 3 + [(1.0, 0, 0.95, 0.0)] * 2
+    _check(z, asked, rng.random(14), f32, pad=5, offset=3)
+    _check(z, [(1.3, 0, 1.0, f) for f in (1e-3, 1e-2, 1e-4, 0.3, 1e-6, 1e-3, 0.05, 1e-5, 0.5, 0.9, 0.37, 0.01, 0.2, 1e-7)], rng.random(14), f32)
+    _check(z, [(0.7, k, 0.97, 0.0) for k in (2000, 5000, 1024, 1025, 70000, 149999, 1500, 3000, 4000, 77777, 50000, 60000, 1100, 9000)],
+           rng.random(14), f32, offset=1)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_candidates_among_equal_logits(f32):
+    """Cuts of top-k and top-p that fall among hundreds of equal logits within the candidates."""
+    announce(f"sample equal candidates f32={f32}")
+    rng = np.random.default_rng(22)
+    z = rng.standard_normal((8, 30000)) - 8
+    for r in range(8):
+        at = rng.permutation(30000)
+        z[r, at[:5]] = 4.0
+        z[r, at[5:5 + 150 * (r + 1)]] = 3.0
+    _check(z, [(1.0, k, p, 0.0) for k, p in ((64, 1.0), (100, 0.9), (300, 0.5), (0, 0.8), (700, 0.999), (0, 0.5), (1000, 0.99), (1024, 0.7))],
+           rng.random(8), f32)
+
+
+def test_calls_at_once_and_graphs_that_share_a_workspace():
+    import torch
+
+    announce("sample at once")
+    rows, vocab = 24, 40000
+    cases = []
+    for s in (1, 2):
+        rng = np.random.default_rng(s)
+        bits, held = _logits(rng.exponential(1.3, (rows, vocab)) - 4, True)
+        asked, u, want = _prepare(held, [MIX[r % len(MIX)] for r in range(rows)], rng.random(rows))
+        cols = [to_dev(np.array(c, np.int32 if i == 1 else np.float32)) for i, c in enumerate(zip(*asked))]
+        cases.append((to_dev(bits), to_dev(np.array(u, np.float32)), empty_dev(rows, np.int32), cols, want))
+    spaces = [A.sample_workspace(rows, vocab) for _ in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+
+    def call(i, ws):
+        z, u, tokens, cols, _ = cases[i]
+        A.dispatch_sample_tokens(z, u, tokens, ws, num_rows=rows, vocab=vocab, temperature=cols[0], top_k=cols[1], top_p=cols[2], min_p=cols[3])
+
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                call(i, spaces[i])
+    torch.cuda.synchronize()
+    graphs = []
+    for i in range(2):
+        assert list(from_dev(cases[i][2], np.int32)) == cases[i][4]
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(i, spaces[0])
+        graphs.append(g)
+    for i in (0, 1, 1, 0, 1):
+        cases[i][2].zero_()
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert list(from_dev(cases[i][2], np.int32)) == cases[i][4]
+    del graphs

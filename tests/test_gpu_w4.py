@@ -183,3 +183,62 @@ def test_refusals():
     for bad in (dict(cols=192), dict(rows=0), dict(cols=0), dict(x=x[1:], seq_len=3), dict(seq_len=-1)):
         with pytest.raises(InfernoHipError):
             call(**bad)
+
+
+@pytest.mark.parametrize("m,k", [(61, 4096), (300, 4096), (16, 8192)])
+def test_calls_at_once_and_graphs_that_share_a_workspace(m, k):
+    """Two streams with a workspace each; then two graphs over one workspace, replayed in turn."""
+    import torch
+
+    announce(f"w4 at once m={m} k={k}")
+    n, group, fmt = 2816, 64, "int4"
+    cases = [S.random_w4(np.random.default_rng(s), m, n, k, group) for s in (1, 2)]
+    want = [_run(*c, group, fmt) for c in cases]
+    dev = [[to_dev(t) for t in c] for c in cases]
+    outs = [empty_dev(m * n, np.uint16) for _ in cases]
+    spaces = [A.w4_gemm_workspace(n, k, m) for _ in cases]
+    assert spaces[0] is not None
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+
+    def call(i, ws):
+        A.dispatch_w4_gemm_cols(*dev[i], outs[i], rows=n, cols=k, seq_len=m, group=group, w_format=fmt, workspace=ws)
+
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                call(i, spaces[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert np.array_equal(from_dev(outs[i], np.uint16).reshape(m, n), want[i])
+    graphs = []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(i, spaces[0])
+        graphs.append(g)
+    for i in (0, 1, 1, 0, 1):
+        outs[i].zero_()
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(from_dev(outs[i], np.uint16).reshape(m, n), want[i])
+    del graphs
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 300, 8320), (16, 65, 16384), (5, 2816, 12288), (64, 48, 32768), (2, 20000, 512), (16, 20000, 256),
+                                   (3, 6000, 8192), (90, 16, 65536), (130, 2816, 8192), (1, 3, 131072)])
+def test_long_rows_and_other_plans(m, n, k):
+    """Past the sizes of the other tests: spans of long rows, the columns between the kernels' ranges."""
+    announce(f"w4 long m={m} n={n} k={k}")
+    for group, fmt in ((32, "int4"), (128, "e2m1")):
+        _check(*S.random_w4(np.random.default_rng(m + n + k), m, n, k, group), group, fmt)
+
+
+def test_a_workspace_that_is_too_small():
+    x, codes, scales, out = (empty_dev(n, t) for n, t in ((64 * 4096, np.uint16), (2816 * 2048, np.uint8), (2816 * 128, np.uint16), (64 * 2816, np.uint16)))
+    ws = A.w4_gemm_workspace(2816, 4096, 64)
+    args = dict(rows=2816, cols=4096, seq_len=64, group=32, w_format="int4")
+    A.dispatch_w4_gemm_cols(x, codes, scales, out, workspace=ws, **args)
+    for bad in (None, ws[:-1], ws[1:]):
+        with pytest.raises(InfernoHipError):
+            A.dispatch_w4_gemm_cols(x, codes, scales, out, workspace=bad, **args)
