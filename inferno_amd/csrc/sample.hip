@@ -556,22 +556,8 @@ struct Crossing {
   }
 };
 
-// Descending, in place.  Each entry counts those above it.
-template <int kT>
-__device__ __forceinline__ void sort_descending(unsigned long long* v, unsigned long long* tmp, int n) {
-  for (int i = threadIdx.x; i < n; i += kT) {
-    const unsigned long long mine = v[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += v[j] > mine;
-    tmp[rank] = mine;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kT) v[i] = tmp[i];
-  __syncthreads();
-}
-
 constexpr int kMaxBand = 11264;
-constexpr int kMaxEqual = 1024;  // equal logits at the cut of a wide row
+constexpr int kMaxEqual = 1024;  // entries of a fine bin of the band: about as many equal logits
 constexpr uint32_t kInfKey = 0xFF800000u;  // of +inf
 
 // A row without a top-k that keeps very many tokens: one pass over its logits.
@@ -579,7 +565,7 @@ constexpr uint32_t kInfKey = 0xFF800000u;  // of +inf
 // min-p alone: the pass adds the weights of the kept ones by sub-chunk.  top-p: first a sample (about
 // 16,000 of the logits, evenly spread) says where the weights below add up to about 1 - top_p of all;
 // those are many small ones, so a sample of them is good to a few percent.  Tokens above that
-// band go to the sums, those within it to a list, in which the cut is then found from its keys' bits.
+// band go to the sums, those within it to a list, in which the cut is then found.
 // False if it is not there (or the list is full, or very many are equal): the caller descends.
 //
 // A CU takes 2 us for each instruction on all of 2^18 logits, so the pass does little for each:
@@ -603,7 +589,7 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
   const double floor_w = static_cast<double>(asked.min_p);
   // Bins of (zmax - z) * per, of which `above` is the first of the band; logits from z_from on are looked at.
   float per, z_from;
-  int above;
+  int above, end = 0;  // of the band's bins
   double goal = 0.0;  // in units
   if (nucleus) {
     goal = static_cast<double>(asked.top_p) * total * w.unit;
@@ -652,7 +638,7 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
     if (after < rest_u - slack) atomicMin(&s_b, tid);
     __syncthreads();
     above = s_a;
-    const int end = max(s_a, s_b) + 1;
+    end = max(s_a, s_b) + 1;
     if (end >= kBand) return false;
     z_from = zmax - static_cast<float>(end) / per;
   } else {
@@ -741,49 +727,49 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
   if (tid == kThreads - 1) s_u64 = above_incl;
   __syncthreads();
   const int listed = s_n;
+  const double mass_above = static_cast<double>(s_u64);
+  __syncthreads();
   uint32_t cut_key = 0, cut_index = 0xFFFFFFFFu;  // kept: above the key, or it up to that index
   if (nucleus) {
     if (listed > kMaxBand) return false;
-    const double left = __builtin_ceil(goal - static_cast<double>(s_u64));
+    const double left = __builtin_ceil(goal - mass_above);
     if (!(left >= 1.0)) return false;  // the cut lies above the band
     const unsigned long long target = static_cast<unsigned long long>(left);
-    uint32_t prefix = 0;
-    unsigned long long ahead = 0;
-    for (int level = 0; level < 3; ++level) {
-      const int lo = level == 0 ? 21 : level == 1 ? 10 : 0;
-      const int width = level == 2 ? 10 : 11;
-      for (int b = tid; b < kBins; b += kThreads) digits[b] = 0;
-      __syncthreads();
-      for (int i = tid; i < listed; i += kThreads) {
-        const uint32_t key = static_cast<uint32_t>(band[i] >> 32);
-        if (level > 0 && (key >> (lo + width)) != prefix) continue;
-        atomicAdd(&digits[(key >> lo) & ((1u << width) - 1)], w.fixed(key));
-      }
-      if (tid == 0) found->bin = kBins;
-      __syncthreads();
-      const Found f = find_from_top(digits, target - ahead, waves, found);
-      if (f.bin == kBins) return false;  // the cut lies below the band
-      ahead += f.above;
-      prefix = (prefix << width) | f.bin;
-    }
-    // Of the tokens of that key the lowest indexes, as many as it takes.
-    const unsigned long long each = w.fixed(prefix);
-    const unsigned long long ties = (target - ahead + each - 1) / each;
-    if (tid == 0) s_n = 0;
+    // Finer bins of the band, the highest for its top; then the entries of the one bin by themselves.
+    const float fine = static_cast<float>(kBins) / static_cast<float>(end - above);
+    auto bin_of = [&](unsigned long long e) {
+      const float x = (zmax - logit_of(static_cast<uint32_t>(e >> 32))) * per - static_cast<float>(above);
+      return kBins - 1 - min(max(static_cast<int>(x * fine), 0), kBins - 1);
+    };
+    for (int b = tid; b < kBins; b += kThreads) digits[b] = 0;
+    if (tid == 0) found->bin = kBins, s_n = 0;
     __syncthreads();
     for (int i = tid; i < listed; i += kThreads)
-      if (static_cast<uint32_t>(band[i] >> 32) == prefix) {
+      atomicAdd(&digits[bin_of(band[i])], w.fixed(static_cast<uint32_t>(band[i] >> 32)));
+    __syncthreads();
+    const Found f = find_from_top(digits, target, waves, found);
+    if (f.bin == kBins) return false;  // the cut lies below the band
+    unsigned long long* weights = digits;
+    for (int i = tid; i < listed; i += kThreads)
+      if (bin_of(band[i]) == static_cast<int>(f.bin)) {
         const int slot = atomicAdd(&s_n, 1);
-        if (slot < kMaxEqual) digits[slot] = band[i];
+        if (slot < kMaxEqual) {
+          order[slot] = band[i];
+          weights[slot] = w.fixed(static_cast<uint32_t>(band[i] >> 32));
+        }
       }
     __syncthreads();
     const int equal = s_n;
-    __syncthreads();
     if (equal > kMaxEqual) return false;
-    sort_descending<kThreads>(digits, order, equal);
-    cut_key = prefix;
-    cut_index = 0xFFFFFFFFu - static_cast<uint32_t>(
-        digits[min(static_cast<int>(ties), equal) - 1]);
+    if (tid < equal) {
+      const unsigned long long mine = order[tid];
+      unsigned long long sum = f.above;
+      for (int j = 0; j < equal; ++j) sum += order[j] > mine ? weights[j] : 0;
+      if (sum < target && target <= sum + weights[tid]) s_u64 = mine;
+    }
+    __syncthreads();
+    cut_key = static_cast<uint32_t>(s_u64 >> 32);
+    cut_index = 0xFFFFFFFFu - static_cast<uint32_t>(s_u64);
     __syncthreads();
   }
   for (int i = tid; i < min(listed, kMaxBand); i += kThreads) {
@@ -1053,7 +1039,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
       __syncthreads();
       const int bin = s_at, count = s_num;
       if (bin >= 0) {
-        if (count <= 2 * want + 64) {
+        if (count <= min(2 * want + 64, 1536)) {
           uint32_t least = 0xFFFFFFFFu;
 #pragma unroll
           for (int j = 0; j < PER; ++j)

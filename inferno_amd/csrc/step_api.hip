@@ -30,6 +30,17 @@ int32_t launched(hipError_t err, const char* what) {
   return ifr::abi_ok();
 }
 
+// A buffer of a call; no two of which one is written may share memory.
+struct Span {
+  const void* at;
+  int64_t bytes;
+};
+bool overlap(Span a, Span b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  if (!a.at || !b.at || a.bytes <= 0 || b.bytes <= 0) return false;
+  return x < y ? y - x < static_cast<uint64_t>(a.bytes) : x - y < static_cast<uint64_t>(b.bytes);
+}
+
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 hipStream_t as_stream(uint64_t s) { return reinterpret_cast<hipStream_t>(static_cast<uintptr_t>(s)); }
 
@@ -72,6 +83,12 @@ int32_t ifr_dispatch_w4_gemm_cols(const void* x, const void* codes, const void* 
   const int64_t need = ifr::w4_gemm_workspace_bytes(seq_len, rows, cols);
   if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
     return fail(IFR_ESPACE, "workspace needs %lld bytes, 16-byte aligned", (long long)need);
+  const Span out{output, 2 * seq_len * rows}, space{need > 0 ? workspace : nullptr, need};
+  for (const Span in : {Span{x, 2 * seq_len * cols}, Span{codes, rows * (cols / 2)},
+                        Span{scales, 2 * rows * (cols / group)}})
+    if (overlap(out, in) || overlap(space, in))
+      return fail(IFR_EINVAL, "output or workspace overlaps an input");
+  if (overlap(out, space)) return fail(IFR_EINVAL, "output overlaps the workspace");
   const ifr::W4Args a{static_cast<const uint16_t*>(x), static_cast<const uint8_t*>(codes),
                       static_cast<const uint16_t*>(scales), static_cast<uint16_t*>(output),
                       static_cast<float*>(workspace), workspace_bytes, seq_len, rows, cols,
@@ -102,8 +119,15 @@ int32_t ifr_norm_residual(const void* y, const void* residual, void* residual_ou
   for (const void* p : {y, residual, static_cast<const void*>(residual_out),
                         static_cast<const void*>(x_out), post_weight, gate, pre_weight})
     if (!aligned(p, 16)) return fail(IFR_EINVAL, "every pointer must be 16-byte aligned");
-  if (x_out == residual_out || x_out == residual || residual_out == y)
-    return fail(IFR_EINVAL, "x_out and residual_out overlap, or an output its other input");
+  const int64_t n = seq_len * hidden, res = residual_type == IFR_RESIDUAL_F32 ? 4 * n : 2 * n;
+  const Span r_out{residual_out, res}, xs{x_out, 2 * n}, ys{y, 2 * n}, rs{residual, res};
+  // In place, from its start, each output may be the input that it follows.
+  if (overlap(r_out, xs) || overlap(r_out, ys) || overlap(xs, rs) ||
+      (residual_out != residual && overlap(r_out, rs)) || (x_out != y && overlap(xs, ys)))
+    return fail(IFR_EINVAL, "x_out and residual_out overlap, or an output another input than its own");
+  const Span gates{gate, 2 * ((gate_stride ? (seq_len - 1) * gate_stride : 0) + hidden)};
+  for (const Span in : {gates, Span{post_weight, 2 * hidden}, Span{pre_weight, 2 * hidden}})
+    if (overlap(r_out, in) || overlap(xs, in)) return fail(IFR_EINVAL, "an output overlaps a gate or weight");
   const ifr::NormResidualArgs a{static_cast<const uint16_t*>(y), residual, residual_out,
                                 static_cast<uint16_t*>(x_out),
                                 static_cast<const uint16_t*>(post_weight),
@@ -141,6 +165,14 @@ int32_t ifr_dispatch_sample_tokens(const void* logits, const float* uniform, int
   const int64_t need = ifr::sample_workspace_bytes(num_rows, vocab);
   if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
     return fail(IFR_ESPACE, "workspace needs %lld bytes, 16-byte aligned", (long long)need);
+  const Span out{tokens, 4 * num_rows}, space{need > 0 ? workspace : nullptr, need};
+  const int64_t size = logits_type == IFR_LOGITS_F32 ? 4 : 2;
+  for (const Span in : {Span{logits, size * ((num_rows - 1) * row_stride + vocab)}, Span{uniform, 4 * num_rows},
+                        Span{temperature, 4 * num_rows}, Span{top_k, 4 * num_rows}, Span{top_p, 4 * num_rows},
+                        Span{min_p, 4 * num_rows}})
+    if (overlap(out, in) || overlap(space, in))
+      return fail(IFR_EINVAL, "tokens or workspace overlap an input");
+  if (overlap(out, space)) return fail(IFR_EINVAL, "tokens overlap the workspace");
   const ifr::SampleArgs a{logits, row_stride, logits_type == IFR_LOGITS_F32, temperature, top_k,
                           top_p, min_p, uniform, tokens, num_rows, vocab, workspace};
   return launched(ifr::launch_sample(a, as_stream(stream)), "sample_tokens");

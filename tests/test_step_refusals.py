@@ -6,11 +6,15 @@ import pytest
 from inferno_amd import _lib
 
 EINVAL, ESPACE = -1, -4
-P = 1 << 20  # an address that is 16-byte aligned and never read
+P = 1 << 40  # addresses that are 16-byte aligned, far apart and never read
+
+
+def at(i):
+    return P * (i + 1)
 
 
 def w4(**kw):
-    a = dict(x=P, codes=P, scales=P, output=P, rows=64, cols=256, seq_len=4, group=32, w_format=1, workspace=None,
+    a = dict(x=P, codes=at(1), scales=at(2), output=at(3), rows=64, cols=256, seq_len=4, group=32, w_format=1, workspace=None,
              workspace_bytes=0)
     a.update(kw)
     return _lib.lib().ifr_dispatch_w4_gemm_cols(*a.values(), 0)
@@ -19,7 +23,10 @@ def w4(**kw):
 @pytest.mark.parametrize("bad", [dict(rows=0), dict(rows=-1), dict(rows=(1 << 24) + 1), dict(cols=0), dict(cols=192), dict(cols=1 << 21),
                                  dict(seq_len=-1), dict(seq_len=(1 << 19) + 1), dict(group=16), dict(group=0), dict(group=256),
                                  dict(w_format=0), dict(w_format=3), dict(x=None), dict(codes=None), dict(scales=None), dict(output=None),
-                                 dict(x=P + 2), dict(codes=P + 8), dict(scales=P + 4), dict(output=P + 2)])
+                                 dict(x=P + 2), dict(codes=P + 8), dict(scales=P + 4), dict(output=P + 2),
+                                 dict(output=P), dict(output=P + 2032), dict(output=P - 496), dict(output=at(1) + 8176), dict(output=at(2) + 16),
+                                 dict(rows=2816, cols=4096, seq_len=64, workspace=at(3) + 16, workspace_bytes=1 << 40),
+                                 dict(rows=2816, cols=4096, seq_len=64, workspace=at(1) + 16, workspace_bytes=1 << 40)])
 def test_w4_refuses(bad):
     assert w4(**bad) == EINVAL, _lib.last_error()
 
@@ -38,9 +45,9 @@ def test_w4_workspace_too_small():
             need = size(rows, cols, m)
             assert 0 <= need <= 64 * rows * m * 4 and need % 4 == 0
             if need:
-                assert w4(rows=rows, cols=cols, seq_len=m, workspace=P, workspace_bytes=need - 1) == ESPACE
+                assert w4(rows=rows, cols=cols, seq_len=m, workspace=at(4), workspace_bytes=need - 1) == ESPACE
                 assert w4(rows=rows, cols=cols, seq_len=m, workspace=None, workspace_bytes=need) == ESPACE
-                assert w4(rows=rows, cols=cols, seq_len=m, workspace=P + 4, workspace_bytes=need) == ESPACE
+                assert w4(rows=rows, cols=cols, seq_len=m, workspace=at(4) + 4, workspace_bytes=need) == ESPACE
 
 
 def norm(**kw):
@@ -55,7 +62,9 @@ def norm(**kw):
                                  dict(eps=float("nan")), dict(eps=float("inf")), dict(gate=P, gate_stride=8), dict(gate=P, gate_stride=68),
                                  dict(gate=P, gate_stride=-64), dict(y=None), dict(residual=None), dict(residual_out=None), dict(y=P + 2),
                                  dict(residual=P + 8), dict(gate=P + 4), dict(post=P + 2), dict(pre=P + 2), dict(x_out=2 * P), dict(x_out=3 * P),
-                                 dict(residual_out=P)])
+                                 dict(residual_out=P), dict(residual_out=2 * P + 16), dict(x_out=P + 16), dict(x_out=P - 16),
+                                 dict(gate=3 * P), dict(post=4 * P + 16), dict(pre=3 * P + 496), dict(residual_out=P + 496),
+                                 dict(gate=5 * P, gate_stride=P, seq_len=2, residual_out=6 * P + 112)])
 def test_norm_refuses(bad):
     assert norm(**bad) == EINVAL, _lib.last_error()
 
@@ -65,15 +74,16 @@ def test_norm_nothing_to_do():
 
 
 def sample(**kw):
-    a = dict(logits=P, uniform=P, tokens=P, temperature=None, top_k=None, top_p=None, min_p=None, rows=4, vocab=100, stride=100, kind=1,
-             workspace=P, workspace_bytes=1 << 40)
+    a = dict(logits=P, uniform=at(1), tokens=at(2), temperature=None, top_k=None, top_p=None, min_p=None, rows=4, vocab=100, stride=100, kind=1,
+             workspace=at(3), workspace_bytes=1 << 40)
     a.update(kw)
     return _lib.lib().ifr_dispatch_sample_tokens(*a.values(), 0)
 
 
 @pytest.mark.parametrize("bad", [dict(rows=-1), dict(rows=(1 << 20) + 1), dict(vocab=0), dict(vocab=(1 << 20) + 1, stride=1 << 21), dict(stride=99),
                                  dict(stride=(1 << 32) + 1), dict(kind=2), dict(logits=None), dict(uniform=None), dict(tokens=None), dict(logits=P + 2),
-                                 dict(logits=P + 1, kind=0), dict(uniform=P + 1), dict(top_k=P + 2), dict(min_p=P + 2)])
+                                 dict(logits=P + 1, kind=0), dict(uniform=P + 1), dict(top_k=P + 2), dict(min_p=P + 2), dict(tokens=P + 1584), dict(tokens=at(1) + 8),
+                                 dict(min_p=at(2)), dict(workspace=P + 16), dict(workspace=at(2)), dict(top_k=at(3) + 16)])
 def test_sample_refuses(bad):
     assert sample(**bad) == EINVAL, _lib.last_error()
 
