@@ -15,7 +15,8 @@
 // workgroup a row, which in most cases reads a few of those 64 again and is done:
 //  - without any limit, the sums give the 64 tokens in which the draw lands;
 //  - a top-k of up to 1,024: the k-th largest of the 64s' largest is at most the k-th largest
-//    logit, so the candidates are the tokens above it, little more than k, which are sorted;
+//    logit, so the candidates are the tokens above it, little more than k, and histograms of them
+//    say where the cuts and the draw lie (Crossing);
 //  - top-p alone: the same with 128 and then 1,024, if the cut lies above; min-p alone has its
 //    threshold.
 // The third, with a larger workgroup a row, takes the rows that are left: a cut among very many
@@ -312,132 +313,150 @@ __device__ __forceinline__ double uniform_of(const SampleArgs& a, int64_t row) {
   return u > 0.0f ? (u < 1.0f ? static_cast<double>(u) : 1.0 - 0x1p-24) : 0.0;
 }
 
-// The row by its keys' bits.
-template <bool kF32>
-__device__ __forceinline__ void sample_descent(const SampleArgs& a, int shift, int64_t row,
-                                            uint32_t top, unsigned long long* bins,
-                                            uint32_t* tie_counts, unsigned long long* waves,
-                                            Found* found_at) {
-  Found& found = *found_at;
-  const Asked asked(a, row);
-  const int vocab = static_cast<int>(a.vocab);
-  const void* z = static_cast<const char*>(a.logits) + row * a.row_stride * (kF32 ? 4 : 2);
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int64_t k = asked.k;
-  const float top_p = asked.top_p, min_p = asked.min_p;
-  int valid = 0;
-  for (int i = tid; i < vocab; i += kThreads) valid += key_of(load_logit<kF32>(z, i)) != 0;
-  unsigned long long count = block_inclusive<unsigned long long>(valid, waves);
-  if (tid == kThreads - 1) found.above = count;
-  __syncthreads();
-  count = found.above;
-  __syncthreads();
-  const Weights w{top, static_cast<double>(logit_of(top)), asked.rate(),
-                  static_cast<double>(1ull << shift)};
+// One lane's atomic for the wave where all its lanes have one bin and weight, as in a row of few
+// different logits: 64 atomics at one address run one after the other.
+__device__ __forceinline__ void add_to_bin(unsigned long long* bins, int bin, unsigned long long v) {
+  if (!v) return;
+  const int one = uniform_i32(bin);
+  const unsigned long long here = __ballot(true), same = __ballot(bin == one);
+  if (here != same) {
+    atomicAdd(&bins[bin], v);
+    return;
+  }
+  const uint32_t low = uniform_i32(static_cast<int>(v)), high = uniform_i32(static_cast<int>(v >> 32));
+  const unsigned long long first = (static_cast<unsigned long long>(high) << 32) | low;
+  if (__ballot(v == first) == here) {  // equal weights too
+    if (__lane_id() == __ffsll(here) - 1) atomicAdd(&bins[bin], first * __popcll(here));
+  } else {
+    atomicAdd(&bins[bin], v);
+  }
+}
 
-  // Keys of `digit` bits at a time: the histogram of value(key) over the keys that
-  // agree with `prefix` above the digit.
-  Cut cut{1, count};  // key 1 stands for no logit: everything that can be drawn
-  auto descend = [&](unsigned long long target, auto value) {
+// The row by its keys' bits: a pass over it for each of the three digits of each cut, and one for the
+// draw.  What bounds it is the one CU's instructions on every logit of each pass: 217 us for a top-k of 1,025
+// of 2^18 f32 logits, 473 for a top-p of 0.5 of as many equal ones (318 and 958 with one load ahead).
+template <bool kF32>
+__device__ __forceinline__ void sample_descent(const SampleArgs& a, int64_t row, const RowView<kF32>& view,
+                                               const Asked& asked, const Weights& w, int num_subs,
+                                               unsigned long long* bins, uint32_t* tie_counts,
+                                               unsigned long long* waves, Found* found) {
+  constexpr int kPer = RowView<kF32>::kPer;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int vectors = num_subs * kSub / kPer;
+  __shared__ unsigned long long s_total;
+  // visit(keys, first place) for every vector of the row, in no order.
+  auto each_vector = [&](auto visit) {
+    constexpr int kAhead = 4;
+    for (int v0 = tid; v0 - tid < vectors; v0 += kAhead * kThreads) {
+      uint4 raw[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) raw[i] = view.raw(min(v0 + i * kThreads, vectors) * kPer);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        float z[kPer];
+        RowView<kF32>::unpack(raw[i], z);
+        uint32_t key[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) key[j] = v0 + i * kThreads < vectors ? key_of(z[j]) : 0;
+        visit(key, (v0 + i * kThreads) * kPer);
+      }
+    }
+  };
+  auto sum_of_all = [&](unsigned long long mine) {
+    const unsigned long long incl = block_inclusive<unsigned long long>(mine, waves);
+    if (tid == kThreads - 1) s_total = incl;
+    __syncthreads();
+    const unsigned long long all = s_total;
+    __syncthreads();
+    return all;
+  };
+  // The key in which the sum of value(key), from the largest key on, reaches target_of(the sum of
+  // all), and the sum above that key; key 0 if the target is 0.
+  auto descend = [&](auto value, auto target_of) {
     uint32_t prefix = 0;
-    unsigned long long above = 0;
+    unsigned long long above = 0, target = 0;
     for (int level = 0; level < 3; ++level) {
       const int lo = level == 0 ? 21 : level == 1 ? 10 : 0;
       const int width = level == 2 ? 10 : 11;
       for (int b = tid; b < kBins; b += kThreads) bins[b] = 0;
       __syncthreads();
-      for (int i = tid; i < vocab; i += kThreads) {
-        const uint32_t key = key_of(load_logit<kF32>(z, i));
-        if (key == 0 || (level > 0 && (key >> (lo + width)) != prefix)) continue;
-        const unsigned long long v = value(key);
-        if (v) atomicAdd(&bins[(key >> lo) & ((1u << width) - 1)], v);
-      }
+      each_vector([&](const uint32_t (&key)[kPer], int) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (key[j] != 0 && (level == 0 || (key[j] >> (lo + width)) == prefix))
+            add_to_bin(bins, (key[j] >> lo) & ((1u << width) - 1), value(key[j]));
+      });
       __syncthreads();
-      const Found f = find_from_top(bins, target - above, waves, found_at);
+      if (level == 0) {
+        target = target_of(sum_of_all(bins[2 * tid] + bins[2 * tid + 1]));
+        if (target == 0) return Found{0, 0};  // block-uniform
+      }
+      const Found f = find_from_top(bins, target - above, waves, found);
       above += f.above;
       prefix = (prefix << width) | f.bin;
-      __syncthreads();
     }
     return Found{prefix, above};
   };
-  if (k > 0 && static_cast<unsigned long long>(k) < count) {
-    const Found f = descend(static_cast<unsigned long long>(k),
-                            [](uint32_t) -> unsigned long long { return 1; });
-    cut = {f.bin, static_cast<unsigned long long>(k) - f.above};
+  Cut cut{1, 0};  // key 1 stands for no logit: everything that can be drawn
+  if (asked.k > 0) {
+    const unsigned long long k = static_cast<unsigned long long>(asked.k);
+    const Found f = descend([](uint32_t) { return 1ull; },
+                            [&](unsigned long long alive) { return k < alive ? k : 0; });
+    if (f.bin) cut = {f.bin, k - f.above};
   }
-  // The kept ties of the top-k cut, all of one weight, count as one sum behind the rest.
-  if (top_p < 1.0f) {
-    const unsigned long long tie = w.fixed(cut.key);
-    auto value = [&](uint32_t key) -> unsigned long long {
-      return key > cut.key ? w.fixed(key) : 0;
-    };
-    unsigned long long mine = 0;
-    for (int i = tid; i < vocab; i += kThreads) {
-      const uint32_t key = key_of(load_logit<kF32>(z, i));
-      if (key) mine += value(key);
-    }
-    mine = block_inclusive<unsigned long long>(mine, waves);
-    if (tid == kThreads - 1) found.above = mine;
-    __syncthreads();
-    const unsigned long long strict = found.above;
-    __syncthreads();
-    const unsigned long long total = strict + cut.ties * tie;
-    const double want = __builtin_ceil(static_cast<double>(top_p) * static_cast<double>(total));
-    unsigned long long target = want < 1.0 ? 1 : static_cast<unsigned long long>(want);
-    target = target < total ? target : total;
-    if (target > strict) {  // within the ties of the top-k cut
-      cut.ties = (target - strict + tie - 1) / tie;
-    } else {
-      const Found f = descend(target, value);
+  if (asked.top_p < 1.0f) {
+    // The kept ties of the top-k cut, all of one weight, count as one sum behind the rest.
+    const unsigned long long tie = cut.ties ? w.fixed(cut.key) : 0;
+    unsigned long long target = 0;
+    bool in_ties = false;
+    const Found f = descend([&](uint32_t key) { return key > cut.key ? w.fixed(key) : 0; },
+                            [&](unsigned long long strict) {
+      const unsigned long long all = strict + cut.ties * tie;
+      const double want = __builtin_ceil(static_cast<double>(asked.top_p) * static_cast<double>(all));
+      target = want < 1.0 ? 1 : static_cast<unsigned long long>(want);
+      target = target < all ? target : all;
+      in_ties = target > strict;
+      if (in_ties) cut.ties = (target - strict + tie - 1) / tie;
+      return in_ties ? 0ull : target;
+    });
+    if (!in_ties) {
       const unsigned long long each = w.fixed(f.bin);
       cut = {f.bin, (target - f.above + each - 1) / each};
     }
   }
 
-  // By index: the weight and the ties of each sub-chunk of 2^sub tokens.
-  int sub = 8;
-  while (((vocab - 1) >> sub) + 1 > kMaxSubs) ++sub;
-  const int subs = ((vocab - 1) >> sub) + 1;
-  const double floor_w = static_cast<double>(min_p);
+  // By place: the weight and the ties of each of up to kMaxSubs parts of the row.
+  int part = 6;  // log2 of a part's places
+  while (((num_subs * kSub - 1) >> part) + 1 > kMaxSubs) ++part;
+  const double floor_w = static_cast<double>(asked.min_p);
   auto kept = [&](uint32_t key) -> unsigned long long {
-    if (key == 0) return 0;
     const double v = w.real(key);
-    return v >= floor_w || key == top ? w.units(v) : 0;
+    return v >= floor_w || key == w.top ? w.units(v) : 0;
   };
   const unsigned long long tie = kept(cut.key);
-  for (int s = tid; s < kMaxSubs; s += kThreads)
-    if (s >= subs) {
-      bins[s] = 0;
-      tie_counts[s] = 0;
-    }
-  for (int s = tid >> 6; s < subs; s += kThreads / 64) {
+  __syncthreads();
+  for (int s = tid; s < kMaxSubs; s += kThreads) bins[s] = 0, tie_counts[s] = 0;
+  __syncthreads();
+  each_vector([&](const uint32_t (&key)[kPer], int place) {
     unsigned long long sum = 0;
     uint32_t ties = 0;
-    const int end = min(vocab, (s + 1) << sub);
-    for (int i = (s << sub) + lane; i < end; i += 64) {
-      const uint32_t key = key_of(load_logit<kF32>(z, i));
-      if (key > cut.key) sum += kept(key);
-      ties += key == cut.key;
-    }
 #pragma unroll
-    for (int d = 32; d > 0; d /= 2) {
-      sum += __shfl_xor(sum, d);
-      ties += __shfl_xor(ties, d);
+    for (int j = 0; j < kPer; ++j) {
+      if (key[j] > cut.key) sum += kept(key[j]);
+      ties += key[j] == cut.key;
     }
-    if (lane == 0) {
-      bins[s] = sum;
-      tie_counts[s] = ties;
-    }
-  }
+    if (sum) atomicAdd(&bins[place >> part], sum);
+    if (ties) atomicAdd(&tie_counts[place >> part], ties);
+  });
   __syncthreads();
-  // Thread t has sub-chunks 4t .. 4t + 3.
-  constexpr int kPer = kMaxSubs / kThreads;
+  // Thread t has parts 4t .. 4t + 3.
+  constexpr int kEach = kMaxSubs / kThreads;
   unsigned long long ties = 0, sum = 0;
-  for (int j = 0; j < kPer; ++j) ties += tie_counts[kPer * tid + j];
-  unsigned long long ties_before = block_inclusive<unsigned long long>(ties, waves) - ties;
+  for (int j = 0; j < kEach; ++j) ties += tie_counts[kEach * tid + j];
+  const unsigned long long ties_before = block_inclusive<unsigned long long>(ties, waves) - ties;
   unsigned long long first_ties = ties_before;
-  for (int j = 0; j < kPer; ++j) {
-    const int s = kPer * tid + j;
+  for (int j = 0; j < kEach; ++j) {
+    const int s = kEach * tid + j;
     const unsigned long long left = first_ties < cut.ties ? cut.ties - first_ties : 0;
     const unsigned long long here = tie_counts[s] < left ? tie_counts[s] : left;
     first_ties += tie_counts[s];
@@ -445,21 +464,20 @@ __device__ __forceinline__ void sample_descent(const SampleArgs& a, int shift, i
     sum += bins[s];
   }
   const unsigned long long incl = block_inclusive<unsigned long long>(sum, waves);
-  if (tid == kThreads - 1) found.above = incl;
+  if (tid == kThreads - 1) s_total = incl;
   __syncthreads();
-  const unsigned long long total = found.above;
-  __syncthreads();
+  const unsigned long long total = s_total;
   unsigned long long goal = static_cast<unsigned long long>(uniform_of(a, row) * static_cast<double>(total));
   if (goal >= total) goal = total - 1;  // total >= 1: the largest logit is kept
-  __shared__ int s_sub;
+  __shared__ int s_part;
   __shared__ unsigned long long s_before, s_ties;
   if (incl - sum <= goal && goal < incl) {
     unsigned long long before = incl - sum;
     unsigned long long ties_at = ties_before;
-    for (int j = 0; j < kPer; ++j) {
-      const int s = kPer * tid + j;
+    for (int j = 0; j < kEach; ++j) {
+      const int s = kEach * tid + j;
       if (goal < before + bins[s]) {
-        s_sub = s;
+        s_part = s;
         s_before = before;
         s_ties = ties_at;
         break;
@@ -471,23 +489,16 @@ __device__ __forceinline__ void sample_descent(const SampleArgs& a, int shift, i
   __syncthreads();
   if (tid >= 64) return;
   unsigned long long before = s_before, ties_at = s_ties;
-  const int end = min(vocab, (s_sub + 1) << sub);
-  for (int i0 = s_sub << sub; i0 < end; i0 += 64) {
-    const int i = i0 + lane;
-    const uint32_t key = i < end ? key_of(load_logit<kF32>(z, i)) : 0;
-    const unsigned long long is_tie = __ballot(key == cut.key && key != 0);
-    const unsigned long long order =
-        ties_at + __popcll(is_tie & ((1ull << lane) - 1));
-    unsigned long long v = key > cut.key ? kept(key) : key == cut.key && order < cut.ties ? tie : 0;
-    if (key == 0) v = 0;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const unsigned long long o = __shfl_up(v, d);
-      if (lane >= d) v += o;
-    }
+  const int end = (s_part + 1) << part;
+  for (int p0 = s_part << part; p0 < end; p0 += 64) {
+    const uint32_t key = view.key(p0 + lane);
+    const unsigned long long is_tie = __ballot(key == cut.key);
+    const unsigned long long order = ties_at + __popcll(is_tie & ((1ull << lane) - 1));
+    const unsigned long long v = wave_inclusive(
+        key > cut.key ? kept(key) : key == cut.key && order < cut.ties ? tie : 0);
     const unsigned long long hit = __ballot(before + v > goal);
     if (hit) {
-      if (lane == 0) a.tokens[row] = i0 + static_cast<int>(__ffsll(hit)) - 1;
+      if (lane == 0) a.tokens[row] = p0 + static_cast<int>(__ffsll(hit)) - 1 - view.shift;
       return;
     }
     before += __shfl(v, 63);
@@ -851,7 +862,7 @@ __global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a, int
   if (asked.k == 0 && mine.top != kInfKey &&
       sample_wide<kF32>(a, row, view, asked, w, mine.total, num_subs, bins, digits, band, waves, &found))
     return;
-  sample_descent<kF32>(a, shift, row, mine.top, bins, reinterpret_cast<uint32_t*>(digits), waves, &found);
+  sample_descent<kF32>(a, row, view, asked, w, num_subs, bins, reinterpret_cast<uint32_t*>(digits), waves, &found);
 }
 
 // The first thread by number whose condition holds, or else the last whose `or_else` does.
