@@ -19,10 +19,11 @@
 //    say where the cuts and the draw lie (Crossing);
 //  - top-p alone: the same with 128 and then 1,024, if the cut lies above; min-p alone has its
 //    threshold.
-// The third, with a larger workgroup a row, takes the rows that are left: a cut among very many
-// tokens in one pass (sample_wide), a larger top-k or very many equal logits by descending
-// through the keys, 11, 11 and 10 bits at a time, in histograms of counts or weights of the row.
-#include <type_traits>
+// The third, with larger workgroups, takes the rows that are left: a cut among very many tokens in one
+// pass (sample_wide), in parts of the row where there are few rows; a larger top-k or very many equal
+// logits by descending through the keys, 11, 11 and 10 bits at a time, in histograms of counts or
+// weights of the row.
+#include <algorithm>
 
 #include "common.hpp"
 #include "step.hpp"
@@ -571,6 +572,24 @@ constexpr int kMaxBand = 11264;
 constexpr int kMaxEqual = 1024;  // entries of a fine bin of the band: about as many equal logits
 constexpr uint32_t kInfKey = 0xFF800000u;  // of +inf
 
+// What the second launch leaves for the third.
+struct RowRest {
+  double total;     // the sum of the row's weights, if it has one
+  uint32_t top;     // its largest key
+  uint32_t is_left;
+  // Of the parts of a row: the weights above the band, the entries of the band, parts that are done.
+  unsigned long long above;
+  uint32_t listed, done;
+};
+
+// A row in parts, of whole groups of sub-chunks; the last one to end joins them.
+struct Parts {
+  int count, mine;
+  RowRest* rest;
+  unsigned long long* band;      // [kMaxBand]
+  unsigned long long* sub_sums;  // [kMaxSubs]
+};
+
 // A row without a top-k that keeps very many tokens: one pass over its logits.
 //
 // min-p alone: the pass adds the weights of the kept ones by sub-chunk.  top-p: first a sample (about
@@ -584,9 +603,9 @@ constexpr uint32_t kInfKey = 0xFF800000u;  // of +inf
 template <bool kF32>
 __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, const RowView<kF32>& view,
                                          const Asked& asked, const Weights& w, double total,
-                                         int num_subs, unsigned long long* sub_sums,
+                                         int num_subs, const Parts& parts, unsigned long long* sub_sums,
                                          unsigned long long* digits, unsigned long long* band,
-                                         unsigned long long* waves, Found* found) {
+                                         unsigned long long* waves, Found* found, bool* joined) {
   unsigned long long* queues = digits;  // between the two uses of the digits
   __shared__ unsigned long long order[kMaxEqual];
   constexpr int kPer = RowView<kF32>::kPer;
@@ -690,8 +709,8 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
     }
     head += n;
   };
-  auto push = [&](float z, int place) {
-    const bool in = z >= z_from;
+  auto push = [&](float z, float from, int place) {
+    const bool in = z >= from;
     const unsigned long long m = __ballot(in);
     if (!m) return;
     if (in)
@@ -702,44 +721,75 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
     __builtin_amdgcn_wave_barrier();
     if (tail - head >= 64) take(64);
   };
+  const int groups = ((num_subs - 1) >> group) + 1;
+  const int first_group = static_cast<int>(static_cast<int64_t>(groups) * parts.mine / parts.count);
+  const int end_group = static_cast<int>(static_cast<int64_t>(groups) * (parts.mine + 1) / parts.count);
+  const int v_first = max(view.first_full(), (first_group << group) * (kSub / kPer));
+  const int v_end = min(view.end_full(), (end_group << group) * (kSub / kPer));
   // (Few loads ahead: each place where the queue is emptied is a copy of that code, and 32 and more
   // of them no longer fit the instruction cache.)
   constexpr int kAhead = kF32 ? 4 : 2;
-  const int v_first = view.first_full(), v_end = view.end_full();
-  const int rounds = max(v_end - v_first, 0) / (kAhead * kThreads);  // of vectors that all threads have
-  const int v_rest = v_first + rounds * kAhead * kThreads;
-  if (rounds > 0) {
+  if (v_first < v_end) {
     uint4 next[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) next[i] = view.full(v_first + tid + i * kThreads);
-    for (int v = v_first + tid; v < v_rest; v += kAhead * kThreads) {
+    for (int i = 0; i < kAhead; ++i) next[i] = view.full(min(v_first + tid + i * kThreads, v_end - 1));
+    for (int v = v_first + tid; v - tid < v_end; v += kAhead * kThreads) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
+        const int at = v + i * kThreads;
+        const float from = at < v_end ? z_from : __builtin_inff();  // no logit here is +inf
         float z[kPer];
         RowView<kF32>::split(next[i], z);
-        next[i] = view.full(min(v + (i + kAhead) * kThreads, v_end - 1));
+        next[i] = view.full(min(at + kAhead * kThreads, v_end - 1));
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) push(z[j], (v + i * kThreads) * kPer + j);
+        for (int j = 0; j < kPer; ++j) push(z[j], from, at * kPer + j);
       }
     }
   }
-#pragma unroll 1
-  for (int p = v_rest * kPer; p < v_end * kPer; p += kThreads)
-    push(p + tid < v_end * kPer ? load_logit<kF32>(view.z, p + tid - view.shift) : -__builtin_inff(),
-         p + tid);
-  if (wave == 0) {  // the ends: less than two vectors
-    const int place = lane < kPer ? lane : max(v_end, v_first) * kPer + lane - kPer;
-    const bool end = lane < kPer ? v_first > 0 : lane < 2 * kPer;
+  if (wave == 0) {  // the row's ends: less than two vectors
+    const int row_end = max(view.end_full(), view.first_full()) * kPer;
+    const int place = lane < kPer ? lane : row_end + lane - kPer;
+    const bool end = lane < kPer ? parts.mine == 0 && view.first_full() > 0
+                                 : parts.mine == parts.count - 1 && lane < 2 * kPer;
     const uint32_t key = end ? view.key(place) : 0;
-    push(key ? logit_of(key) : -__builtin_inff(), place);
+    push(key ? logit_of(key) : -__builtin_inff(), z_from, place);
   }
   take(tail - head);
   const unsigned long long above_incl = block_inclusive<unsigned long long>(my_above, waves);
   if (tid == kThreads - 1) s_u64 = above_incl;
   __syncthreads();
-  const int listed = s_n;
-  const double mass_above = static_cast<double>(s_u64);
+  int listed = s_n;
+  unsigned long long sum_above = s_u64;
   __syncthreads();
+  if (parts.count > 1) {
+    if (tid == 0) {
+      s_a = static_cast<int>(atomicAdd(&parts.rest->listed, static_cast<uint32_t>(listed)));
+      atomicAdd(&parts.rest->above, sum_above);
+    }
+    __syncthreads();
+    const int slot = s_a;
+    for (int i = tid; i < min(listed, kMaxBand - slot); i += kThreads) parts.band[slot + i] = band[i];
+    for (int i = first_group + tid; i < end_group; i += kThreads) parts.sub_sums[i] = sub_sums[i];
+    __syncthreads();
+    // All that this workgroup wrote is seen by the one that counts last.
+    if (tid == 0)
+      s_b = __hip_atomic_fetch_add(&parts.rest->done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+            static_cast<uint32_t>(parts.count - 1);
+    __syncthreads();
+    if (!s_b) return true;  // block-uniform
+    if (tid == 0) {
+      s_n = static_cast<int>(__hip_atomic_load(&parts.rest->listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+      s_u64 = __hip_atomic_load(&parts.rest->above, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    listed = s_n;
+    sum_above = s_u64;
+    for (int i = tid; i < min(listed, kMaxBand); i += kThreads) band[i] = parts.band[i];
+    for (int i = tid; i < groups; i += kThreads) sub_sums[i] = parts.sub_sums[i];
+    __syncthreads();
+  }
+  *joined = true;
+  const double mass_above = static_cast<double>(sum_above);
   uint32_t cut_key = 0, cut_index = 0xFFFFFFFFu;  // kept: above the key, or it up to that index
   if (nucleus) {
     if (listed > kMaxBand) return false;
@@ -836,32 +886,31 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
   }
 }
 
-// What the second launch leaves for the third.
-struct RowRest {
-  double total;     // the sum of the row's weights, if it has one
-  uint32_t top;     // its largest key
-  uint32_t is_left;
-};
-
 template <bool kF32>
-__global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a, int shift,
-                                                               const RowRest* __restrict__ rest,
+__global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a, int shift, RowRest* rest,
+                                                               unsigned long long* joins, int num_parts,
                                                                int num_subs) {
   __shared__ unsigned long long bins[kMaxSubs];
   __shared__ unsigned long long digits[kBins];
   __shared__ unsigned long long band[kMaxBand];
   __shared__ unsigned long long waves[kThreads / 64];
   __shared__ Found found;
-  const int64_t row = blockIdx.x;
-  const RowRest mine = rest[row];
-  if (!mine.is_left) return;  // block-uniform
+  const int64_t row = blockIdx.x / static_cast<unsigned>(num_parts);
+  if (!rest[row].is_left) return;  // block-uniform
   const Asked asked(a, row);
   const RowView<kF32> view(a, row);
-  const Weights w{mine.top, static_cast<double>(logit_of(mine.top)), asked.rate(),
+  const uint32_t top = rest[row].top;
+  const Weights w{top, static_cast<double>(logit_of(top)), asked.rate(),
                   static_cast<double>(1ull << shift)};
-  if (asked.k == 0 && mine.top != kInfKey &&
-      sample_wide<kF32>(a, row, view, asked, w, mine.total, num_subs, bins, digits, band, waves, &found))
+  unsigned long long* join = joins + row * (kMaxBand + kMaxSubs);
+  const Parts parts{num_parts, static_cast<int>(blockIdx.x - row * num_parts), rest + row, join, join + kMaxBand};
+  // What sample_wide finds before its parts join is the same in all of them.
+  const bool wide = asked.k == 0 && top != kInfKey;
+  bool joined = false;
+  if (wide && sample_wide<kF32>(a, row, view, asked, w, rest[row].total, num_subs, parts, bins, digits, band,
+                                waves, &found, &joined))
     return;
+  if (!joined && parts.mine != 0) return;
   sample_descent<kF32>(a, row, view, asked, w, num_subs, bins, reinterpret_cast<uint32_t*>(digits), waves, &found);
 }
 
@@ -1005,7 +1054,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
   }
 
   auto leave = [&]() {
-    if (tid == 0) rest[row] = {total, top, 1};
+    if (tid == 0) rest[row] = {total, top, 1, 0, 0, 0};
   };
   if (asked.k > kMaxK) return leave();
   const float zmax = logit_of(top), zlow = logit_of(low);
@@ -1244,6 +1293,14 @@ int weight_shift(int64_t vocab) {
   return bits < 11 ? 51 : 62 - bits;
 }
 
+// Workgroups of a row in the third launch: for up to 128 rows the CUs that would be idle otherwise, with
+// 64 sub-chunks or more each.  For rows of 2^18 f32 logits of which tens of thousands are kept, all three
+// launches: 102 -> 58 us (top-p) and 46 -> 24 us (min-p) for one row, 128 -> 108 and 94 -> 79 us for 64.
+int64_t rest_parts(int64_t rows, int64_t vocab) {
+  const int64_t fill = std::min<int64_t>(256 / std::max<int64_t>(rows, 1), 8);
+  return std::max<int64_t>(std::min(fill, vocab / (64 * kSub)), 1);
+}
+
 int64_t sub_chunks(int64_t vocab) { return (vocab + 7 + kSub - 1) / kSub; }
 
 template <bool kF32>
@@ -1251,7 +1308,9 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
   const int subs = static_cast<int>(sub_chunks(a.vocab));
   double* sums = static_cast<double*>(a.workspace);
   RowRest* rest = reinterpret_cast<RowRest*>(sums + a.rows * subs);
-  uint32_t* tops = reinterpret_cast<uint32_t*>(rest + a.rows);
+  const int parts = static_cast<int>(rest_parts(a.rows, a.vocab));
+  unsigned long long* joins = reinterpret_cast<unsigned long long*>(rest + a.rows);
+  uint32_t* tops = reinterpret_cast<uint32_t*>(joins + (parts > 1 ? a.rows * (kMaxBand + kMaxSubs) : 0));
   constexpr int kChunk = kScanThreads * kScanVectors * RowView<kF32>::kPer;
   const int chunks = (subs * kSub + kChunk - 1) / kChunk;
   hipLaunchKernelGGL(sample_scan_kernel<kF32>, dim3(static_cast<unsigned>(a.rows * chunks)),
@@ -1270,15 +1329,17 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
                        sums, rest, subs);
   err = hipGetLastError();
   if (err != hipSuccess) return err;
-  hipLaunchKernelGGL(sample_rest_kernel<kF32>, grid, dim3(kThreads), 0, stream, a,
-                     weight_shift(a.vocab), rest, subs);
+  hipLaunchKernelGGL(sample_rest_kernel<kF32>, dim3(static_cast<unsigned>(a.rows * parts)), dim3(kThreads), 0,
+                     stream, a, weight_shift(a.vocab), rest, joins, parts, subs);
   return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t sample_workspace_bytes(int64_t rows, int64_t vocab) {
-  return (rows * (sub_chunks(vocab) * 12 + static_cast<int64_t>(sizeof(RowRest))) + 15) / 16 * 16;
+  // For up to 128 rows in parts also where there are more, so that a workspace does for fewer rows.
+  const int64_t join = rest_parts(1, vocab) > 1 ? std::min<int64_t>(rows, 128) * (kMaxBand + kMaxSubs) * 8 : 0;
+  return (rows * (sub_chunks(vocab) * 12 + static_cast<int64_t>(sizeof(RowRest))) + join + 15) / 16 * 16;
 }
 
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {

@@ -300,6 +300,19 @@ def test_candidates_among_equal_logits(f32):
            rng.random(8), f32)
 
 
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("rows,vocab", [(1, 40003), (3, 8191), (5, 12289), (70, 40003), (128, 9000), (129, 9000)])
+def test_rows_that_keep_many_among_few_and_many_rows(rows, vocab, f32):
+    """The workgroups that share a row number from one to eight, by the rows and the vocabulary."""
+    announce(f"sample parts rows={rows} vocab={vocab} f32={f32}")
+    rng = np.random.default_rng(rows)
+    z = rng.standard_normal((rows, vocab)) * 0.7
+    z[1::4] = np.sort(z[1::4], axis=1)  # all that is kept in one part
+    z[2::4, 5:] = -np.inf               # and in the first places
+    asked = [[(1.0, 0, 0.9, 0.0), (1.0, 0, 1.0, 1e-3), (0.8, 0, 0.97, 1e-3), (1.0, 5000, 0.9, 0.0)][(r // 4) % 4] for r in range(rows)]
+    _check(z, asked, rng.random(rows), f32, pad=3, offset=1)
+
+
 def test_calls_at_once_and_graphs_that_share_a_workspace():
     import torch
 
