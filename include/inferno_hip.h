@@ -495,11 +495,12 @@ int32_t ifr_kv8_attention(const void* image_dev, const int64_t* info, const void
  * scales [rows][cols / group] bf16, any numbers.  v: IFR_W4_INT4 -8 to 7 in two's
  * complement; IFR_W4_E2M1 0, 0.5, 1, 1.5, 2, 3, 4, 6 and, from code 8, their negatives.
  * Sums are f32, and nothing is rounded before the output; their order depends on
- * seq_len, and where a workspace is used, on its size.  A token's results depend on
- * its own x alone, so infinities and NaN stay in their token.
+ * seq_len.  A token's results depend on its own x alone, so infinities and NaN stay in
+ * their token.
  * group 32, 64 or 128; cols a multiple of 128; any rows.  All pointers 16-byte aligned.
- * workspace: device memory of ifr_w4_gemm_workspace_bytes (0: null will do), written
- * before it is read in every call; calls that may overlap each need their own. */
+ * workspace: device memory of ifr_w4_gemm_workspace_bytes (0: null will do; that of a
+ * seq_len does for all below it), written before it is read in every call; calls that may
+ * overlap each need their own. */
 #define IFR_W4_INT4 1
 #define IFR_W4_E2M1 2
 int64_t ifr_w4_gemm_workspace_bytes(int64_t rows, int64_t cols, int64_t seq_len);
@@ -548,8 +549,8 @@ int32_t ifr_norm_residual(const void* y, const void* residual, void* residual_ou
  * Logits of +inf share the draw.
  * logits [num_rows][row_stride] of logits_type, of which vocab (1 to 2^20) are read;
  * num_rows up to 2^20.  workspace: device memory of ifr_sample_workspace_bytes, 16-byte
- * aligned (0: null will do), written before it is read in every call; calls that may
- * overlap each need their own. */
+ * aligned (0: null will do; that of num_rows does for all below it), written before it is
+ * read in every call; calls that may overlap each need their own. */
 #define IFR_LOGITS_BF16 0
 #define IFR_LOGITS_F32 1
 int64_t ifr_sample_workspace_bytes(int64_t num_rows, int64_t vocab);

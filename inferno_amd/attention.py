@@ -462,7 +462,7 @@ def _tensor(device: int, name: str, t, numel: int, kind: frozenset) -> int:
 
 
 def w4_gemm_workspace(rows: int, cols: int, seq_len: int, device="cuda"):
-    """f32 workspace for dispatch_w4_gemm_cols at this shape (None if unneeded)."""
+    """f32 workspace for dispatch_w4_gemm_cols at this shape and up to that seq_len (None if unneeded)."""
     import torch
 
     n = lib().ifr_w4_gemm_workspace_bytes(rows, cols, seq_len)
@@ -529,7 +529,8 @@ def dispatch_norm_residual(y, residual, residual_out, x_out=None, *, hidden: int
 
 
 def sample_workspace(num_rows: int, vocab: int, device="cuda"):
-    """Workspace for dispatch_sample_tokens at this shape (None if unneeded)."""
+    """Workspace for dispatch_sample_tokens at this vocab and up to that num_rows (None if
+    unneeded)."""
     import torch
 
     n = lib().ifr_sample_workspace_bytes(num_rows, vocab)

@@ -16,7 +16,6 @@ struct W4Args {
   const uint16_t* scales;  // [N][K / group] bf16
   uint16_t* out;           // [M][N] bf16
   float* workspace;
-  int64_t workspace_bytes;
   int64_t M, N, K;
   int group, format;
 };

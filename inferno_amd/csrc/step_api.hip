@@ -91,7 +91,7 @@ int32_t ifr_dispatch_w4_gemm_cols(const void* x, const void* codes, const void* 
   if (overlap(out, space)) return fail(IFR_EINVAL, "output overlaps the workspace");
   const ifr::W4Args a{static_cast<const uint16_t*>(x), static_cast<const uint8_t*>(codes),
                       static_cast<const uint16_t*>(scales), static_cast<uint16_t*>(output),
-                      static_cast<float*>(workspace), workspace_bytes, seq_len, rows, cols,
+                      static_cast<float*>(workspace), seq_len, rows, cols,
                       static_cast<int>(group), static_cast<int>(w_format)};
   return launched(ifr::launch_w4_gemm(a, as_stream(stream)), "w4_gemm_cols");
 }

@@ -756,15 +756,19 @@ constexpr int64_t kManyColumns = 32768;
 // has several at once, 23 or 43; spans add a launch and the partial sums' way out and back.
 // It picks the best measured or one within 12 % of it: 65 tokens 15.1 us (best 13.4), 256 20.4
 // (19.6), 512 28.0 (28.0; one span of 128 tokens 48.3), 1,024 43.4 (43.4).
+// Spans only up to 768 workgroups, which bounds the workspace for every M.
+constexpr int kTileSpans = 16;
+constexpr int64_t kTileBlocks = 768;
 Plan tile_plan(int64_t M, int64_t N, int steps) {
   Plan best{kTile, 2, 4, 1, steps};
   double best_us = 1e30;
   for (int mb = 1; mb <= 2; ++mb) {
     const int64_t tiles = ceil_div(M, 64 * mb) * ceil_div(N, kTileN);
-    for (int want = 1; want <= 16 && (want == 1 || steps >= 4 * want); ++want) {
+    for (int want = 1; want <= kTileSpans && (want == 1 || steps >= 4 * want); ++want) {
       const int span = static_cast<int>(ceil_div(steps, want));
       const int splits = static_cast<int>(ceil_div(steps, span));
       const int64_t blocks = tiles * splits;
+      if (splits > 1 && blocks > kTileBlocks) break;
       const double tile = blocks <= 256 ? (mb == 1 ? 33.0 : 45.0)
                                         : (mb == 1 ? 23.0 : 43.0) * static_cast<double>(ceil_div(blocks, 256));
       double us = 2.5 + tile * span / 32.0;
@@ -896,9 +900,18 @@ hipError_t launch_format(const W4Args& a, hipStream_t stream) {
 
 }  // namespace
 
+// For every number of tokens up to M: exact for each kind of plan up to 64, beyond the bound that
+// kTileBlocks sets (of tiles of 128 x 128).
 int64_t w4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  const Plan p = plan_of(M, N, K);
-  return p.splits > 1 ? p.splits * part_stride(M, N) * 4 : 0;
+  int64_t floats = 0;
+  for (const int64_t up_to : {16, 32, 64}) {
+    const int64_t m = std::min(M, up_to);
+    const Plan p = plan_of(m, N, K);
+    if (p.splits > 1) floats = std::max(floats, p.splits * part_stride(m, N));
+  }
+  if (M > 64 && K / 128 >= 8 && 2 * ceil_div(N, kTileN) <= kTileBlocks)
+    floats = std::max(floats, std::min(kTileSpans * part_stride(M, N), kTileBlocks * 128 * kTileN));
+  return floats * 4;
 }
 
 hipError_t launch_w4_gemm(const W4Args& a, hipStream_t stream) {

@@ -38,6 +38,18 @@ def test_w4_nothing_to_do():
     assert [size(0, 256, 1), size(64, 100, 1), size(64, 256, -1), size(64, 256, 1 << 20)] == [-1] * 4
 
 
+def test_a_workspace_does_for_fewer_tokens_and_rows():
+    size = _lib.lib().ifr_w4_gemm_workspace_bytes
+    for rows, cols in ((2816, 4096), (2816, 8192), (64, 65536), (33000, 4096), (262144, 2816), (512, 1024), (100, 128)):
+        sizes = [size(rows, cols, m) for m in [*range(0, 1300), *range(1300, 20000, 61)]]
+        assert sizes == sorted(sizes)
+        assert sizes[-1] <= 64 << 20
+    size = _lib.lib().ifr_sample_workspace_bytes
+    for vocab in (1, 8191, 8192, 262144, 1 << 20):
+        sizes = [size(rows, vocab) for rows in range(0, 600)]
+        assert sizes == sorted(sizes)
+
+
 def test_w4_workspace_too_small():
     size = _lib.lib().ifr_w4_gemm_workspace_bytes
     for rows, cols in ((2816, 8192), (64, 65536), (272, 4096)):
