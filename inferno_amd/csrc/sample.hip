@@ -20,9 +20,9 @@
 //  - top-p alone: the same with 128 and then 1,024, if the cut lies above; min-p alone has its
 //    threshold.
 // The third, with larger workgroups, takes the rows that are left: a cut among very many tokens in one
-// pass (sample_wide), in parts of the row where there are few rows; a larger top-k or very many equal
-// logits by descending through the keys, 11, 11 and 10 bits at a time, in histograms of counts or
-// weights of the row.
+// pass (sample_wide), in parts of the row where few are left; a larger top-k or very many equal logits
+// by descending through the keys, 11, 11 and 10 bits at a time, in histograms of counts or weights of
+// the row.
 #include <algorithm>
 
 #include "common.hpp"
@@ -258,10 +258,11 @@ constexpr int kScanVectors = 4;      // of a thread
 // subs[row][s]: the largest key of sub-chunk s; sums[row][s]: its weights relative to that key.
 template <bool kF32>
 __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleArgs a, uint32_t* subs,
-                                                                   double* sums, int num_subs,
-                                                                   int chunks) {
+                                                                   double* sums, uint32_t* num_left,
+                                                                   int num_subs, int chunks) {
   constexpr int kPer = RowView<kF32>::kPer;
   constexpr int kLanes = kSub / kPer;  // of a sub-chunk
+  if (blockIdx.x == 0 && threadIdx.x == 0) *num_left = 0;  // for the second launch
   const int64_t row = blockIdx.x / static_cast<unsigned>(chunks);
   const int chunk = static_cast<int>(blockIdx.x - row * chunks);
   const RowView<kF32> view(a, row);
@@ -574,13 +575,14 @@ constexpr uint32_t kInfKey = 0xFF800000u;  // of +inf
 
 // What the second launch leaves for the third.
 struct RowRest {
-  double total;     // the sum of the row's weights, if it has one
-  uint32_t top;     // its largest key
-  uint32_t is_left;
-  // Of the parts of a row: the weights above the band, the entries of the band, parts that are done.
+  double total;  // the sum of the row's weights, if it has one
+  uint32_t top;  // its largest key
+  // Of the parts of a row: parts that are done, entries of the band, the weights above it.
+  uint32_t done, listed;
   unsigned long long above;
-  uint32_t listed, done;
 };
+
+constexpr uint32_t kJoinRows = 128;  // that may be in parts
 
 // A row in parts, of whole groups of sub-chunks; the last one to end joins them.
 struct Parts {
@@ -593,7 +595,7 @@ struct Parts {
 // A row without a top-k that keeps very many tokens: one pass over its logits.
 //
 // min-p alone: the pass adds the weights of the kept ones by sub-chunk.  top-p: first a sample (about
-// 16,000 of the logits, evenly spread) says where the weights below add up to about 1 - top_p of all;
+// 16,000 of the logits, lines of 128 bytes evenly spread) says where the weights below add up to about 1 - top_p of all;
 // those are many small ones, so a sample of them is good to a few percent.  Tokens above that
 // band go to the sums, those within it to a list, in which the cut is then found.
 // False if it is not there (or the list is full, or very many are equal): the caller descends.
@@ -616,6 +618,7 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
   const int vectors = num_subs * kSub / kPer;
   const float zmax = logit_of(w.top);
   const bool nucleus = asked.top_p < 1.0f;
+  const float rate = static_cast<float>(w.rate);
   const double floor_w = static_cast<double>(asked.min_p);
   // Bins of (zmax - z) * per, of which `above` is the first of the band; logits from z_from on are looked at.
   float per, z_from;
@@ -624,27 +627,36 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
   if (nucleus) {
     goal = static_cast<double>(asked.top_p) * total * w.unit;
     const double rest = (1.0 - static_cast<double>(asked.top_p)) * total;
-    // Tokens of less than rest / vocab add up to less than rest: the cut is above.
-    const double depth = -log2(rest / static_cast<double>(view.vocab)) / w.rate;
-    if (!(depth > 0.0 && depth < 1e30)) return false;
-    per = static_cast<float>((kBand - 1) / depth);
+    // Tokens of less than rest / vocab add up to less than rest: the cut is above.  (f32 will do for
+    // what the band is found by.)
+    const float depth = -__builtin_amdgcn_logf(static_cast<float>(rest) / static_cast<float>(view.vocab)) / rate;
+    if (!(depth > 0.0f && depth < 1e30f)) return false;
+    per = static_cast<float>(kBand - 1) / depth;
     if (!(per > 0.0f && per < 1e30f)) return false;
     for (int i = tid; i < kBins; i += kThreads) digits[i] = 0;
     __syncthreads();
     const int stride = max(1, vectors / (16384 / kPer));
     unsigned long long tail_sum = 0;  // of the last bin
-    for (int v = tid * stride; v < vectors; v += kThreads * stride) {
-      float z[kPer];
-      view.logits(v * kPer, z);
+    constexpr int kLoads = 16 / kPer;  // all of most threads'
+    // Whole lines of 128 bytes, one of `stride`.
+    auto sampled = [&](int i) { return i / 8 * (8 * stride) + i % 8; };
+    for (int i0 = tid; sampled(i0) < vectors; i0 += kLoads * kThreads) {
+      uint4 raw[kLoads];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const double wz = exp2_neg((static_cast<double>(z[j]) - w.zmax) * w.rate);
-        const unsigned long long f = w.units(wz);
-        const float x = (zmax - z[j]) * per;
-        if (x < kBand - 1)
-          atomicAdd(&digits[static_cast<int>(x)], f);
-        else
-          tail_sum += f;  // what lies below the looked-at bins
+      for (int i = 0; i < kLoads; ++i) raw[i] = view.raw(min(sampled(i0 + i * kThreads), vectors) * kPer);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        float z[kPer];
+        RowView<kF32>::unpack(raw[i], z);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const float x = zmax - z[j];
+          const unsigned long long f = w.units(static_cast<double>(__builtin_amdgcn_exp2f(-x * rate)));
+          if (x * per < kBand - 1)
+            atomicAdd(&digits[static_cast<int>(x * per)], f);
+          else
+            tail_sum += f;  // what lies below the looked-at bins
+        }
       }
     }
     tail_sum = wave_inclusive(tail_sum);
@@ -660,8 +672,9 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
     const double seen = static_cast<double>(s_u64);
     const double below = (seen - (incl - mine)) * stride, after = (seen - incl) * stride;
     const double rest_u = rest * w.unit;
-    const double weight = exp2_neg(-static_cast<double>(tid) / per * w.rate) * w.unit;
-    const double slack = stride == 1 ? 0.0 : 2.5 * sqrt(stride * weight * rest_u) + rest_u / 128.0;
+    const float weight = __builtin_amdgcn_exp2f(-static_cast<float>(tid) / per * rate) * static_cast<float>(w.unit);
+    const float spread = stride == 1 ? 0.0f : 2.5f * (sqrtf(static_cast<float>(stride) * weight) * sqrtf(static_cast<float>(rest_u)));
+    const double slack = static_cast<double>(spread) + rest_u / 128.0;
     // The band: from the last bin above which too little can be cut off, to the first below which
     // too much would be.
     if (below > rest_u + slack) atomicMax(&s_a, tid);
@@ -886,24 +899,32 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
   }
 }
 
+// left[0]: how many rows are left; left[1 ..]: which, in no order.  Where the grid has several workgroups
+// for each, they take parts of it.
 template <bool kF32>
 __global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a, int shift, RowRest* rest,
-                                                               unsigned long long* joins, int num_parts,
+                                                               const uint32_t* __restrict__ left,
+                                                               unsigned long long* joins, int max_parts,
                                                                int num_subs) {
   __shared__ unsigned long long bins[kMaxSubs];
   __shared__ unsigned long long digits[kBins];
   __shared__ unsigned long long band[kMaxBand];
   __shared__ unsigned long long waves[kThreads / 64];
   __shared__ Found found;
-  const int64_t row = blockIdx.x / static_cast<unsigned>(num_parts);
-  if (!rest[row].is_left) return;  // block-uniform
+  const uint32_t num_left = left[0];
+  const uint32_t num_parts =
+      num_left > kJoinRows ? 1 : min(static_cast<uint32_t>(max_parts), gridDim.x / max(num_left, 1u));
+  const uint32_t slot = blockIdx.x / num_parts;
+  if (slot >= num_left) return;  // block-uniform
+  const int64_t row = left[1 + slot];
   const Asked asked(a, row);
   const RowView<kF32> view(a, row);
   const uint32_t top = rest[row].top;
   const Weights w{top, static_cast<double>(logit_of(top)), asked.rate(),
                   static_cast<double>(1ull << shift)};
-  unsigned long long* join = joins + row * (kMaxBand + kMaxSubs);
-  const Parts parts{num_parts, static_cast<int>(blockIdx.x - row * num_parts), rest + row, join, join + kMaxBand};
+  unsigned long long* join = joins + static_cast<int64_t>(slot) * (kMaxBand + kMaxSubs);
+  const Parts parts{static_cast<int>(num_parts), static_cast<int>(blockIdx.x - slot * num_parts), rest + row, join,
+                    join + kMaxBand};
   // What sample_wide finds before its parts join is the same in all of them.
   const bool wide = asked.k == 0 && top != kInfKey;
   bool joined = false;
@@ -930,7 +951,7 @@ __device__ __forceinline__ int first_thread(bool holds, bool or_else, int* first
 template <bool kF32, int PER>
 __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
     SampleArgs a, const uint32_t* __restrict__ subs, const double* __restrict__ sums,
-    RowRest* __restrict__ rest, int num_subs) {
+    RowRest* __restrict__ rest, uint32_t* left, int num_subs) {
   constexpr int kWaves = kPickThreads / 64;
   constexpr int kPickBins = 2 * kPickThreads;
   constexpr int kEach = kMaxTaken / kPickThreads;  // entries of a thread
@@ -989,10 +1010,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
     __syncthreads();
     if (wave == 0) {
       const unsigned long long m = top ? __ballot(view.key(s_at * kSub + lane) == top) : 0;
-      if (lane == 0) {
-        a.tokens[row] = top ? s_at * kSub + __ffsll(m) - 1 - view.shift : -1;
-        rest[row].is_left = 0;
-      }
+      if (lane == 0) a.tokens[row] = top ? s_at * kSub + __ffsll(m) - 1 - view.shift : -1;
     }
     return;
   }
@@ -1046,15 +1064,15 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
     const unsigned long long hit = __ballot(v > 0.0 && sum > s_sum);
     const unsigned long long any = __ballot(v > 0.0);
     const int l = hit ? __ffsll(hit) - 1 : 63 - __clzll(any);
-    if (lane == 0) {
-      a.tokens[row] = s_num * kSub + l - view.shift;
-      rest[row].is_left = 0;
-    }
+    if (lane == 0) a.tokens[row] = s_num * kSub + l - view.shift;
     return;
   }
 
   auto leave = [&]() {
-    if (tid == 0) rest[row] = {total, top, 1, 0, 0, 0};
+    if (tid == 0) {
+      rest[row] = {total, top, 0, 0, 0};
+      left[1 + atomicAdd(&left[0], 1u)] = static_cast<uint32_t>(row);
+    }
   };
   if (asked.k > kMaxK) return leave();
   const float zmax = logit_of(top), zlow = logit_of(low);
@@ -1280,10 +1298,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
         const unsigned long long goal = static_cast<unsigned long long>(u * static_cast<double>(listed));
         return min(goal, listed - 1) + 1;
       });
-  if (tid == 0) {
-    a.tokens[row] = static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(drawn));
-    rest[row].is_left = 0;
-  }
+  if (tid == 0) a.tokens[row] = static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(drawn));
 }
 
 // Bits of the integers that stand for weights of at most 1: sums of a row stay below 2^63.
@@ -1293,53 +1308,57 @@ int weight_shift(int64_t vocab) {
   return bits < 11 ? 51 : 62 - bits;
 }
 
-// Workgroups of a row in the third launch: for up to 128 rows the CUs that would be idle otherwise, with
-// 64 sub-chunks or more each.  For rows of 2^18 f32 logits of which tens of thousands are kept, all three
-// launches: 102 -> 58 us (top-p) and 46 -> 24 us (min-p) for one row, 128 -> 108 and 94 -> 79 us for 64.
-int64_t rest_parts(int64_t rows, int64_t vocab) {
-  const int64_t fill = std::min<int64_t>(256 / std::max<int64_t>(rows, 1), 8);
-  return std::max<int64_t>(std::min(fill, vocab / (64 * kSub)), 1);
-}
+// Workgroups of the third launch: as many as rows, or the 256 CUs with up to eight a row, each of 64
+// sub-chunks or more.  Of a batch few rows are left for it: 42 of 256 rows of 2^18 under a top-p of 0.95, which take
+// 44 us in six parts each (the workgroups start and sample for 12, pass for 8, meet for 10 and cut and draw for 8)
+// where a workgroup each took 75; and for one such row all three launches take 58 us where they took 102.
+int64_t rest_parts(int64_t vocab) { return std::clamp<int64_t>(vocab / (64 * kSub), 1, 8); }
+int64_t rest_blocks(int64_t rows, int64_t vocab) { return std::max(rows, std::min<int64_t>(rows * rest_parts(vocab), 256)); }
 
 int64_t sub_chunks(int64_t vocab) { return (vocab + 7 + kSub - 1) / kSub; }
+
+// Where the parts of a row meet.
+int64_t join_longs(int64_t rows, int64_t vocab) {
+  return rest_parts(vocab) > 1 ? std::min<int64_t>(rows, kJoinRows) * (kMaxBand + kMaxSubs) : 0;
+}
 
 template <bool kF32>
 hipError_t launch(const SampleArgs& a, hipStream_t stream) {
   const int subs = static_cast<int>(sub_chunks(a.vocab));
   double* sums = static_cast<double*>(a.workspace);
   RowRest* rest = reinterpret_cast<RowRest*>(sums + a.rows * subs);
-  const int parts = static_cast<int>(rest_parts(a.rows, a.vocab));
+  const int parts = static_cast<int>(rest_parts(a.vocab));
   unsigned long long* joins = reinterpret_cast<unsigned long long*>(rest + a.rows);
-  uint32_t* tops = reinterpret_cast<uint32_t*>(joins + (parts > 1 ? a.rows * (kMaxBand + kMaxSubs) : 0));
+  uint32_t* left = reinterpret_cast<uint32_t*>(joins + join_longs(a.rows, a.vocab));
+  uint32_t* tops = left + 1 + a.rows;
   constexpr int kChunk = kScanThreads * kScanVectors * RowView<kF32>::kPer;
   const int chunks = (subs * kSub + kChunk - 1) / kChunk;
   hipLaunchKernelGGL(sample_scan_kernel<kF32>, dim3(static_cast<unsigned>(a.rows * chunks)),
-                     dim3(kScanThreads), 0, stream, a, tops, sums, subs, chunks);
+                     dim3(kScanThreads), 0, stream, a, tops, sums, left, subs, chunks);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   const dim3 grid(static_cast<unsigned>(a.rows));
   if (subs <= kPickThreads)
     hipLaunchKernelGGL((sample_pick_kernel<kF32, 1>), grid, dim3(kPickThreads), 0, stream, a, tops,
-                       sums, rest, subs);
+                       sums, rest, left, subs);
   else if (subs <= 9 * kPickThreads)
     hipLaunchKernelGGL((sample_pick_kernel<kF32, 9>), grid, dim3(kPickThreads), 0, stream, a, tops,
-                       sums, rest, subs);
+                       sums, rest, left, subs);
   else
     hipLaunchKernelGGL((sample_pick_kernel<kF32, 33>), grid, dim3(kPickThreads), 0, stream, a, tops,
-                       sums, rest, subs);
+                       sums, rest, left, subs);
   err = hipGetLastError();
   if (err != hipSuccess) return err;
-  hipLaunchKernelGGL(sample_rest_kernel<kF32>, dim3(static_cast<unsigned>(a.rows * parts)), dim3(kThreads), 0,
-                     stream, a, weight_shift(a.vocab), rest, joins, parts, subs);
+  hipLaunchKernelGGL(sample_rest_kernel<kF32>, dim3(static_cast<unsigned>(rest_blocks(a.rows, a.vocab))),
+                     dim3(kThreads), 0, stream, a, weight_shift(a.vocab), rest, left, joins, parts, subs);
   return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t sample_workspace_bytes(int64_t rows, int64_t vocab) {
-  // For up to 128 rows in parts also where there are more, so that a workspace does for fewer rows.
-  const int64_t join = rest_parts(1, vocab) > 1 ? std::min<int64_t>(rows, 128) * (kMaxBand + kMaxSubs) * 8 : 0;
-  return (rows * (sub_chunks(vocab) * 12 + static_cast<int64_t>(sizeof(RowRest))) + join + 15) / 16 * 16;
+  return (rows * (sub_chunks(vocab) * 12 + static_cast<int64_t>(sizeof(RowRest)) + 4) + 4 +
+          join_longs(rows, vocab) * 8 + 15) / 16 * 16;
 }
 
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {

@@ -313,6 +313,18 @@ def test_rows_that_keep_many_among_few_and_many_rows(rows, vocab, f32):
     _check(z, asked, rng.random(rows), f32, pad=3, offset=1)
 
 
+@pytest.mark.parametrize("rows,every", [(300, 3), (300, 60), (40, 13)])
+def test_a_few_rows_that_keep_many_in_a_batch(rows, every):
+    """The rows that the third launch takes are dealt to its workgroups by how many there are."""
+    announce(f"sample few left rows={rows} every={every}")
+    rng = np.random.default_rng(every)
+    vocab = 20001
+    z = rng.standard_normal((rows, vocab)) * 0.7
+    wide = [(1.0, 0, 0.9, 0.0), (1.0, 0, 1.0, 1e-3), (0.8, 0, 0.97, 1e-3), (1.0, 5000, 0.9, 0.0)]
+    asked = [wide[(r // every) % 4] if r % every == every - 1 else (0.0, 0, 1.0, 0.0) if r % 2 else OFF for r in range(rows)]
+    _check(z, asked, rng.random(rows), True)
+
+
 def test_calls_at_once_and_graphs_that_share_a_workspace():
     import torch
 
