@@ -256,6 +256,9 @@ constexpr int kScanThreads = 256;
 constexpr int kScanVectors = 4;      // of a thread
 
 // subs[row][s]: the largest key of sub-chunk s; sums[row][s]: its weights relative to that key.
+// 16 lanes (f32) or 8 (bf16) have a sub-chunk, one load of 16 bytes each, four sub-chunks after each other.
+// Without sums it is bound by its loads; with them, by some 20 instructions in 64 bits for each logit:
+// 256 rows of 2^18 f32 logits take 84 us, 3.2 TB/s (54 at the rate of a copy), 64 mixed rows of bf16 17.
 template <bool kF32>
 __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleArgs a, uint32_t* subs,
                                                                    double* sums, uint32_t* num_left,
@@ -595,9 +598,9 @@ struct Parts {
 // A row without a top-k that keeps very many tokens: one pass over its logits.
 //
 // min-p alone: the pass adds the weights of the kept ones by sub-chunk.  top-p: first a sample (about
-// 16,000 of the logits, lines of 128 bytes evenly spread) says where the weights below add up to about 1 - top_p of all;
-// those are many small ones, so a sample of them is good to a few percent.  Tokens above that
-// band go to the sums, those within it to a list, in which the cut is then found.
+// 16,000 of the logits, lines of 128 bytes evenly spread) says where the weights below add up to about
+// 1 - top_p of all; those are many small ones, so a sample of them is good to a few percent.  Tokens
+// above that band go to the sums, those within it to a list, in which the cut is then found.
 // False if it is not there (or the list is full, or very many are equal): the caller descends.
 //
 // A CU takes 2 us for each instruction on all of 2^18 logits, so the pass does little for each:
@@ -673,7 +676,8 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
     const double below = (seen - (incl - mine)) * stride, after = (seen - incl) * stride;
     const double rest_u = rest * w.unit;
     const float weight = __builtin_amdgcn_exp2f(-static_cast<float>(tid) / per * rate) * static_cast<float>(w.unit);
-    const float spread = stride == 1 ? 0.0f : 2.5f * (sqrtf(static_cast<float>(stride) * weight) * sqrtf(static_cast<float>(rest_u)));
+    const float spread = stride == 1 ? 0.0f : 2.5f * sqrtf(static_cast<float>(stride) * weight) *
+                                                  sqrtf(static_cast<float>(rest_u));
     const double slack = static_cast<double>(spread) + rest_u / 128.0;
     // The band: from the last bin above which too little can be cut off, to the first below which
     // too much would be.
@@ -948,6 +952,10 @@ __device__ __forceinline__ int first_thread(bool holds, bool or_else, int* first
 }
 
 // One workgroup a row.  PER: sub-chunks a thread looks at.
+// A chain of short steps, each behind a barrier, and of two reads of memory: for one row of 2^18 f32 logits
+// under a top-k of 64 and a top-p the largest keys take 2.2 us, a threshold 3.5, listing and reading the
+// candidates 4.4, the three histograms of them 6.  512 threads; a row of which 1,024 sub-chunks are read takes
+// about 16 us more.
 template <bool kF32, int PER>
 __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
     SampleArgs a, const uint32_t* __restrict__ subs, const double* __restrict__ sums,
@@ -1313,7 +1321,9 @@ int weight_shift(int64_t vocab) {
 // 44 us in six parts each (the workgroups start and sample for 12, pass for 8, meet for 10 and cut and draw for 8)
 // where a workgroup each took 75; and for one such row all three launches take 58 us where they took 102.
 int64_t rest_parts(int64_t vocab) { return std::clamp<int64_t>(vocab / (64 * kSub), 1, 8); }
-int64_t rest_blocks(int64_t rows, int64_t vocab) { return std::max(rows, std::min<int64_t>(rows * rest_parts(vocab), 256)); }
+int64_t rest_blocks(int64_t rows, int64_t vocab) {
+  return std::max(rows, std::min<int64_t>(rows * rest_parts(vocab), 256));
+}
 
 int64_t sub_chunks(int64_t vocab) { return (vocab + 7 + kSub - 1) / kSub; }
 

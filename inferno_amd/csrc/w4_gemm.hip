@@ -107,32 +107,24 @@ struct StepScales {
   }
 };
 
-// sum += the step's products, TM tiles of 16 tokens.  R: the values of a lane that stand for
-// tokens (token t is row 4 (t / R) + t % R of its tile: with at most four tokens one value a
-// lane has to be scaled, not four).
-template <int kFmt, int kGroup, int TM, int R>
-__device__ __forceinline__ void multiply_step(const bf16x8_t (&xf)[TM][4], uint4 w,
-                                              const StepScales<kGroup>& s, f32x4_t (&sum)[TM]) {
+// sum += the step's products, 16 tokens.  R: the values of a lane that stand for tokens (token t
+// is row 4 (t / R) + t % R: with at most four tokens one value a lane has to be scaled, not four).
+template <int kFmt, int kGroup, int R>
+__device__ __forceinline__ void multiply_step(const bf16x8_t (&xf)[4], uint4 w,
+                                              const StepScales<kGroup>& s, f32x4_t& sum) {
   order_words<kGroup>(w);
   const uint32_t word[4] = {w.x, w.y, w.z, w.w};
   constexpr int kPer = kGroup / 32;  // words of a group
 #pragma unroll
   for (int g = 0; g < 4 / kPer; ++g) {
-    f32x4_t acc[TM];
+    f32x4_t acc{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int t = 0; t < TM; ++t) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const bf16x8_t b = w4_values<kFmt>(word[g * kPer + j]);
-#pragma unroll
-      for (int t = 0; t < TM; ++t)
-        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[t][g * kPer + j], b, acc[t], 0, 0, 0);
-    }
+    for (int j = 0; j < kPer; ++j)
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[g * kPer + j], w4_values<kFmt>(word[g * kPer + j]),
+                                                    acc, 0, 0, 0);
     const float sc = s.get(g);
 #pragma unroll
-    for (int t = 0; t < TM; ++t)
-#pragma unroll
-      for (int i = 0; i < R; ++i) sum[t][i] = __builtin_fmaf(sc, acc[t][i], sum[t][i]);
+    for (int i = 0; i < R; ++i) sum[i] = __builtin_fmaf(sc, acc[i], sum[i]);
   }
 }
 
@@ -144,6 +136,8 @@ __device__ __forceinline__ int token_of_row(int row) {
 // Up to 16 tokens and few columns: a workgroup takes `cols` columns (NT tiles of 16), its waves
 // take ST steps of k in turn, and their sums meet in LDS, added in wave order.  Every load of
 // ST steps is under way before the first product; x comes from L2.
+// Bound by latency: one token x 2,816 x 4,096 (int4, groups of 128; 6.1 MB) takes 5.1 us, one launch of
+// 256 workgroups of 11 columns whose waves have one round of loads each.
 template <int kFmt, int kGroup, int NT, int ST, int R>
 __global__ __launch_bounds__(1024) void w4_few_kernel(W4Args a, int cols) {
   __shared__ float part[16][NT * R][64];
@@ -161,13 +155,13 @@ __global__ __launch_bounds__(1024) void w4_few_kernel(W4Args a, int cols) {
     wp[t] = a.codes + n * (K / 2) + 16 * q;
     sp[t] = a.scales + n * (K / kGroup);
   }
-  f32x4_t sum[NT][1];
+  f32x4_t sum[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) sum[t][0] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t = 0; t < NT; ++t) sum[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   for (int s0 = wave * ST; s0 < steps; s0 += waves * ST) {
     uint4 w[ST][NT];
     StepScales<kGroup> sc[ST][NT];
-    bf16x8_t xf[ST][1][4];
+    bf16x8_t xf[ST][4];
 #pragma unroll
     for (int i = 0; i < ST; ++i) {
       const int s = min(s0 + i, steps - 1);
@@ -182,7 +176,7 @@ __global__ __launch_bounds__(1024) void w4_few_kernel(W4Args a, int cols) {
       const int s = min(s0 + i, steps - 1);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        xf[i][0][j] = *reinterpret_cast<const bf16x8_t*>(xp + 128 * s + x_offset<kGroup>(j, q));
+        xf[i][j] = *reinterpret_cast<const bf16x8_t*>(xp + 128 * s + x_offset<kGroup>(j, q));
     }
     __builtin_amdgcn_sched_barrier(0);  // every load ahead of the first product
 #pragma unroll
@@ -190,12 +184,12 @@ __global__ __launch_bounds__(1024) void w4_few_kernel(W4Args a, int cols) {
       if (s0 + i < steps)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-          multiply_step<kFmt, kGroup, 1, R>(xf[i], w[i][t], sc[i][t], sum[t]);
+          multiply_step<kFmt, kGroup, R>(xf[i], w[i][t], sc[i][t], sum[t]);
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int i = 0; i < R; ++i) part[wave][t * R + i][lane] = sum[t][0][i];
+    for (int i = 0; i < R; ++i) part[wave][t * R + i][lane] = sum[t][i];
   __syncthreads();
   for (int e = threadIdx.x; e < NT * R * 64; e += blockDim.x) {
     const int v = e >> 6, l = e & 63;
@@ -242,6 +236,8 @@ struct ScaleWindow {
 // Up to four tokens against many columns: a wave takes NT tiles of 16 columns over all of k, with x in
 // LDS, a chunk of k at a time, and the codes straight from memory into registers, two steps
 // ahead.
+// Bound by HBM reads: one token x 262,144 x 2,816 (int4, groups of 128) takes 66 us, 5.8 TB/s, and reads
+// 1.0 times its 381 MB.
 constexpr int kStreamWaves = 8;
 constexpr int kStreamTiles = 2;  // NT
 constexpr int kStreamLds = 56 * 1024;  // x: two workgroups a CU
@@ -285,21 +281,21 @@ __global__ __launch_bounds__(64 * kStreamWaves, 4) void w4_stream_kernel(W4Args 
   load_window(0);
   load(0);
 
-  f32x4_t sum[NT][1];
+  f32x4_t sum[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) sum[t][0] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t = 0; t < NT; ++t) sum[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   const uint8_t* xrow = xs + min(token_of_row<1>(r), M - 1) * pitch;
   auto multiply = [&](const uint4 (&now)[NT], int s, int in_chunk) {
-    bf16x8_t xf[1][4];
+    bf16x8_t xf[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      xf[0][j] = *reinterpret_cast<const bf16x8_t*>(xrow + 256 * in_chunk + 2 * x_offset<kGroup>(j, q));
+      xf[j] = *reinterpret_cast<const bf16x8_t*>(xrow + 256 * in_chunk + 2 * x_offset<kGroup>(j, q));
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       StepScales<kGroup> sc;
       sc.load(reinterpret_cast<const uint16_t*>(my_scales + t * 16 * kScalePitch +
                                                 s % Window::kSteps * Window::kStepBytes));
-      multiply_step<kFmt, kGroup, 1, 1>(xf, now[t], sc, sum[t]);
+      multiply_step<kFmt, kGroup, 1>(xf, now[t], sc, sum[t]);
     }
   };
   for (int c0 = 0; c0 < steps; c0 += chunk_steps) {
@@ -335,7 +331,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, 4) void w4_stream_kernel(W4Args 
     const int n = n0 + 16 * t + r;
     if (n < N && q < M)
       a.out[static_cast<int64_t>(q) * N + n] =
-          static_cast<uint16_t>(pack_bf16(kUnit<kFmt> * sum[t][0][0], 0.0f));
+          static_cast<uint16_t>(pack_bf16(kUnit<kFmt> * sum[t][0], 0.0f));
   }
 }
 
@@ -343,6 +339,10 @@ __global__ __launch_bounds__(64 * kStreamWaves, 4) void w4_stream_kernel(W4Args 
 // from memory into LDS by themselves (global_load_lds), one unit ahead, so that W waves of NT tiles
 // share it behind one barrier a unit.  The codes of a unit are loaded again as soon as the unit
 // before is multiplied, two units ahead of their use.
+//
+// Bound by no one part: 64 tokens x 262,143 x 2,816 (e2m1, groups of 32) takes 160 us, 2.9 TB/s, with the matrix
+// units busy for 26 %, a CU's vector instructions for about half of the time and 43 % of its waves'
+// time spent waiting; without its stores, its loads of x or its reads of LDS it takes 4 to 13 % less.
 //
 // 16-byte chunk c of x row r lies at c ^ (r % 16), so that the 16 rows of a quarter of a
 // fragment read lie in 16 different bank groups.
@@ -533,7 +533,9 @@ __global__ __launch_bounds__(256) void w4_reduce_kernel(const float* __restrict_
 // c + 2.  The weight is B (column l % 32).  Its codes come the same way, 128 k (two chunks) a
 // stage, two stages ahead, and become bf16 in registers; scales 16 bytes a row at a time.  Straight
 // into registers a load would touch 32 lines for 1 KiB of codes, and again for the scales, which
-// costs more of the CU's address unit than the products take (142 against 124 us at 4,099 x 2,816 x 4,096).
+// costs more of the CU's address unit than the products take (142 against 124 us at 4,099 x 2,816 x 4,096;
+// now 115, 822 TFLOP/s, matrix units 34 % busy: the conversions of the codes and the fma of the scales take
+// the time, on the same SIMDs).
 //
 // A group's products are summed by themselves and then scaled into the total: exact products, at
 // the price of as many registers again and of an fma for each sum and group.  Rounding scale times
