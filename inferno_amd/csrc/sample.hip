@@ -787,8 +787,10 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
     const int slot = s_a;
     for (int i = tid; i < min(listed, kMaxBand - slot); i += kThreads) parts.band[slot + i] = band[i];
     for (int i = first_group + tid; i < end_group; i += kThreads) parts.sub_sums[i] = sub_sums[i];
+    // All that this workgroup wrote is seen by the one that counts last: each wave's stores have reached the L2
+    // ahead of the barrier, and the release of thread 0 behind it takes them on from there.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    // All that this workgroup wrote is seen by the one that counts last.
     if (tid == 0)
       s_b = __hip_atomic_fetch_add(&parts.rest->done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
             static_cast<uint32_t>(parts.count - 1);

@@ -325,6 +325,29 @@ def test_a_few_rows_that_keep_many_in_a_batch(rows, every):
     _check(z, asked, rng.random(rows), True)
 
 
+def test_parts_of_a_row_meet_the_same_way_every_time():
+    """Rows in eight parts each, call behind call into one workspace, the rows' order changing between them."""
+    import torch
+
+    announce("sample parts again")
+    rng = np.random.default_rng(31)
+    rows, vocab = 16, 100003
+    bits, held = _logits(rng.standard_normal((rows, vocab)), True)
+    asked, u, want = _prepare(held, [(1.0, 0, 0.9, 0.0), (1.0, 0, 1.0, 1e-3)] * (rows // 2), rng.random(rows))
+    z, du = to_dev(bits), to_dev(np.array(u, np.float32))
+    cols = [to_dev(np.array(c, np.int32 if i == 1 else np.float32)) for i, c in enumerate(zip(*asked))]
+    tokens, ws = empty_dev(rows, np.int32), A.sample_workspace(rows, vocab)
+    got = []
+    for i in range(30):
+        order = torch.from_numpy(np.roll(np.arange(rows), i)).to(z.device)
+        one = [t[order].contiguous() for t in (z, du, *cols)]
+        A.dispatch_sample_tokens(one[0], one[1], tokens, ws, num_rows=rows, vocab=vocab, temperature=one[2], top_k=one[3],
+                                 top_p=one[4], min_p=one[5])
+        got.append((i, tokens.clone()))
+    for i, t in got:
+        assert list(from_dev(t, np.int32)) == list(np.roll(want, i)), i
+
+
 def test_calls_at_once_and_graphs_that_share_a_workspace():
     import torch
 
