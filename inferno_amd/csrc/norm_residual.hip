@@ -149,22 +149,23 @@ hipError_t launch_wc(const NormResidualArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int W>
-hipError_t launch_w(const NormResidualArgs& a, hipStream_t stream) {
-  const int64_t c = (a.hidden / 8 + 64 * W - 1) / (64 * W);
-  if (c <= 1) return launch_wc<W, 1>(a, stream);
-  if (c <= 2) return launch_wc<W, 2>(a, stream);
-  if (c <= 4) return launch_wc<W, 4>(a, stream);
-  return launch_wc<W, 8>(a, stream);
-}
-
 }  // namespace
 
+// A wave a row to 1,024 elements, four waves to 8,192, 16 beyond, as few chunks a lane as that takes.  Both
+// sides in us, bf16, both weights, replayed from a graph, one token | 16,384:
+//   512   1 wave 2.3 | 12.0, 4 waves 2.5 | 17.2     1,024   1 wave 2.7 | 21.4, 4 waves 2.5 | 23.0
+//   2,048 1 wave 3.8 | 48.1, 4 waves 2.6 | 42.0     4,096   4 waves 4.1 | 95, 16 waves 3.0 | 112
+//   8,192 4 waves 4.4 | 189, 16 waves 3.7 | 194     16,384  16 waves 4.9 | 397, 4 waves 6.5 | 399
 hipError_t launch_norm_residual(const NormResidualArgs& a, hipStream_t stream) {
   const int64_t chunks = a.hidden / 8;
-  if (chunks <= 64 * 4) return launch_w<1>(a, stream);
-  if (chunks <= 256 * 4) return launch_w<4>(a, stream);
-  return launch_w<16>(a, stream);
+  if (chunks <= 64) return launch_wc<1, 1>(a, stream);
+  if (chunks <= 64 * 2) return launch_wc<1, 2>(a, stream);
+  if (chunks <= 256) return launch_wc<4, 1>(a, stream);
+  if (chunks <= 256 * 2) return launch_wc<4, 2>(a, stream);
+  if (chunks <= 256 * 4) return launch_wc<4, 4>(a, stream);
+  if (chunks <= 1024 * 2) return launch_wc<16, 2>(a, stream);
+  if (chunks <= 1024 * 4) return launch_wc<16, 4>(a, stream);
+  return launch_wc<16, 8>(a, stream);
 }
 
 }  // namespace ifr

@@ -73,6 +73,13 @@ def test_against_64_bits(rows, hidden, gate, f32):
     _check(_case(rows + hidden, rows, hidden, f32, gate))
 
 
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("hidden", [1016, 1024, 1032, 2040, 2048, 2056, 4104, 8184, 8200, 16376, 32768, 32776])
+def test_lengths_on_both_sides_of_each_variant(hidden, f32):
+    announce(f"norm_residual hidden={hidden} f32={f32}")
+    _check(_case(hidden, 6, hidden, f32, "token"))
+
+
 @pytest.mark.parametrize("rows", [1, 70, 1500])
 @pytest.mark.parametrize("post,pre,x,post_norm", [(False, False, True, True), (False, True, True, False), (False, False, False, False),
                                                   (True, False, False, True), (True, False, True, True)])
