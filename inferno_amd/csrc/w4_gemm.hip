@@ -335,7 +335,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, 4) void w4_stream_kernel(W4Args 
   }
 }
 
-// 17 to 64 tokens, and 5 to 16 against many columns: as the stream kernel, with x in units of two steps that go
+// 17 to 64 tokens, and 5 to 16 against many columns or from k past 4,096: as the stream kernel, with x in units of two steps that go
 // from memory into LDS by themselves (global_load_lds), one unit ahead, so that W waves of NT tiles
 // share it behind one barrier a unit.  The codes of a unit are loaded again as soon as the unit
 // before is multiplied, two units ahead of their use.
@@ -788,16 +788,22 @@ Plan plan_of(int64_t M, int64_t N, int64_t K) {
   const int steps = static_cast<int>(K / 128);
   // Past four tokens each workgroup of the first reads all of x (16 x 2,816 x 8,192: 12.3 us against 10.0
   // in spans of k; at 4,096 7.6).
+  // Columns of a workgroup, us at k of 2,816, 16 | 32 | 64: one token x 4,096 4.0 | 5.0 | 6.9, x 8,192 5.7 | 5.5 | 7.4,
+  // x 30,000 16.3 | 12.7 | 14.3; 16 tokens x 4,096 5.9 | 6.9 | 9.1, x 8,192 9.4 | 7.5 | 9.4, x 30,000 29.5 | 23.2 | 19.1.
   if ((M <= 4 || (M <= 16 && K <= 4096)) && N < kManyColumns)
-    return {kFew, N <= 4096 ? 1 : N <= 8192 ? 2 : 4, 16, 1, steps};
+    return {kFew, N <= 4096 ? 1 : M <= 4 || N <= 8192 ? 2 : 4, 16, 1, steps};
   if (M <= 4) return {kStream, kStreamTiles, kStreamWaves, 1, steps};
   if (M <= 64) {
     const bool many = N >= kManyColumns;
     const int nt = M > 16 && M <= 32 && many ? 2 : 1;
     const int waves = !many ? 4 : M <= 32 ? 16 : 8;
     const int64_t blocks = ceil_div(N, 16 * nt * waves);
-    // Spans of an even number of steps, four at least.
-    const int64_t want = std::min<int64_t>(M <= 16 ? ceil_div(352, blocks) : ceil_div(256, blocks), std::min(16, (steps + 3) / 4));
+    // Spans of an even number of steps, six where there are that many, for 512 workgroups.  us in spans for
+    // 256 | 352 | 512: 5 tokens x 8,192 x 8,192 17.5 | 16.1 | 14.6, 64 26.5 | 24.3 | 22.5; 61 x 2,816 x 4,096 in
+    // spans of six steps 12.2, of four 12.9.  (Workgroups of 16 waves have other sums: 5 x 33,000 x 4,096 24.9 us for
+    // 352, 27.7 for 512; of two tiles a wave, 20 tokens, 41.4 for 256 and 38.0 for 512.)
+    const int64_t full = many && M <= 16 ? 352 : 512;
+    const int64_t want = std::min<int64_t>(ceil_div(full, blocks), std::min(16, (steps + 4) / 5));
     const int span = static_cast<int>(ceil_div(ceil_div(steps, want), 2) * 2);
     return {kBatch, nt, waves, static_cast<int>(ceil_div(steps, span)), span};
   }
@@ -805,16 +811,13 @@ Plan plan_of(int64_t M, int64_t N, int64_t K) {
 }
 int64_t part_stride(int64_t M, int64_t N) { return (M * N + 3) / 4 * 4; }
 
-template <int kFmt, int kGroup, int NT, int ST>
+template <int kFmt, int kGroup, int NT, int ST, int R>
 hipError_t launch_few(const W4Args& a, hipStream_t stream) {
   const int cols = NT > 1 ? 16 * NT : static_cast<int>(std::min<int64_t>(16, ceil_div(a.N, 256)));
   const int64_t steps = a.K / 128;
   const dim3 grid(static_cast<unsigned>(ceil_div(a.N, cols)));
   const dim3 block(static_cast<unsigned>(64 * std::min<int64_t>(16, ceil_div(steps, ST))));
-  if (a.M <= 4)
-    hipLaunchKernelGGL((w4_few_kernel<kFmt, kGroup, NT, ST, 1>), grid, block, 0, stream, a, cols);
-  else
-    hipLaunchKernelGGL((w4_few_kernel<kFmt, kGroup, NT, ST, 4>), grid, block, 0, stream, a, cols);
+  hipLaunchKernelGGL((w4_few_kernel<kFmt, kGroup, NT, ST, R>), grid, block, 0, stream, a, cols);
   return hipGetLastError();
 }
 
@@ -876,10 +879,11 @@ template <int kFmt, int kGroup>
 hipError_t launch_group(const W4Args& a, hipStream_t stream) {
   const Plan p = plan_of(a.M, a.N, a.K);
   if (p.kind == kFew) {
-    if (p.nt == 4) return launch_few<kFmt, kGroup, 4, 2>(a, stream);
-    if (p.nt == 2) return launch_few<kFmt, kGroup, 2, 2>(a, stream);
-    if (a.K > 4096) return launch_few<kFmt, kGroup, 1, 4>(a, stream);
-    return launch_few<kFmt, kGroup, 1, 2>(a, stream);
+    if (p.nt == 4) return launch_few<kFmt, kGroup, 4, 2, 4>(a, stream);
+    if (p.nt == 2)
+      return a.M <= 4 ? launch_few<kFmt, kGroup, 2, 2, 1>(a, stream) : launch_few<kFmt, kGroup, 2, 2, 4>(a, stream);
+    if (a.K > 4096) return launch_few<kFmt, kGroup, 1, 4, 1>(a, stream);  // four tokens at most
+    return a.M <= 4 ? launch_few<kFmt, kGroup, 1, 2, 1>(a, stream) : launch_few<kFmt, kGroup, 1, 2, 4>(a, stream);
   }
   if (p.kind == kStream) return launch_stream<kFmt, kGroup>(a, stream);
   if (p.kind == kBatch) {
