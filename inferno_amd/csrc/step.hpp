@@ -20,6 +20,8 @@ struct W4Args {
   int group, format;
 };
 int64_t w4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
+// {kind, tiles, waves, spans of k, steps of a span}, as plan_of in w4_gemm.hip has them.
+void w4_gemm_plan(int64_t M, int64_t N, int64_t K, int64_t* plan);
 hipError_t launch_w4_gemm(const W4Args& a, hipStream_t stream);
 
 struct NormResidualArgs {

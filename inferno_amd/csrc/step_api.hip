@@ -65,6 +65,11 @@ int64_t ifr_w4_gemm_workspace_bytes(int64_t rows, int64_t cols, int64_t seq_len)
   return seq_len == 0 ? 0 : ifr::w4_gemm_workspace_bytes(seq_len, rows, cols);
 }
 
+// Not part of the C API: the launch that a shape takes, for the tests to hold on to.
+void ifr_internal_w4_plan(int64_t rows, int64_t cols, int64_t seq_len, int64_t* plan) {
+  ifr::w4_gemm_plan(seq_len, rows, cols, plan);
+}
+
 int32_t ifr_dispatch_w4_gemm_cols(const void* x, const void* codes, const void* scales,
                                   void* output, int64_t rows, int64_t cols, int64_t seq_len,
                                   int64_t group, int64_t w_format, void* workspace,

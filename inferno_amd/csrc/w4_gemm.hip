@@ -920,6 +920,11 @@ int64_t w4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   return floats * 4;
 }
 
+void w4_gemm_plan(int64_t M, int64_t N, int64_t K, int64_t* plan) {
+  const Plan p = plan_of(M, N, K);
+  plan[0] = p.kind, plan[1] = p.nt, plan[2] = p.waves, plan[3] = p.splits, plan[4] = p.span;
+}
+
 hipError_t launch_w4_gemm(const W4Args& a, hipStream_t stream) {
   return a.format == kW4Int4 ? launch_format<kW4Int4>(a, stream)
                              : launch_format<kW4E2m1>(a, stream);
