@@ -540,7 +540,10 @@ int32_t ifr_norm_residual(const void* y, const void* residual, void* residual_ou
  *   M   = { i in P : w_i >= min_p }
  *   token = the first i of M, by index, with
  *           (sum over j <= i in M of w_j) > u * (sum over M of w)
- * Sums have 64 bits, and the draw does not depend on how the work is cut.  temperature,
+ * Weights and sums have 64 bits, and a row's draw does not depend on the other rows.  In rows
+ * with a limit (top_k, top_p or min_p) a weight is held to 2^-52 of the largest or 2^-56 of the
+ * row's sum, whichever is more: what weighs less is not drawn, and a border between two tokens
+ * is off by less than 2^-31 of the whole.  temperature,
  * top_k, top_p, min_p and uniform hold a number for each row, in device memory; each of the
  * first four may be null.  A temperature of 0, below it or NaN takes the first of the
  * largest logits; top_k <= 0, top_p >= 1 or NaN and min_p <= 0 or NaN are off; top_p <= 0

@@ -8,7 +8,10 @@
 // A draw lands next to a border between two tokens as often as the sums are wrong there: with
 // 2^18 tokens of equal weight f32 sums would give another token in 2 to 3 % of draws.  So the
 // weights and sums have 64 bits (f64 adds run at the rate of f32 ones on this card), and every sum is
-// taken in an order that does not depend on timing.
+// taken in an order that does not depend on timing.  Where atomics add, the weights are integers, of a
+// unit of 2^-51 of the largest or, in the third launch, of at most 2^-55 of the row's sum if that is more
+// (unit_bits): each is off by half a unit, which moves a border by less than 2^-31 of the whole in
+// rows of up to 2^20 tokens, and a weight below half a unit counts as nothing.
 //
 // Three launches.  The first reads every logit once and leaves, for each 64 places, the
 // largest key and, for rows that need it, the sum of weights relative to it.  The second has a
@@ -77,6 +80,13 @@ __device__ __forceinline__ double exp2_neg(double t) {
   p = __builtin_fma(p, f, kTaylor<1>);
   p = __builtin_fma(p, f, 1.0);
   return t > -1000.0 ? __builtin_ldexp(p, static_cast<int>(n)) : 0.0;
+}
+
+// Bits behind the point of the integers that stand for weights of at most 1, of which a row has `sum`, at
+// least 1: their sums stay below 2^62 and half a unit for each.
+__device__ __forceinline__ int unit_bits(double sum) {
+  const int log2_sum = static_cast<int>(__builtin_bit_cast(unsigned long long, sum) >> 52) - 1023;  // rounded down
+  return min(51, 61 - log2_sum);
 }
 
 struct Weights {
@@ -578,8 +588,9 @@ constexpr uint32_t kInfKey = 0xFF800000u;  // of +inf
 
 // What the second launch leaves for the third.
 struct RowRest {
-  double total;  // the sum of the row's weights, if it has one
-  uint32_t top;  // its largest key
+  double total;       // the sum of the row's weights, if it has one
+  uint32_t top;       // its largest key
+  int32_t unit_bits;  // of the integers of its weights
   // Of the parts of a row: parts that are done, entries of the band, the weights above it.
   uint32_t done, listed;
   unsigned long long above;
@@ -908,7 +919,7 @@ __device__ __forceinline__ bool sample_wide(const SampleArgs& a, int64_t row, co
 // left[0]: how many rows are left; left[1 ..]: which, in no order.  Where the grid has several workgroups
 // for each, they take parts of it.
 template <bool kF32>
-__global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a, int shift, RowRest* rest,
+__global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a, RowRest* rest,
                                                                const uint32_t* __restrict__ left,
                                                                unsigned long long* joins, int max_parts,
                                                                int num_subs) {
@@ -927,7 +938,7 @@ __global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a, int
   const RowView<kF32> view(a, row);
   const uint32_t top = rest[row].top;
   const Weights w{top, static_cast<double>(logit_of(top)), asked.rate(),
-                  static_cast<double>(1ull << shift)};
+                  static_cast<double>(1ull << rest[row].unit_bits)};
   unsigned long long* join = joins + static_cast<int64_t>(slot) * (kMaxBand + kMaxSubs);
   const Parts parts{static_cast<int>(num_parts), static_cast<int>(blockIdx.x - slot * num_parts), rest + row, join,
                     join + kMaxBand};
@@ -1078,13 +1089,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
     return;
   }
 
-  auto leave = [&]() {
-    if (tid == 0) {
-      rest[row] = {total, top, 0, 0, 0};
-      left[1 + atomicAdd(&left[0], 1u)] = static_cast<uint32_t>(row);
-    }
-  };
-  if (asked.k > kMaxK) return leave();
+  bool leaves = asked.k > kMaxK;  // to the third launch; block-uniform
   const float zmax = logit_of(top), zlow = logit_of(low);
   const double floor_w = static_cast<double>(asked.min_p);
   const bool by_floor = asked.k == 0 && asked.top_p == 1.0f;
@@ -1095,7 +1100,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
   auto bin_of = [&](uint32_t key) {
     return binned ? min(static_cast<int>((zmax - logit_of(key)) * per), kPickBins - 1) : 0;
   };
-  if (!by_floor) {
+  if (!by_floor && !leaves) {
 #pragma unroll
     for (int j = 0; j < PER; ++j)
       if (sub[j]) atomicAdd(&bins[bin_of(sub[j])], 1u);
@@ -1105,7 +1110,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
   int want = asked.k > 0 ? static_cast<int>(asked.k) : 128;
   // Thread t has the candidates t, t + kPickThreads, ..: (key, lowest index first), weight.
   unsigned long long entry[kEach], weight[kEach];
-  for (;;) {
+  while (!leaves) {
     // A key t0 with `want` sub-chunks or more at or above it, and not many more; 1 (every token that
     // can be drawn) if there are not as many.
     uint32_t t0 = 1;
@@ -1236,7 +1241,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
       __syncthreads();
       fits = s_last <= kMaxTaken;
     }
-    if (!fits) return leave();  // block-uniform
+    if (!fits) {  // block-uniform
+      leaves = true;
+      break;
+    }
     const int n = s_last;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
@@ -1281,13 +1289,30 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
       return goal < 1.0 ? 1ull : static_cast<unsigned long long>(goal);
     });
     if (below) {
-      if (want == kMaxK || guess) return leave();
+      leaves = want == kMaxK || guess;
       want = kMaxK;
       __syncthreads();
       continue;
     }
     keep_from(cut);
     break;
+  }
+  if (leaves) {
+    double most = total;  // the sum of the row's weights, or what it cannot pass
+    if (!asked.needs_sums()) {
+      double mine = 0.0;  // (read again: a rolled loop over them needs no registers)
+#pragma unroll 2
+      for (int s = tid; s < num_subs; s += kPickThreads) {
+        const uint32_t key = subs[row * num_subs + s];
+        mine += key ? kSub * w.real(key) : 0.0;
+      }
+      most = block_inclusive<double>(mine, reinterpret_cast<double*>(waves));
+    }
+    if (tid == kPickThreads - 1) {
+      rest[row] = {total, top, unit_bits(most), 0, 0, 0};
+      left[1 + atomicAdd(&left[0], 1u)] = static_cast<uint32_t>(row);
+    }
+    return;
   }
   if (asked.min_p > 0.0f) {
 #pragma unroll
@@ -1309,13 +1334,6 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
         return min(goal, listed - 1) + 1;
       });
   if (tid == 0) a.tokens[row] = static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(drawn));
-}
-
-// Bits of the integers that stand for weights of at most 1: sums of a row stay below 2^63.
-int weight_shift(int64_t vocab) {
-  int bits = 0;
-  while ((int64_t{1} << bits) < vocab) ++bits;
-  return bits < 11 ? 51 : 62 - bits;
 }
 
 // Workgroups of the third launch: as many as rows, or the 256 CUs with up to eight a row, each of 64
@@ -1362,7 +1380,7 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
   err = hipGetLastError();
   if (err != hipSuccess) return err;
   hipLaunchKernelGGL(sample_rest_kernel<kF32>, dim3(static_cast<unsigned>(rest_blocks(a.rows, a.vocab))),
-                     dim3(kThreads), 0, stream, a, weight_shift(a.vocab), rest, left, joins, parts, subs);
+                     dim3(kThreads), 0, stream, a, rest, left, joins, parts, subs);
   return hipGetLastError();
 }
 
