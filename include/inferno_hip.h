@@ -521,7 +521,8 @@ int32_t ifr_dispatch_w4_gemm_cols(const void* x, const void* codes, const void* 
  * [gate rows][hidden] bf16 with gate_stride 0 for one row for all tokens, else the
  * elements between two tokens' rows (a multiple of 8, hidden or more).  residual_out may
  * be residual, and x_out may be y; otherwise outputs overlap nothing.  hidden: a multiple
- * of 8, up to 65,536; eps > 0.  The sum of a row's squares has to stay in f32's range.
+ * of 8, up to 65,536; seq_len up to 2^24; eps > 0.  The sum of a row's squares has to stay in
+ * f32's range.
  * All pointers 16-byte aligned. */
 #define IFR_RESIDUAL_BF16 0
 #define IFR_RESIDUAL_F32 1

@@ -4,6 +4,8 @@
 //   r' = residual_scale * residual + block_scale * (gate * t)
 //   x  = r' / sqrt(mean(r'^2) + eps) * pre_weight
 // in f32; r' and x are each rounded once, x from the unrounded r'.
+#include <algorithm>
+
 #include "common.hpp"
 #include "step.hpp"
 
@@ -138,15 +140,29 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_residual_kernel(No
   }
 }
 
+// One launch, but for millions of long rows as many as their threads need.
 template <int W, int C>
-hipError_t launch_wc(const NormResidualArgs& a, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(W == 1 ? (a.rows + 3) / 4 : a.rows));
-  const dim3 block(W == 1 ? 256 : 64 * W);
-  if (a.f32)
-    hipLaunchKernelGGL((norm_residual_kernel<W, C, true>), grid, block, 0, stream, a);
-  else
-    hipLaunchKernelGGL((norm_residual_kernel<W, C, false>), grid, block, 0, stream, a);
-  return hipGetLastError();
+hipError_t launch_wc(const NormResidualArgs& all, hipStream_t stream) {
+  constexpr int kThreads = W == 1 ? 256 : 64 * W, kRows = W == 1 ? 4 : 1;  // of a workgroup
+  constexpr int64_t kMaxRows = max_blocks(kThreads) * kRows;
+  for (int64_t row0 = 0; row0 < all.rows; row0 += kMaxRows) {
+    NormResidualArgs a = all;
+    const int64_t at = row0 * a.hidden, res = at * (a.f32 ? 4 : 2);
+    a.rows = std::min(all.rows - row0, kMaxRows);
+    a.y += at;
+    a.residual = static_cast<const char*>(a.residual) + res;
+    a.residual_out = static_cast<char*>(a.residual_out) + res;
+    if (a.x_out) a.x_out += at;
+    if (a.gate) a.gate += row0 * a.gate_stride;
+    const dim3 grid(static_cast<unsigned>((a.rows + kRows - 1) / kRows));
+    if (a.f32)
+      hipLaunchKernelGGL((norm_residual_kernel<W, C, true>), grid, dim3(kThreads), 0, stream, a);
+    else
+      hipLaunchKernelGGL((norm_residual_kernel<W, C, false>), grid, dim3(kThreads), 0, stream, a);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  return hipSuccess;
 }
 
 }  // namespace

@@ -7,6 +7,9 @@
 
 namespace ifr {
 
+// Workgroups of a launch, whose grid has less than 2^32 threads.
+constexpr int64_t max_blocks(int threads) { return ((int64_t{1} << 32) - 1) / threads; }
+
 constexpr int kW4Int4 = 1;  // IFR_W4_INT4
 constexpr int kW4E2m1 = 2;  // IFR_W4_E2M1
 
