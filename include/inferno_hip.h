@@ -552,7 +552,8 @@ int32_t ifr_norm_residual(const void* y, const void* residual, void* residual_ou
  * inside, NaN as 0.  Logits of -inf and NaN are never drawn; a row of nothing else gives -1.
  * Logits of +inf share the draw.
  * logits [num_rows][row_stride] of logits_type, of which vocab (1 to 2^20) are read;
- * num_rows up to 2^20.  workspace: device memory of ifr_sample_workspace_bytes, 16-byte
+ * num_rows up to 2^20, and num_rows * vocab up to 2^35 (past that a call is refused that has
+ * 2^24 pieces of 16 KiB of logits or more, each row's its own).  workspace: device memory of ifr_sample_workspace_bytes, 16-byte
  * aligned (0: null will do; that of num_rows does for all below it), written before it is
  * read in every call; calls that may overlap each need their own. */
 #define IFR_LOGITS_BF16 0

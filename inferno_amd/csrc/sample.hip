@@ -262,7 +262,6 @@ struct RowView {
 };
 
 constexpr int kSub = 64;             // places of a sub-chunk
-constexpr int kScanThreads = 256;
 constexpr int kScanVectors = 4;      // of a thread
 
 // subs[row][s]: the largest key of sub-chunk s; sums[row][s]: its weights relative to that key.
@@ -1361,10 +1360,9 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
   unsigned long long* joins = reinterpret_cast<unsigned long long*>(rest + a.rows);
   uint32_t* left = reinterpret_cast<uint32_t*>(joins + join_longs(a.rows, a.vocab));
   uint32_t* tops = left + 1 + a.rows;
-  constexpr int kChunk = kScanThreads * kScanVectors * RowView<kF32>::kPer;
-  const int chunks = (subs * kSub + kChunk - 1) / kChunk;
-  hipLaunchKernelGGL(sample_scan_kernel<kF32>, dim3(static_cast<unsigned>(a.rows * chunks)),
-                     dim3(kScanThreads), 0, stream, a, tops, sums, left, subs, chunks);
+  const int64_t blocks = sample_scan_blocks(a.rows, a.vocab, kF32);
+  hipLaunchKernelGGL(sample_scan_kernel<kF32>, dim3(static_cast<unsigned>(blocks)), dim3(kScanThreads), 0, stream,
+                     a, tops, sums, left, subs, static_cast<int>(blocks / a.rows));
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   const dim3 grid(static_cast<unsigned>(a.rows));
@@ -1389,6 +1387,12 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
 int64_t sample_workspace_bytes(int64_t rows, int64_t vocab) {
   return (rows * (sub_chunks(vocab) * 12 + static_cast<int64_t>(sizeof(RowRest)) + 4) + 4 +
           join_longs(rows, vocab) * 8 + 15) / 16 * 16;
+}
+
+// Each row has workgroups of its own, of 16 KiB of logits each.
+int64_t sample_scan_blocks(int64_t rows, int64_t vocab, bool f32) {
+  const int64_t chunk = kScanThreads * kScanVectors * (f32 ? RowView<true>::kPer : RowView<false>::kPer);
+  return rows * ((sub_chunks(vocab) * kSub + chunk - 1) / chunk);
 }
 
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {

@@ -55,6 +55,9 @@ struct SampleArgs {
   void* workspace;
 };
 int64_t sample_workspace_bytes(int64_t rows, int64_t vocab);
+// Workgroups of the first launch.
+int64_t sample_scan_blocks(int64_t rows, int64_t vocab, bool f32);
+constexpr int kScanThreads = 256;
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream);
 
 }  // namespace ifr

@@ -170,6 +170,8 @@ int32_t ifr_dispatch_sample_tokens(const void* logits, const float* uniform, int
   const int64_t need = ifr::sample_workspace_bytes(num_rows, vocab);
   if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
     return fail(IFR_ESPACE, "workspace needs %lld bytes, 16-byte aligned", (long long)need);
+  if (ifr::sample_scan_blocks(num_rows, vocab, logits_type == IFR_LOGITS_F32) > ifr::max_blocks(ifr::kScanThreads))
+    return fail(IFR_EINVAL, "the rows have 2^24 pieces of 16 KiB of logits or more");
   const Span out{tokens, 4 * num_rows}, space{need > 0 ? workspace : nullptr, need};
   const int64_t size = logits_type == IFR_LOGITS_F32 ? 4 : 2;
   for (const Span in : {Span{logits, size * ((num_rows - 1) * row_stride + vocab)}, Span{uniform, 4 * num_rows},
