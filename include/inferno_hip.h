@@ -497,7 +497,8 @@ int32_t ifr_kv8_attention(const void* image_dev, const int64_t* info, const void
  * Sums are f32, and nothing is rounded before the output; their order depends on
  * seq_len.  A token's results depend on its own x alone, so infinities and NaN stay in
  * their token.
- * group 32, 64 or 128; cols a multiple of 128; any rows.  All pointers 16-byte aligned.
+ * group 32, 64 or 128; cols a multiple of 128, up to 2^20; rows up to 2^24; seq_len up to
+ * 2^19.  All pointers 16-byte aligned.
  * workspace: device memory of ifr_w4_gemm_workspace_bytes (0: null will do; that of a
  * seq_len does for all below it), written before it is read in every call; calls that may
  * overlap each need their own. */
