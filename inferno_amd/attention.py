@@ -16,15 +16,20 @@ from .kv import (FULL, SLIDING, AttentionPlan, KVRunTable, WindowPlan,
                  flash_partial_stride)
 
 
-def _stream() -> int:
-    """The current HIP stream of the current device (torch's capture stream
+def _device_stream() -> tuple[int, int]:
+    """The current device and its current HIP stream (torch's capture stream
     under graph capture), as the raw handle the C ABI takes."""
     import torch
 
+    device = torch.cuda.current_device()
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     if raw is not None:
-        return int(raw(torch.cuda.current_device()))
-    return int(torch.cuda.current_stream().cuda_stream)
+        return device, int(raw(device))
+    return device, int(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _stream() -> int:
+    return _device_stream()[1]
 
 
 def _ptr(t) -> int:
@@ -440,14 +445,6 @@ def _kinds() -> dict[str, frozenset]:
                       byte=frozenset((torch.uint8, torch.int8)),
                       f32=frozenset((torch.float32,)), i32=frozenset((torch.int32,)))
     return _KINDS
-
-
-def _device_stream() -> tuple[int, int]:
-    """The current device and its current stream."""
-    import torch
-
-    device = torch.cuda.current_device()
-    return device, int(torch._C._cuda_getCurrentRawStream(device))
 
 
 def _tensor(device: int, name: str, t, numel: int, kind: frozenset) -> int:
