@@ -549,7 +549,7 @@ int32_t ifr_norm_residual(const void* y, const void* residual, void* residual_ou
  * top_k, top_p, min_p and uniform hold a number for each row, in device memory; each of the
  * first four may be null.  A temperature of 0, below it or NaN takes the first of the
  * largest logits; top_k <= 0, top_p >= 1 or NaN and min_p <= 0 or NaN are off; top_p <= 0
- * keeps one token, min_p >= 1 the largest logits.  u outside [0, 1) counts as the nearest
+ * keeps one token, min_p >= 1 the largest logits alone.  u outside [0, 1) counts as the nearest
  * inside, NaN as 0.  Logits of -inf and NaN are never drawn; a row of nothing else gives -1.
  * Logits of +inf share the draw.
  * logits [num_rows][row_stride] of logits_type, of which vocab (1 to 2^20) are read;

@@ -184,6 +184,7 @@ struct Asked {
     if (!(top_p > 0.0f)) top_p = 0.0f;
     min_p = a.min_p ? a.min_p[row] : 0.0f;
     if (!(min_p > 0.0f)) min_p = 0.0f;
+    if (min_p >= 1.0f) min_p = 2.0f;  // the largest alone: a weight next to 1 rounds to 1
   }
   __device__ __forceinline__ double rate() const {
     return t > 0.0f ? kLog2E / static_cast<double>(t) : kLog2E;
