@@ -1252,12 +1252,28 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(
       const int i = tid + kPickThreads * j;
       entry[j] = i < n ? cand[i] : 0;
     }
-    // Bins of the logits from the largest down to t0.
-    const float t0_per = static_cast<float>(kPickBins - 1) / (zmax - logit_of(t0));
-    const bool t0_binned = t0 > 1 && t0_per > 0.0f && t0_per < 1e30f;
+    // Bins of the candidates' logits, from the largest down to t0.  Without a t0, where every token of a vocabulary of
+    // up to 2,048 is one, down to the smallest, or bins of the keys if that lies far below (a mask of the type's
+    // lowest value): the entries of a bin are compared with each other, and 1,000 of them in one bin took 150 us.
+    uint32_t bottom = t0;
+    if (t0 == 1) {  // block-uniform
+      bottom = top;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (entry[j]) bottom = min(bottom, static_cast<uint32_t>(entry[j] >> 32));
+      if (tid == 0) s_key = top;
+      __syncthreads();
+      atomicMin(&s_key, bottom);
+      __syncthreads();
+      bottom = s_key;
+    }
+    const float range = zmax - logit_of(bottom), per_logit = static_cast<float>(kPickBins - 1) / range;
+    const bool linear = per_logit > 0.0f && per_logit < 1e30f && (t0 > 1 || range * w.rate < 256.0);
+    const int key_shift = max(0, 22 - __builtin_clz((top - bottom) | 1u));  // to 1,024 bins
     auto entry_bin = [&](int j) {
-      const float z = logit_of(static_cast<uint32_t>(entry[j] >> 32));
-      return t0_binned ? min(static_cast<int>((zmax - z) * t0_per), kPickBins - 1) : 0;
+      const uint32_t key = static_cast<uint32_t>(entry[j] >> 32);
+      return linear ? min(static_cast<int>((zmax - logit_of(key)) * per_logit), kPickBins - 1)
+                    : static_cast<int>((top - key) >> key_shift);
     };
     auto keep_from = [&](unsigned long long cut) {
 #pragma unroll
