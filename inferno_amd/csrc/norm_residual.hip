@@ -61,9 +61,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_residual_kernel(No
   constexpr bool kAhead = C <= 4;
   uint4 y[C], g[kAhead ? C : 1], pw[kAhead ? C : 1], qw[kAhead ? C : 1];
   float r[C][8];
-  const uint4* gates = a.gate ? reinterpret_cast<const uint4*>(a.gate + row * a.gate_stride) : nullptr;
-  const uint4* posts = reinterpret_cast<const uint4*>(a.post_weight);
-  const uint4* pres = reinterpret_cast<const uint4*>(a.pre_weight);
+  auto gate_at = [&](int at) { return reinterpret_cast<const uint4*>(a.gate + row * a.gate_stride)[at]; };
+  auto post_at = [&](int at) { return reinterpret_cast<const uint4*>(a.post_weight)[at]; };
+  auto pre_at = [&](int at) { return reinterpret_cast<const uint4*>(a.pre_weight)[at]; };
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int at = c * kRowThreads + t;
@@ -80,9 +80,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_residual_kernel(No
                                                row * hidden)[at], r[c]);
       }
       if constexpr (kAhead) {
-        if (a.gate) g[c] = gates[at];
-        if (a.post_weight) pw[c] = posts[at];
-        if (a.pre_weight) qw[c] = pres[at];
+        if (a.gate) g[c] = gate_at(at);
+        if (a.post_weight) pw[c] = post_at(at);
+        if (a.pre_weight) qw[c] = pre_at(at);
       }
     }
   }
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_residual_kernel(No
     float v[8], w[8];
     unpack8(y[c], v);
     if (a.post_weight) {
-      unpack8(kAhead ? pw[kAhead ? c : 0] : posts[at], w);
+      unpack8(kAhead ? pw[kAhead ? c : 0] : post_at(at), w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
     } else {
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_residual_kernel(No
       for (int i = 0; i < 8; ++i) v[i] = v[i] * inv;
     }
     if (a.gate) {
-      unpack8(kAhead ? g[kAhead ? c : 0] : gates[at], w);
+      unpack8(kAhead ? g[kAhead ? c : 0] : gate_at(at), w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = v[i] * w[i];
     }
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_residual_kernel(No
     const int at = c * kRowThreads + again;
     if (at >= chunks) continue;
     float v[8], w[8];
-    if (a.pre_weight) unpack8(kAhead ? qw[kAhead ? c : 0] : pres[at], w);
+    if (a.pre_weight) unpack8(kAhead ? qw[kAhead ? c : 0] : pre_at(at), w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = a.pre_weight ? r[c][i] * inv * w[i] : r[c][i] * inv;
     reinterpret_cast<uint4*>(a.x_out + row * hidden)[at] = pack8(v);
