@@ -968,7 +968,7 @@ __device__ __forceinline__ int first_thread(bool holds, bool or_else, int* first
 // A chain of short steps, each behind a barrier, and of two reads of memory: for one row of 2^18 f32 logits
 // under a top-k of 64 and a top-p the largest keys take 2.2 us, a threshold 3.5, listing and reading the
 // candidates 4.4, the three histograms of them 6.  512 threads; a row of which 1,024 sub-chunks are read takes
-// about 16 us more.  With 33 sub-chunks a thread (vocabularies past 294,905) up to 312 B a lane lie in scratch
+// about 16 us more.  With 33 sub-chunks a thread (vocabularies past 294,905) up to 324 B a lane lie in scratch
 // memory: a call for one row of 294,000 | 295,500 takes 21.4 | 26.3 us as above, 24.2 | 37.6 under a top-p alone.
 template <bool kF32, int PER>
 __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(

@@ -749,14 +749,15 @@ struct Plan {
 };
 
 // From 32,768 columns there are 128 workgroups of 256 columns or more, and the kernels that
-// stream them.
+// stream them.  us for one token, columns over waves | streams: k of 2,816, int4 in groups of 128, 32,768 columns 15.9 | 17.8,
+// 50,257 23.8 | 19.6, 128,256 51.6 | 38.2; k of 4,096 25.5 | 23.0, 41.7 | 24.1, 93.3 | 51.0.
 constexpr int64_t kManyColumns = 32768;
 
 // Tokens of a tile and spans of k past 64 tokens: the cheapest by a model of the launch, fitted to 65
-// to 1,024 tokens, both tiles and 1 to 16 spans at N = 2,816, K = 4,096, int4 in groups of 128: 32
+// to 1,024 tokens, both tiles and 1 to 16 spans at N = 2,816, K = 4,096, int4 in groups of 128 alone: 32
 // steps of up to 256 tiles take 33 us (64 tokens) or 45 (128), of each 256 of more tiles, of which a CU
 // has several at once, 23 or 43; spans add a launch and the partial sums' way out and back.
-// It picks the best measured or one within 12 % of it: 65 tokens 15.1 us (best 13.4), 256 20.4
+// It picks the best measured or one within 13 % of it: 65 tokens 15.1 us (best 13.4), 256 20.4
 // (19.6), 512 28.0 (28.0; one span of 128 tokens 48.3), 1,024 43.4 (43.4).
 // Spans only up to 768 workgroups, which bounds the workspace for every M.
 constexpr int kTileSpans = 16;
