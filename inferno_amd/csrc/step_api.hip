@@ -66,8 +66,10 @@ int64_t ifr_w4_gemm_workspace_bytes(int64_t rows, int64_t cols, int64_t seq_len)
 }
 
 // Not part of the C API: the launch that a shape takes, for the tests to hold on to.
-void ifr_internal_w4_plan(int64_t rows, int64_t cols, int64_t seq_len, int64_t* plan) {
+int32_t ifr_internal_w4_plan(int64_t rows, int64_t cols, int64_t seq_len, int64_t* plan) {
+  if (!w4_shape(rows, cols, seq_len) || seq_len == 0) return fail(IFR_EINVAL, "bad w4_gemm_cols shape");
   ifr::w4_gemm_plan(seq_len, rows, cols, plan);
+  return ifr::abi_ok();
 }
 
 int32_t ifr_dispatch_w4_gemm_cols(const void* x, const void* codes, const void* scales,

@@ -9,6 +9,10 @@ def test_the_plan_of_a_shape(shape):
     assert plan(*shape) == PLANS[shape]
 
 
+def test_a_shape_that_is_refused_has_no_plan():
+    assert [plan(*s) for s in ((0, 16, 128), (1, 0, 128), (1, 16, 100), (1 << 20, 16, 128))] == [None] * 4
+
+
 def test_every_kernel_is_run():
     few, batch, long_batch, tile = set(), set(), set(), set()
     for (m, _, k), (kind, nt, waves, splits, span) in PLANS.items():

@@ -32,7 +32,6 @@ def plan(tokens, rows, cols):
     from inferno_amd._lib import I64, P_I64, lib
 
     fn = lib().ifr_internal_w4_plan
-    fn.restype, fn.argtypes = None, [I64, I64, I64, P_I64]
+    fn.restype, fn.argtypes = C.c_int32, [I64, I64, I64, P_I64]
     out = (C.c_int64 * 5)()
-    fn(rows, cols, tokens, out)
-    return tuple(out)
+    return tuple(out) if fn(rows, cols, tokens, out) == 0 else None
